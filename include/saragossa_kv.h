@@ -36,6 +36,7 @@ extern "C" {
 
 #define SKV_DTYPE_F32 0  /* GpuElement::F32: rows kept as they arrive */
 #define SKV_DTYPE_BF16 1 /* GpuElement::Bf16 */
+#define SKV_DTYPE_FP4 2  /* codes of 4 bits, a power of two per 32 dims (no counterpart in the reference) */
 
 #define SKV_PAGE_ROWS 16
 

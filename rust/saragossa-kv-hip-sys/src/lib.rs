@@ -27,6 +27,7 @@ pub const SKV_ERR_DEVICE: i32 = 3;
 pub const SKV_ERR_MEMORY: i32 = 4;
 pub const SKV_DTYPE_F32: i32 = 0;
 pub const SKV_DTYPE_BF16: i32 = 1;
+pub const SKV_DTYPE_FP4: i32 = 2;
 pub const SKV_PAGE_ROWS: usize = 16;
 pub const SKV_STATIC_SCRATCH_BYTES: usize = 8 << 20;
 

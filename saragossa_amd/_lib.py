@@ -8,7 +8,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = os.path.join(_HERE, "libsaragossa_kv.so")
 
 OK, ERR_DIMENSION, ERR_CONFIG, ERR_DEVICE, ERR_MEMORY = 0, 1, 2, 3, 4
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_FP4 = 0, 1, 2
 PAGE_ROWS = 16
 
 

@@ -2,6 +2,7 @@
 // to rows, and the plain three-phase attention kernel kept behind the
 // RETI_RUST_FLASH_SDPA kill-switch.
 #include "append_tile.h"
+#include "fp4_tile.h"
 
 namespace skv {
 
@@ -23,6 +24,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
     if (a.n_rows <= 0) return hipSuccess;
+    if (a.g.fp4) return launch_store_fp4(a, s);
     const AppendArgs b = append_placed(a);
     const AppendGrid r = append_grid(a);
     const int units = a.g.tile_elems >> 3, per = r.spread ? 1 : r.rounds;
@@ -155,6 +157,7 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
 }
 
 hipError_t launch_gather(const GatherArgs &a, hipStream_t s) {
+    if (a.g.fp4) return launch_load_fp4(a, s);
     const int groups = (a.g.head_dim + 7) >> 3;
     const long total = (long)a.g.kv_heads * groups * a.n_rows;
     if (total <= 0) return hipSuccess;
@@ -171,6 +174,19 @@ hipError_t launch_gather(const GatherArgs &a, hipStream_t s) {
 // attention_decode_naive_bf16 (src/decode_resident/kernels.rs:90-164) behind
 // RETI_RUST_FLASH_SDPA=0 and serves as an independent check of the matrix-core kernel.
 // ------------------------------------------------------------------------------------
+// Element (row r, dim d) of a kv head's tile of K or of V, of any element type.
+__device__ __forceinline__ float naive_value(const uint16_t *pool, const Geom &g, int page, int kvh, int r, int d, bool v) {
+    if (g.fp4) {
+        const int P = g.P;
+        const uint32_t code = fp4_codes(pool, g, page, kvh)[v ? v4_code(P, r, d) : k4_code(r, d)] >> (v ? (d >> 4 & 1) * 4 : (d & 1) * 4);
+        const uint32_t power = fp4_powers(pool, g, page, kvh)[v ? v4_power(P, r, d >> 5) : k4_power(P, r, d >> 5)];
+        return __uint_as_float(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, __uint_as_float(power << 23), 0)) << 16);
+    }
+    const uint16_t *t = pool + (long)page * g.page_elems + (long)kvh * g.tile_elems;
+    if (g.f32) return reinterpret_cast<const float *>(t)[v ? v_index_f32(r, d) : k_index_f32(r, d)];
+    return bf16_to_f32(t[v ? v_index(g.P, r, d) : k_index(g.P, r, d)]);
+}
+
 __global__ __launch_bounds__(256) void naive_kernel(NaiveArgs a) {
     // the __f*_rn intrinsics are plain operators here: without this they fuse into FMAs
 #pragma clang fp contract(off)
@@ -188,11 +204,9 @@ __global__ __launch_bounds__(256) void naive_kernel(NaiveArgs a) {
         const long slot = slot_of(a.window_start + i, g.ring_rows);
         const int page = a.table[slot >> 4];
         const int r = (int)(slot & 15);
-        const uint16_t *kt = a.k_pool + (long)page * g.page_elems + (long)kvh * g.tile_elems;
-        const float *ktf = reinterpret_cast<const float *>(kt);
         float dot = 0.0f;
         for (int d = 0; d < g.head_dim; ++d)
-            dot = __fadd_rn(dot, __fmul_rn(q[d], g.f32 ? ktf[k_index_f32(r, d)] : bf16_to_f32(kt[k_index(g.P, r, d)])));
+            dot = __fadd_rn(dot, __fmul_rn(q[d], naive_value(a.k_pool, g, page, kvh, r, d, false)));
         const float sc = __fmul_rn(dot, a.inv_scale);
         scores[i] = sc;
         mx = fmaxf(mx, sc);
@@ -225,9 +239,8 @@ __global__ __launch_bounds__(256) void naive_kernel(NaiveArgs a) {
             const long slot = slot_of(a.window_start + i, g.ring_rows);
             const int page = a.table[slot >> 4];
             const int r = (int)(slot & 15);
-            const uint16_t *vt = a.v_pool + (long)page * g.page_elems + (long)kvh * g.tile_elems;
             const float pr = uniform ? 1.0f / (float)nkeys : scores[i] / sum;
-            const float val = g.f32 ? reinterpret_cast<const float *>(vt)[v_index_f32(r, d)] : bf16_to_f32(vt[v_index(g.P, r, d)]);
+            const float val = naive_value(a.v_pool, g, page, kvh, r, d, true);
             acc = __fadd_rn(acc, __fmul_rn(pr, val));
         }
         a.out[(long)h * g.head_dim + d] = acc;

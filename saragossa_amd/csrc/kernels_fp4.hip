@@ -1,0 +1,563 @@
+// gfx950 kernels of the 4-bit element (fp4_tile.h): rows stored as codes, read back, and attended.
+#include "append_tile.h"
+#include "fp4_tile.h"
+
+namespace skv {
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float float4_t;
+typedef __attribute__((ext_vector_type(16))) float float16_t;
+typedef __attribute__((ext_vector_type(32))) float float32_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u2;
+typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+typedef __attribute__((ext_vector_type(6))) uint32_t u6;
+typedef __attribute__((ext_vector_type(8))) int int8v_t;
+
+namespace {
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Byte B of two codes as two bf16 values, the low nibble's in the low half; `power` has the group's byte in its exponent field (the rest of
+// it is not looked at)
+template <int B>
+__device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(power), B));
+}
+
+// 32 values as e2m3 codes of x / scale, and the codes' values. These conversions take several passes and write their results as they go: a result
+// register that is also an operand is read back changed (seen: the scale in the first result register, the values after the first few wrong),
+// and the compiler does not know. Operands are kept alive behind the instruction, so that they have registers of their own.
+__device__ __forceinline__ u6 to_fp6(const float (&x)[32], float scale) {
+    float16_t even, odd; // they take turns in the result
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        even[e] = x[2 * e];
+        odd[e] = x[2 * e + 1];
+    }
+    u6 codes = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
+    asm volatile("" : "+v"(codes) : "v"(even), "v"(odd), "v"(scale));
+    return codes;
+}
+__device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
+    float32_t x = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(codes, scale);
+    asm volatile("" : "+v"(x) : "v"(codes), "v"(scale));
+    return x;
+}
+
+} // namespace
+
+// ------------------------------------------------------------------------------------
+// Rows stored: f32 rows -> codes and powers. Eight neighbouring lanes take a group of a row, four dims each (128 bytes side by side), find
+// its largest magnitude among themselves and convert. K: the eight's 16 bits are the lane's 16 bytes of the matrix operand as they stand. V: a
+// byte holds the dims c and c + 16, which lanes four apart exchange, and a word the byte of four rows, which lanes eight apart
+// exchange; a quad of rows that the batch covers is stored as words, one that it shares with older rows as bytes.
+// A workgroup takes 256 such eighths of one (page, kv head) of K or V.
+// ------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void store_fp4_kernel(AppendArgs a) {
+    const Geom g = a.g;
+    const int groups = g.P >> 5, parts = (groups + 1) >> 1;
+    const bool is_v = (int)blockIdx.z >= parts;
+    const int part = (int)blockIdx.z - (is_v ? parts : 0), kvh = blockIdx.y;
+    int logical = a.first_page + (int)blockIdx.x;
+    if (a.ring_pages > 0 && logical >= a.ring_pages) logical -= a.ring_pages;
+    const int page = a.table ? a.table[logical] : logical;
+    const int row0 = (int)blockIdx.x * 16 - a.first_row; // batch row of the page's first row
+    const int r_lo = max(-row0, 0), r_hi = min(16, a.n_rows - row0); // rows of the page in the batch
+
+    const int lane = threadIdx.x & 63, o = threadIdx.x & 7, i = (threadIdx.x >> 3) & 3;
+    const int rest = (int)(threadIdx.x >> 5) + part * 8, quad = rest & 3, grp = rest >> 2;
+    const int r = quad * 4 + i, d = grp * 32 + o * 4;
+    const int row = min(max(r, r_lo), r_hi - 1); // clamped: every lane takes part in the exchanges
+    const int kv_dim = g.kv_heads * g.head_dim;
+    const float *src = (is_v ? a.v_src : a.k_src) + (long)(row0 + row) * kv_dim + kvh * g.head_dim;
+    float x[4];
+    if (a.vec) { // uniform
+        const float4_t v = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = d < g.head_dim ? v[e] : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = src[min(d + e, g.head_dim - 1)];
+            x[e] = d + e < g.head_dim ? v : 0.0f;
+        }
+    }
+    uint32_t power;
+    const uint32_t codes = fp4_codes_of(x, power);
+    const bool real = grp < groups; // (an odd number of groups fills half of its last workgroup)
+    const bool in = real && r >= r_lo && r < r_hi;
+    uint16_t *pool = is_v ? a.v_pool : a.k_pool;
+    uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
+    if (!is_v) { // uniform
+        if (in) {
+            *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
+            if (o == 0) pp[k4_power(g.P, r, grp)] = (uint8_t)power;
+        }
+        return;
+    }
+    const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
+    const uint32_t low = o < 4 ? codes : other, high = o < 4 ? other : codes;
+    const uint32_t mine = nibbles_apart(low) | nibbles_apart(high) << 4; // dims 4 (o % 4) .. of the row, each with the one 16 further
+    uint32_t word = 0; // column 4 (o % 4) + i: byte q is row q of the quad
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t of_row = (uint32_t)__shfl((int)mine, (lane & ~24) | q << 3);
+        word |= (of_row >> (8 * i) & 255u) << (8 * q);
+    }
+    if (in && o == 0) pp[v4_power(g.P, r, grp)] = (uint8_t)power;
+    if (o >= 4 || !real) return;
+    uint8_t *dst = cp + v4_code(g.P, quad * 4, grp * 32 + o * 4 + i);
+    if (quad * 4 >= r_lo && quad * 4 + 4 <= r_hi) {
+        *reinterpret_cast<uint32_t *>(dst) = word;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (quad * 4 + q >= r_lo && quad * 4 + q < r_hi) dst[q] = (uint8_t)(word >> (8 * q));
+    }
+}
+
+hipError_t launch_store_fp4(const AppendArgs &a, hipStream_t s) {
+    if (a.n_rows <= 0) return hipSuccess;
+    AppendArgs b = append_placed(a);
+    b.vec = b.vec && ((uintptr_t)a.v_src & 15) == 0;
+    const long pages = (a.first_pos + a.n_rows + 15) / 16 - a.first_pos / 16;
+    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(2 * ((a.g.P / 32 + 1) / 2)));
+    hipLaunchKernelGGL(store_fp4_kernel, grid, dim3(256), 0, s, b);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------
+// Rows read back as bf16, which holds every value exactly: the store's steps the other way round, with the same division of the work.
+// ------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void load_fp4_kernel(GatherArgs a, int vec) {
+    const Geom g = a.g;
+    const int groups = g.P >> 5, parts = (groups + 1) >> 1;
+    const bool is_v = (int)blockIdx.z >= parts;
+    const int part = (int)blockIdx.z - (is_v ? parts : 0), kvh = blockIdx.y;
+    uint16_t *out = is_v ? a.v_dst : a.k_dst;
+    if (!out) return;
+    const long pos0 = (a.first_pos / 16 + blockIdx.x) * 16;
+    const int page = a.table[slot_of(pos0, g.ring_rows) >> 4];
+    const int lane = threadIdx.x & 63, o = threadIdx.x & 7, i = (threadIdx.x >> 3) & 3;
+    const int rest = (int)(threadIdx.x >> 5) + part * 8, quad = rest & 3, grp = min(rest >> 2, groups - 1);
+    const int r = quad * 4 + i, d = grp * 32 + o * 4;
+    const uint8_t *cp = fp4_codes(is_v ? a.v_pool : a.k_pool, g, page, kvh), *pp = fp4_powers(is_v ? a.v_pool : a.k_pool, g, page, kvh);
+    const uint32_t power = (uint32_t)pp[is_v ? v4_power(g.P, r, grp) : k4_power(g.P, r, grp)] << 23;
+    uint32_t codes = 0;
+    if (is_v) { // uniform
+        const uint32_t word = *reinterpret_cast<const uint32_t *>(cp + v4_code(g.P, quad * 4, grp * 32 + (o & 3) * 4 + i));
+        const int half = o < 4 ? 0 : 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t col = (uint32_t)__shfl((int)word, (lane & ~24) | k << 3);
+            codes |= (col >> (8 * i + half) & 15u) << (4 * k);
+        }
+    } else {
+        codes = *reinterpret_cast<const uint16_t *>(cp + k4_code(r, d));
+    }
+    const long row = pos0 + r - a.first_pos;
+    if (rest >> 2 >= groups || row < 0 || row >= a.n_rows || d >= g.head_dim) return;
+    const uint32_t v[2] = {code_pair<0>(codes, power), code_pair<1>(codes, power)};
+    uint16_t *dst = out + row * g.kv_heads * g.head_dim + kvh * g.head_dim + d;
+    if (vec) { // uniform
+        *reinterpret_cast<u2 *>(dst) = u2{v[0], v[1]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < g.head_dim) dst[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+    }
+}
+
+hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
+    if (a.n_rows <= 0) return hipSuccess;
+    const int vec = a.g.head_dim % 4 == 0 && (((uintptr_t)a.k_dst | (uintptr_t)a.v_dst) & 7) == 0;
+    const long pages = (a.first_pos + a.n_rows + 15) / 16 - a.first_pos / 16;
+    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(2 * ((a.g.P / 32 + 1) / 2)));
+    hipLaunchKernelGGL(load_fp4_kernel, grid, dim3(256), 0, s, a, vec);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------
+// Attention over the codes: 16 query slots (row, head of the group) of one kv head against a range of the pages, as (o, m, l) or, unsplit, the
+// context. The wavefronts of a workgroup hold the same slots and walk the page pairs in turn.
+//
+// S^T = K . Q^T takes the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4 with K as e2m1 (a lane's 16 bytes are a row's 32 dims of
+// a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as four terms in e2m3 with a power a group and term.
+// A term leaves at most 2^-3, then 2^-7, 2^-12, 2^-17 of the group's power, 2^-19 of its largest value: what two
+// bf16 terms leave of each value. Four such products of 128 dims take 64 cycles, two of bf16 (eight instructions of 32 dims) 128, and
+// the codes would have to be converted.
+// O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to bf16 (exact) in registers, per page and group of dims
+// four conversions, four scales and four byte selections for eight values a lane, and P is two bf16 terms; a pair of pages is the 32 keys of
+// v_mfma_f32_16x16x32_bf16.
+// ------------------------------------------------------------------------------------
+template <int P>
+struct Fp4Tile {
+    static constexpr int G = P / 32, U = fp4_quad(P), NB = (P + 127) / 128, VL = G / U;
+};
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t *p) {
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) {
+        const u4 v = *reinterpret_cast<const u4 *>(p + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+    }
+    if constexpr (N == 3) { // (12 bytes apart: words)
+        typedef __attribute__((ext_vector_type(3), aligned(4))) uint32_t u3;
+        const u3 v = *reinterpret_cast<const u3 *>(p);
+        x[0] = v[0], x[1] = v[1], x[2] = v[2];
+    } else if constexpr (N == 2) {
+        const u2 v = *reinterpret_cast<const u2 *>(p);
+        x[0] = v[0], x[1] = v[1];
+    } else if constexpr (N == 1) {
+        x[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+// 255 in the bytes of w that are
+__device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
+    const uint32_t x = ~w, zero = ~(((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x | 0x7f7f7f7fu); // the top bit of the bytes of x that are 0
+    return (zero >> 7) * 255u;
+}
+
+// LDS: [NB][4 terms][6 words][64 lanes] of the queries, [NB][64] their powers, then the wavefronts' states
+template <int P, int WAVES>
+struct Fp4Lds {
+    static constexpr int NB = Fp4Tile<P>::NB, QUERIES = NB * 4 * 6 * 64, POWERS = NB * 64;
+    static constexpr size_t bytes(int rows) { return ((size_t)(QUERIES + POWERS) + (size_t)WAVES * rows * (P + 4 + 2)) * 4; }
+};
+
+template <int P, int WAVES, bool MQ, bool RING>
+__device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const ChunkPages *c, const int split, const int kvh, const int tile_z) {
+    using T = Fp4Tile<P>;
+    constexpr int THREADS = WAVES * 64, G = T::G, U = T::U, NB = T::NB, VL = T::VL, NT = P / 16, OSTRIDE = P + 4;
+    const Geom g = a.g;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n_slots = (MQ ? a.n_queries : 1) * g.gqa;
+    const int tile = MQ ? longest_first(n_slots, 16, tile_z) : 0;
+    const int rows = min(16, n_slots - tile * 16);
+    const int my_slot = min(tile * 16 + n, n_slots - 1);
+    // the slot's last position and its first
+    auto limit_of = [&](int slot) { return a.q_pos0 + (MQ ? slot_row(g, slot) : 0); };
+    auto start_of = [&](int slot) { return a.window > 0 ? max(a.window_start, limit_of(slot) + 1 - a.window) : a.window_start; };
+    const int my_limit = limit_of(my_slot), my_ws = start_of(my_slot);
+    const int lim_lo = limit_of(tile * 16), lim_hi = limit_of(tile * 16 + rows - 1);
+    const int ws_lo = start_of(tile * 16), ws_hi = start_of(tile * 16 + rows - 1);
+
+    // The pages as a list in the order of positions: entry e < n_old is table[start + e] (less ring_pages past the ring's end), whose first
+    // row has position pos0 + 16 e; behind them (RING) pages outside the layer with the chunk's own rows.
+    const int pos0 = a.page_first * 16, n_old = RING ? c->n_old : INT32_MAX;
+    auto entry_pos = [&](int e) { return RING && e >= n_old ? c->new_first + (e - n_old) * 16 : pos0 + e * 16; };
+    auto entry_of = [&](int pos) { return RING && pos >= c->new_pos0 ? n_old + ((pos - c->new_first) >> 4) : max(pos - pos0, 0) >> 4; };
+    const int e_lo = entry_of(ws_lo), e_hi = entry_of(lim_hi) + 1;
+    const unsigned span = (unsigned)(e_hi - e_lo);
+    const int pb0 = e_lo + (int)(((unsigned)split * span) / (unsigned)a.splits);
+    const int pb1 = e_lo + (int)(((unsigned)(split + 1) * span) / (unsigned)a.splits);
+    // this wavefront's pairs are pb0 + 2 (wave + it * WAVES)
+    const int pairs = (pb1 - pb0 + 1) >> 1, n_it = pairs > wave ? (pairs - wave + WAVES - 1) / WAVES : 0;
+    // physical pages of the next 32 pairs, one a lane
+    int ids = 0;
+    auto fetch_ids = [&](int it) __attribute__((always_inline)) {
+        const int e = min(pb0 + 2 * (wave + (it + (lane >> 1)) * WAVES) + (lane & 1), e_hi - 1);
+        int at = a.ring_base + min(e, n_old - 1);
+        if (at >= a.ring_t) at -= a.ring_t;
+        const int page = a.table[max(at, 0)];
+        ids = RING && e >= n_old ? e - n_old : page;
+    };
+
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    uint32_t *q_codes = lds, *q_powers = lds + Fp4Lds<P, WAVES>::QUERIES;
+    uint32_t kc[2][NB][4], kp[2], vc[2][G], vp[2][G];
+    const int jk = G < 4 ? min(j, G - 1) : j; // (narrow heads: the lanes past the last group take it again, against queries of zero)
+    auto load_k = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int page = __builtin_amdgcn_readlane(ids, (2 * it + h) & 63);
+            const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->k_new : a.k_pool;
+            const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) load_words<4>(kc[h][b], cp + ((4 * b + jk) * 16 + n) * 16);
+            if constexpr (NB == 1) kp[h] = pp[jk * 16 + n];
+            else if constexpr (NB == 2) kp[h] = reinterpret_cast<const uint16_t *>(pp)[j * 16 + n];
+            else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
+        }
+    };
+    auto load_v = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int page = __builtin_amdgcn_readlane(ids, (2 * it + h) & 63);
+            const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->v_new : a.v_pool;
+            const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
+#pragma unroll
+            for (int v = 0; v < VL; ++v) {
+                uint32_t w[U];
+                load_words<U>(w, cp + (v * 64 + lane) * U * 4);
+#pragma unroll
+                for (int u = 0; u < U; ++u) vc[h][v * U + u] = w[u];
+            }
+            load_words<G>(vp[h], pp + j * G * 4);
+        }
+    };
+    fetch_ids(0);
+    load_k(0);
+    load_v(0);
+
+    // ---- queries: block b by wavefront b % WAVES, lane (slot n, group j) its 32 dims
+    for (int b = wave; b < NB; b += WAVES) {
+        const int d0 = b * 128 + j * 32;
+        const float *qrow = a.q + (MQ ? context_row(g, kvh, my_slot) : (long)(kvh * g.gqa + my_slot)) * g.head_dim;
+        float x[32];
+        if (a.q_vec) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const float4_t v = *reinterpret_cast<const float4_t *>(qrow + min(d0 + e, g.head_dim - 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[e + k] = v[k];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = qrow[min(d0 + e, g.head_dim - 1)];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            x[e] = n < rows && d0 + e < g.head_dim ? x[e] * a.qscale : 0.0f;
+            top = max(top, magnitude(x[e]));
+        }
+        // the first term's power is the smallest with the largest value <= 7.5 of it
+        int power = 255;
+        if (top < 0x7f800000u) power = max((int)((top + 0x0fffffu) >> 23) - 2, 18);
+        constexpr int down[4] = {0, 4, 9, 14};
+        if (power < 255) q_powers[b * 64 + lane] = (uint32_t)(power | (power - 4) << 8 | (power - 9) << 16) | (uint32_t)(power - 14) << 24;
+        else q_powers[b * 64 + lane] = 0xffffffffu;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const float scale = __uint_as_float((uint32_t)(power - down[t]) << 23);
+            const u6 codes = to_fp6(x, scale);
+#pragma unroll
+            for (int w = 0; w < 6; ++w) q_codes[((b * 4 + t) * 6 + w) * 64 + lane] = codes[w];
+            if (t < 3) {
+                const float32_t back = from_fp6(codes, scale);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] -= back[e];
+            }
+        }
+    }
+    __syncthreads();
+    int8v_t q_term[NB][4];
+    uint32_t q_power[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        q_power[b] = q_powers[b * 64 + lane];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int w = 0; w < 6; ++w) q_term[b][t][w] = (int)q_codes[((b * 4 + t) * 6 + w) * 64 + lane];
+            q_term[b][t][6] = q_term[b][t][7] = 0;
+        }
+    }
+
+    float4_t o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    for (int it = 0; it < n_it; ++it) {
+        const int e0 = pb0 + 2 * (wave + it * WAVES);
+        const int ea = entry_pos(e0), eb = entry_pos(min(e0 + 1, e_hi - 1));
+        // ---- scores of the pair: keys 4j .. 4j + 3 of slot n, of page a, then b
+        float4_t s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s[h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int8v_t k = {(int)kc[h][b][0], (int)kc[h][b][1], (int)kc[h][b][2], (int)kc[h][b][3], 0, 0, 0, 0};
+                const int kpow = (int)(kp[h] >> (8 * b));
+                s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][3], s[h], 4, 2, 0, kpow, 3, (int)q_power[b]);
+                s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][2], s[h], 4, 2, 0, kpow, 2, (int)q_power[b]);
+                s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][1], s[h], 4, 2, 0, kpow, 1, (int)q_power[b]);
+                s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][0], s[h], 4, 2, 0, kpow, 0, (int)q_power[b]);
+            }
+        }
+        if (it + 1 < n_it) {
+            if (((it + 1) & 31) == 0) fetch_ids(it + 1);
+            load_k(it + 1);
+        }
+        // ---- softmax in base 2; keys outside the slot's range get no weight, and where no slot of the workgroup attends them (rows past the
+        // length, before the window, of a page that is not there) V's powers are cleared as well: 0 x NaN is NaN
+        const int lo_b = RING ? (e0 + 1 >= n_old ? c->new_pos0 : INT32_MIN) : INT32_MIN;
+        const int lo_a = RING ? (e0 >= n_old ? c->new_pos0 : INT32_MIN) : INT32_MIN;
+        const int hi_a = RING && e0 < n_old ? c->new_pos0 - 1 : INT32_MAX;
+        const int hi_b = e0 + 1 >= pb1 ? INT32_MIN : RING && e0 + 1 < n_old ? c->new_pos0 - 1 : INT32_MAX;
+        const bool inside = ea >= max(ws_hi, lo_a) && ea + 15 <= min(lim_lo, hi_a) && eb >= max(ws_hi, lo_b) && eb + 15 <= min(lim_lo, hi_b);
+        if (!inside) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int p0 = (h ? eb : ea) + j * 4, lo = h ? lo_b : lo_a, hi = h ? hi_b : hi_a;
+                uint32_t keep = 0, seen = 0; // keys that some slot attends, that this lane's does
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = p0 + i;
+                    const bool here = pos >= lo && pos <= hi, mine = here && pos >= my_ws && pos <= my_limit;
+                    s[h][i] = mine ? s[h][i] : -INFINITY;
+                    if (mine) seen |= 255u << (8 * i);
+                    if (here && pos >= ws_lo && pos <= lim_hi) keep |= 255u << (8 * i);
+                }
+#pragma unroll
+                for (int t = 0; t < G; ++t) vp[h][t] &= keep;
+                if constexpr (MQ) { // a row that is NaN, attended by some slots and not by others: theirs alone
+#pragma unroll
+                    for (int t = 0; t < G; ++t) {
+                        const uint32_t nan = bytes_255(vp[h][t]);
+                        if (__builtin_amdgcn_ballot_w64(nan != 0)) {
+                            const float x = rows_max((nan & seen) != 0 ? 1.0f : 0.0f) > 0.0f ? NAN : 0.0f;
+                            o[2 * t] += x;
+                            o[2 * t + 1] += x;
+                            vp[h][t] &= ~nan;
+                        }
+                    }
+                }
+            }
+        }
+        float m_blk = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        m_blk = rows_max(m_blk);
+        const float m_new = fmaxf(m_run, m_blk), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = fast_exp2(m_run - m_safe);
+        uint32_t hi[4], lo[4];
+        float psum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = fast_exp2(s[i >> 1][2 * (i & 1)] - m_safe), y = fast_exp2(s[i >> 1][2 * (i & 1) + 1] - m_safe);
+            psum += x + y;
+            typedef __attribute__((ext_vector_type(2))) float f2;
+            hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf16x2_t));
+            lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u)}, bf16x2_t));
+        }
+        l_run = l_run * alpha + psum;
+        const bool rescale = alpha != 1.0f && m_run != -INFINITY; // (a slot without a key so far holds zeros)
+        m_run = m_new;
+        if (__builtin_amdgcn_ballot_w64(rescale)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] *= alpha;
+        }
+        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u4{hi[0], hi[1], hi[2], hi[3]}), pl = __builtin_bit_cast(bf16x8_t, u4{lo[0], lo[1], lo[2], lo[3]});
+        // ---- O^T += V^T . P^T
+#pragma unroll
+        for (int t = 0; t < G; ++t) {
+            u4 first, second; // dims 32 t + n and 32 t + 16 + n of the 32 keys
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t w = vc[h][t], e = vp[h][t];
+                const uint32_t c0 = code_pair<0>(w, e << 23), c1 = code_pair<1>(w, e << 15), c2 = code_pair<2>(w, e << 7), c3 = code_pair<3>(w, e >> 1);
+                first[2 * h] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);
+                first[2 * h + 1] = __builtin_amdgcn_perm(c3, c2, 0x05040100u);
+                second[2 * h] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);
+                second[2 * h + 1] = __builtin_amdgcn_perm(c3, c2, 0x07060302u);
+            }
+            const bf16x8_t va = __builtin_bit_cast(bf16x8_t, first), vb = __builtin_bit_cast(bf16x8_t, second);
+            o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pl, o[2 * t], 0, 0, 0);
+            o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pl, o[2 * t + 1], 0, 0, 0);
+            o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * t], 0, 0, 0);
+            o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * t + 1], 0, 0, 0);
+        }
+        if (it + 1 < n_it) load_v(it + 1);
+    }
+    l_run = rows_sum(l_run);
+
+    // ---- the wavefronts' states meet in LDS, four columns a thread
+    float *xo = reinterpret_cast<float *>(lds + Fp4Lds<P, WAVES>::QUERIES + Fp4Lds<P, WAVES>::POWERS); // [WAVES][rows][OSTRIDE]
+    float *xm = xo + WAVES * rows * OSTRIDE, *xl = xm + WAVES * rows;                                  // [WAVES][rows]
+    if (n < rows) {
+        float *dst = xo + (wave * rows + n) * OSTRIDE + j * 4;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<float4_t *>(dst + t * 16) = o[t];
+        if (j == 0) {
+            xm[wave * rows + n] = m_run;
+            xl[wave * rows + n] = l_run;
+        }
+    }
+    __syncthreads();
+    // (partials are aligned where heads are whole units; the context is the caller's, at any float's address)
+    const bool vec_ok = (g.head_dim & 3) == 0 && (a.splits_total > 1 || (reinterpret_cast<uintptr_t>(a.out) & 15) == 0);
+    for (int u = tid; u < rows * (P / 4); u += THREADS) {
+        const int row = u / (P / 4), c4 = (u - row * (P / 4)) * 4;
+        float mw[WAVES], mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            mw[w] = xm[w * rows + row];
+            mx = fmaxf(mx, mw[w]);
+        }
+        const float m_safe = mx == -INFINITY ? 0.0f : mx;
+        float4_t acc = {0.f, 0.f, 0.f, 0.f};
+        float lsum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float wgt = fast_exp2(mw[w] - m_safe);
+            acc += wgt * *reinterpret_cast<const float4_t *>(&xo[(w * rows + row) * OSTRIDE + c4]);
+            lsum += wgt * xl[w * rows + row];
+        }
+        if (c4 >= g.head_dim) continue;
+        const int slot = tile * 16 + row;
+        float *dst;
+        if (a.splits_total == 1) {
+            acc *= 1.0f / lsum;
+            dst = a.out + (MQ ? context_row(g, kvh, slot) : (long)(kvh * g.gqa + slot)) * g.head_dim + c4;
+        } else {
+            const long pidx = ((long)kvh * a.splits_total + split) * n_slots + slot;
+            dst = a.part_o + pidx * g.head_dim + c4;
+            if (c4 == 0) {
+                a.part_m[pidx] = mx;
+                a.part_l[pidx] = lsum;
+            }
+        }
+        if (vec_ok) {
+            *reinterpret_cast<float4_t *>(dst) = acc;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c4 + i < g.head_dim) dst[i] = acc[i];
+        }
+    }
+}
+
+template <int P, int WAVES, bool MQ, bool RING>
+__global__ __launch_bounds__(WAVES * 64) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
+    fp4_attention_body<P, WAVES, MQ, RING>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+template <int P, int WAVES, bool MQ, bool RING>
+static hipError_t launch_fp4_of(const DecodeArgs &a, const ChunkPages &c, hipStream_t s) {
+    static std::atomic<uint64_t> lds_ok{0}; // per instantiation
+    {
+        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_kernel<P, WAVES, MQ, RING>), lds_ok);
+        if (e != hipSuccess) return e;
+    }
+    const int n_slots = a.n_queries * a.g.gqa;
+    const dim3 grid((unsigned)a.splits, (unsigned)a.g.kv_heads, (unsigned)((n_slots + 15) / 16));
+    const size_t lds = Fp4Lds<P, WAVES>::bytes(n_slots < 16 ? n_slots : 16);
+    hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING>), grid, dim3(WAVES * 64), lds, s, a, c);
+    return hipGetLastError();
+}
+template <int P, int WAVES>
+static hipError_t launch_fp4(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
+    if (c) return launch_fp4_of<P, WAVES, true, true>(a, *c, s);
+    if (a.n_queries * a.g.gqa > 16 || a.n_queries > 1) return launch_fp4_of<P, WAVES, true, false>(a, ChunkPages{}, s);
+    return launch_fp4_of<P, WAVES, false, false>(a, ChunkPages{}, s);
+}
+
+hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
+    if (a.pre || a.k_new || a.split_base != 0) return hipErrorInvalidValue;
+    switch (a.g.P) {
+    case 32: return launch_fp4<32, 8>(a, c, s);
+    case 64: return launch_fp4<64, 8>(a, c, s);
+    case 96: return launch_fp4<96, 8>(a, c, s);
+    case 128: return launch_fp4<128, 8>(a, c, s);
+    case 256: return launch_fp4<256, 8>(a, c, s);
+    case 512: return launch_fp4<512, 4>(a, c, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+} // namespace skv

@@ -457,11 +457,16 @@ int32_t check_window(const skv_layer *L, size_t window_start) {
     return SKV_OK;
 }
 
+// Bytes of a row of one kv head, K or V, as the element keeps it.
+size_t row_bytes(const Geom &g) {
+    const size_t hd = (size_t)g.head_dim;
+    return g.fp4 ? (hd + 1) / 2 + (hd + 31) / 32 : hd * (g.f32 ? 4 : 2);
+}
 bool uses_flash(const skv_layer *L) { return skv_flag_flash_sdpa_enabled() && L->g.P <= 512; }
 // The attention launch of a decode step can append the row itself: always on bf16 layers,
 // on f32 layers where the f32 decode kernel serves the shape (head_dim up to 256, at most 16
 // heads per group).
-bool fused_append_built(const skv_layer *L) { return !L->g.f32 || (L->g.P <= 256 && L->g.gqa <= 16); }
+bool fused_append_built(const skv_layer *L) { return !L->g.fp4 && (!L->g.f32 || (L->g.P <= 256 && L->g.gqa <= 16)); }
 // The fused pre-KV step is built for bf16 layers up to head_dim 512 and for f32 layers up to
 // head_dim 256; wide f32 heads take the separate norm/rotation launches.
 bool wide_f32_heads(const skv_layer *L) { return L->g.f32 && L->g.P > 256; }
@@ -519,6 +524,28 @@ void fill_decode_args(const skv_layer *L, const float *q_dev, float *out_dev, si
     a.new_page = L->table[(size_t)(a.new_slot >> 4)];
     a.q_vec = (tuning().q_vec && (reinterpret_cast<uintptr_t>(q_dev) & 15) == 0 && (g.head_dim & 7) == 0) ? 1 : 0;
     a.g = g;
+}
+
+// The same for the 4-bit element, whose kernel walks the pages that the queries can see as a list in the order of positions: a.page_first is the
+// first one's number, a.ring_base its place in the table, a.ring_t where the table comes round. A wavefront takes a pair of pages at a
+// time; no split leaves one without.
+void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_t window_start, size_t n_queries, DecodeArgs &a) {
+    fill_decode_args(L, q_dev, out_dev, window_start, nullptr, nullptr, n_queries, decode_target_wgs(), a);
+    const Geom &g = L->g;
+    // (a decode step's window_start is the caller's, who may want less than the layer's window or all that a ring holds)
+    const size_t first = (n_queries > 1 ? std::max(window_start, skv_window_start(L->len - n_queries, L->window)) : window_start) / 16;
+    const int ring_pages = g.ring_rows / 16;
+    a.page_first = (int)first;
+    a.ring_base = ring_pages > 0 ? (int)(first % (size_t)ring_pages) : (int)first;
+    a.ring_t = ring_pages > 0 ? ring_pages : INT32_MAX;
+    a.n_pages = (int)((L->len + 15) / 16 - first);
+    a.waves = g.P > 256 ? 4 : 8;
+    a.splits = choose_splits(L, (a.n_pages + 1) / 2, L->len - window_start, a.waves, decode_target_wgs());
+    if (n_queries * (size_t)g.gqa > 16) {
+        const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
+        a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(512 / tiles, 1));
+    }
+    a.splits_total = a.splits;
 }
 
 bool capturing(hipStream_t s) {
@@ -850,6 +877,25 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         return settle();
     }
     const bool use_flash = uses_flash(L) || n_queries > 1;
+    if (g.fp4 && use_flash) {
+        if (k_new || v_new || pre) return fail(SKV_ERR_CONFIG, "KV 4 bits: étape fusionnée non construite pour cette forme");
+        DecodeArgs a{};
+        fill_fp4_args(L, q_dev, out_dev, window_start, n_queries, a);
+        if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
+        if (n_queries > 1 && a.splits > 1) {
+            rc = multi_query_partials(L, s, (size_t)a.splits, n_queries, a, lease);
+            if (rc) return rc;
+        }
+        if (static_partials && a.splits > 1) {
+            rc = partials_in(static_partials, SKV_STATIC_SCRATCH_BYTES, a);
+            if (rc) return rc;
+        }
+        rc = place(a.splits, a.out);
+        if (rc) return rc;
+        SKV_HIP(launch_fp4_attention(a, nullptr, s));
+        if (a.splits > 1) SKV_HIP(n_queries > 1 ? launch_merge_rows(a, s) : launch_merge(a, s));
+        return settle();
+    }
     if (!use_flash) {
         const size_t need = (size_t)g.q_heads * L->capacity;
         if (L->scores_cap < need) {
@@ -1059,9 +1105,9 @@ static int32_t plan_layer(size_t capacity, size_t q_heads, size_t kv_heads, size
     if (q_heads % kv_heads != 0)
         return fail(SKV_ERR_CONFIG, "GQA invalide: q_heads=" + std::to_string(q_heads) +
                                         " non multiple de kv_heads=" + std::to_string(kv_heads));
-    if (dtype != SKV_DTYPE_BF16 && dtype != SKV_DTYPE_F32)
+    if (dtype != SKV_DTYPE_BF16 && dtype != SKV_DTYPE_F32 && dtype != SKV_DTYPE_FP4)
         return fail(SKV_ERR_CONFIG, "élément KV inconnu: " + std::to_string(dtype));
-    const bool f32 = dtype == SKV_DTYPE_F32;
+    const bool f32 = dtype == SKV_DTYPE_F32, fp4 = dtype == SKV_DTYPE_FP4;
     const int P = padded_head_dim(head_dim);
     if (P == 0) return fail(SKV_ERR_CONFIG, "head_dim > 512 non supporté");
     if (capacity > (size_t)1 << 30 || q_heads > 4096 || kv_heads > 4096 || window > (size_t)1 << 30 ||
@@ -1074,7 +1120,8 @@ static int32_t plan_layer(size_t capacity, size_t q_heads, size_t kv_heads, size
     g.P = P;
     set_gqa(g);
     g.f32 = f32 ? 1 : 0;
-    g.tile_elems = P * 16 * (f32 ? 2 : 1);
+    g.fp4 = fp4 ? 1 : 0;
+    g.tile_elems = fp4 ? P * 17 / 4 : P * 16 * (f32 ? 2 : 1);
     g.page_elems = (int)kv_heads * g.tile_elems;
     size_t rows = capacity;
     if (window > 0) {
@@ -1090,7 +1137,8 @@ static int32_t plan_layer(size_t capacity, size_t q_heads, size_t kv_heads, size
         rows = ring;
     }
     p.n_pages = (int)((rows + 15) / 16);
-    p.pool_bytes = (size_t)p.n_pages * kv_heads * pool_head_dim(head_dim) * 16 * (f32 ? sizeof(float) : sizeof(uint16_t));
+    p.pool_bytes = fp4 ? (size_t)p.n_pages * (size_t)g.page_elems * sizeof(uint16_t)
+                       : (size_t)p.n_pages * kv_heads * pool_head_dim(head_dim) * 16 * (f32 ? sizeof(float) : sizeof(uint16_t));
     p.max_splits = std::min(decode_max_splits(), std::max(1, p.n_pages));
     const size_t n_part = (size_t)kv_heads * p.max_splits * g.gqa;
     p.table_bytes = (size_t)p.n_pages * sizeof(int32_t);
@@ -1258,7 +1306,7 @@ size_t skv_kv_heads(const skv_layer *L) { return L ? (size_t)L->g.kv_heads : 0; 
 size_t skv_head_dim(const skv_layer *L) { return L ? (size_t)L->g.head_dim : 0; }
 size_t skv_window(const skv_layer *L) { return L ? L->window : 0; }
 size_t skv_logical_byte_len(const skv_layer *L) {
-    return L ? L->capacity * (size_t)L->g.kv_heads * L->g.head_dim * (L->g.f32 ? 4 : 2) : 0;
+    return L ? L->capacity * (size_t)L->g.kv_heads * row_bytes(L->g) : 0;
 }
 
 int32_t skv_truncate(skv_layer *L, size_t len) try {
@@ -1472,7 +1520,7 @@ static bool context_over_rows(const skv_layer *L, size_t c, const float *out, co
     return over_rows(L->g, out, k, c) || over_rows(L->g, out, v, c);
 }
 
-// A chunk of c > 1 rows on a ring layer (bf16, or f32 where the f32 chunk kernel serves the head_dim). The
+// A chunk of c > 1 rows on a ring layer (bf16, 4 bits, or f32 where the f32 chunk kernel serves the head_dim). The
 // ring holds little more than the window, so the chunk's own rows overwrite rows its first queries still attend. They are therefore first
 // written to pages of the context's scratch; one launch attends the ring's rows and them, in the
 // order of positions, each workgroup only the pages its slots' windows touch; then the rows go
@@ -1506,6 +1554,7 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
     // a context over the chunk's own rows is written once they are in the ring, one over its queries once all are read: by the merge, so
     // there has to be one
     const bool late = context_over_rows(L, c, out, k, v) || over_queries(g, out, q, c) || reads_again(g, out, q);
+    const size_t slots = g.f32 ? (size_t)f32_prefill_slots(g.P, halves) : g.fp4 ? 16 : (size_t)prefill_tile_slots(g.P, shape); // of a workgroup
     StreamScratch::Lease lease;
     void *scratch = nullptr;
     int32_t rc = SKV_OK;
@@ -1523,7 +1572,7 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
         }
     }
     if (!made) {
-        a.splits = chunk_splits(g, c, (size_t)(g.f32 ? f32_prefill_slots(g.P, halves) : prefill_tile_slots(g.P, shape)), walked);
+        a.splits = chunk_splits(g, c, slots, walked);
         if (late) a.splits = std::max(a.splits, 2);
         a.splits_total = a.splits;
         rc = multi_query_partials(L, s, a.splits > 1 ? (size_t)a.splits : 0, c, a, lease, 2 * pool_bytes, &scratch);
@@ -1545,7 +1594,14 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
         SKV_HIP(launch_append(w, s));
         pages.k_new = w.k_pool;
         pages.v_new = w.v_pool;
-        SKV_HIP(g.f32 ? launch_f32_prefill(a, pages, nullptr, halves, s) : launch_prefill_tiles(a, pages, shape, s));
+        if (g.fp4) {
+            a.page_first = pages.first_pos / 16;
+            a.ring_base = pages.start;
+            a.ring_t = pages.ring_pages;
+            SKV_HIP(launch_fp4_attention(a, &pages, s));
+        } else {
+            SKV_HIP(g.f32 ? launch_f32_prefill(a, pages, nullptr, halves, s) : launch_prefill_tiles(a, pages, shape, s));
+        }
     }
     if (a.splits_total == 1) return encode_append(L, s, k, v, c);
     if (late) {
@@ -1553,6 +1609,10 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
         if (rc) return rc;
         SKV_HIP(launch_merge_rows(a, s));
         return SKV_OK;
+    }
+    if (g.fp4) {
+        SKV_HIP(launch_merge_rows(a, s));
+        return encode_append(L, s, k, v, c);
     }
     SKV_HIP(launch_merge_append(a, append_args(L, k, v, c), s)); // (the caller has checked the capacity)
     appended(L, c);
@@ -1643,7 +1703,7 @@ int32_t skv_prefill_chunk_device(skv_layer *L, skv_stream stream, const float *q
         }
         // a few rows over a full bf16 layer (a speculative verify, the rest of a prompt): the multi-query launch
         // appends them itself, as a decode step's does (its last query tile, which sees all of them, stores them)
-        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && tuning().fused_append &&
+        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && !L->g.fp4 && tuning().fused_append &&
             !context_over_rows(L, c, out, k, v) && !takes_tile_kernel(L->g, c, (L->len + c + 15) / 16)) {
             RowsAhead ahead(L, c);
             rc = encode_attention(L, as_stream(stream), q, out, 0, k, v, c);
@@ -1916,7 +1976,7 @@ static int32_t prekv_step(skv_layer *L, skv_stream stream, const skv_rope *rope,
                                            std::to_string(L->capacity) + " atteinte (overflow)");
     hipStream_t s = as_stream(stream);
     const bool fused = tuning().fused_append;
-    if (!fused || !uses_flash(L) || wide_f32_heads(L) || L->g.gqa > 16) {
+    if (!fused || !uses_flash(L) || wide_f32_heads(L) || L->g.fp4 || L->g.gqa > 16) {
         // the same step as separate launches: norm + rotation of q and k, append, attention, gate
         NormRopeArgs n{};
         n.x = q;
@@ -2041,7 +2101,7 @@ int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_s
             return fail(SKV_ERR_DEVICE, "decode_step_batch: pointeur nul (séquence " + std::to_string(i) + ")");
         const Geom &g = L->g, &g0 = seqs[0]->g;
         if (g.q_heads != g0.q_heads || g.kv_heads != g0.kv_heads || g.head_dim != g0.head_dim ||
-            (g.ring_rows > 0) != (g0.ring_rows > 0) || g.f32 != g0.f32 || L->window != seqs[0]->window ||
+            (g.ring_rows > 0) != (g0.ring_rows > 0) || g.f32 != g0.f32 || g.fp4 != g0.fp4 || L->window != seqs[0]->window ||
             L->ctx != seqs[0]->ctx)
             return fail(SKV_ERR_DIMENSION, "decode_step_batch: la séquence " + std::to_string(i) +
                                                " n'a pas la géométrie de la séquence 0");
@@ -2308,8 +2368,9 @@ int32_t skv_probe_merge_device(skv_layer *L, skv_stream stream, float *out_dev) 
     if (L->len == 0) return fail(SKV_ERR_DIMENSION, "probe: cache vide");
     if (!uses_flash(L)) return fail(SKV_ERR_CONFIG, "probe: noyau matriciel seulement");
     DecodeArgs a{};
-    fill_decode_args(L, nullptr, out_dev, skv_window_start(L->len - 1, L->window), nullptr, nullptr, 1,
-                     decode_target_wgs(), a, false, true);
+    const size_t ws = skv_window_start(L->len - 1, L->window);
+    if (L->g.fp4) fill_fp4_args(L, nullptr, out_dev, ws, 1, a);
+    else fill_decode_args(L, nullptr, out_dev, ws, nullptr, nullptr, 1, decode_target_wgs(), a, false, true);
     if (a.splits > 1) SKV_HIP(launch_merge(a, as_stream(stream)));
     return SKV_OK;
 } catch (...) {

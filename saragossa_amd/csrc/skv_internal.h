@@ -58,10 +58,11 @@ struct Geom {
     int head_dim;
     int P;          // padded head dim
     int gqa;        // q_heads / kv_heads
-    int tile_elems; // one (page, kv head) tile in 16-bit units: P * 16 (bf16), P * 32 (f32)
+    int tile_elems; // one (page, kv head) tile in 16-bit units: P * 16 (bf16), P * 32 (f32), P * 17 / 4 (codes and powers of 4 bits)
     int page_elems; // kv_heads * tile_elems
     int ring_rows;  // 0 = full cache; else rows kept by the ring (multiple of 16)
-    int f32;        // 1 = the tiles hold f32 (kernels_f32.hip), 0 = bf16
+    short f32;      // 1 = the tiles hold f32 (kernels_f32.hip)
+    short fp4;      // 1 = codes of 4 bits (fp4_tile.h); neither = bf16
     // slot / gqa as a product: floor(2^(31 + s) / gqa) + 1, s the bits of gqa - 1 (set_gqa)
     uint32_t gqa_mul;
     int gqa_shift;
@@ -443,6 +444,10 @@ hipError_t launch_gather(const GatherArgs &a, hipStream_t s);
 // the split launch for one query row or a chunk (the caller merges as for bf16)
 hipError_t launch_gather_f32(const GatherArgs &a, hipStream_t s);
 hipError_t launch_f32_split(const DecodeArgs &a, hipStream_t s);
+// the 4-bit element (kernels_fp4.hip): rows in, rows out as bf16 (launch_append and launch_gather send them there), attention
+hipError_t launch_store_fp4(const AppendArgs &a, hipStream_t s);
+hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s);
+hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s); // no merge; c null = the layer's own pages
 bool f32_decode_kernel_serves(const DecodeArgs &a); // the launch takes the kernel that can also append the row
 hipError_t launch_decode(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_decode_batch(const DecodeBatchArgs &b, int n_seq, hipStream_t s);

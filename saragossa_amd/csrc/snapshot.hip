@@ -165,7 +165,7 @@ struct SlotLayout {
     // kv heads, head_dim and element: two layers whose pages merely have the same size
     // (bf16 at head_dim 256 and f32 at 128, say) must not exchange pages
     static uint64_t shape_of(const skv_layer *L) {
-        return ((uint64_t)L->g.kv_heads << 32) | ((uint64_t)L->g.head_dim << 1) | (uint64_t)(L->g.f32 & 1);
+        return ((uint64_t)L->g.kv_heads << 32) | ((uint64_t)L->g.head_dim << 2) | (uint64_t)((L->g.fp4 & 1) << 1) | (uint64_t)(L->g.f32 & 1);
     }
     void build(skv_layer *const *layers, size_t n, size_t slots = 0, bool by_layer = false) {
         page_bytes.resize(n);

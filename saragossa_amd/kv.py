@@ -11,7 +11,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import DTYPE_BF16, DTYPE_F32, calls, check, lib, settle
+from ._lib import DTYPE_BF16, DTYPE_F32, DTYPE_FP4, calls, check, lib, settle
 
 
 def _f32(a) -> np.ndarray:
@@ -121,6 +121,12 @@ class DecodeResidentState:
         full_attention chooses for greedy decoding."""
         return self.full_attention_with_element(capacity, q_heads, kv_heads, head_dim,
                                                 DTYPE_F32, window)
+
+    def full_attention_fp4(self, capacity, q_heads, kv_heads, head_dim, window=0):
+        """A layer whose rows are kept as codes of 4 bits with a power of two per 32 dims (no counterpart in
+        the reference): 4.25 bits a value, attended as the values the codes stand for."""
+        return self.full_attention_with_element(capacity, q_heads, kv_heads, head_dim,
+                                                DTYPE_FP4, window)
 
 
 def rope_rotations(position, rope_dims, theta, position_scale=1.0, frequency_dim=0) -> np.ndarray:

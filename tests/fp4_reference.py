@@ -1,0 +1,74 @@
+"""The 4-bit element from its definition, in numpy: what the tests of the device's rows and contexts compare with."""
+import numpy as np
+
+GROUP = 32
+LEVELS = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def stored(rows, head_dim):
+    """What rows [n, heads * head_dim] are worth once stored, in 64 bits: per group of 32 dims of a head the smallest power
+    2^e with max |x| <= 7 * 2^e, e in [-125, 125], and x / 2^e at the nearest of LEVELS, ties to the even index; NaN for a group
+    that is not finite."""
+    x = np.asarray(rows, np.float32).astype(np.float64)
+    n = x.shape[0]
+    x = x.reshape(n, -1, head_dim)
+    out = np.empty_like(x)
+    for d in range(0, head_dim, GROUP):
+        part = x[:, :, d:d + GROUP]
+        top = np.abs(part).max(-1, keepdims=True)
+        finite = np.isfinite(top)
+        safe = np.where(finite, top, 1.0)
+        m, e = np.frexp(safe / 7.0)  # in [1/2, 1) times 2^e: the power is 2^e, or 2^(e - 1) where m is 1/2
+        e = np.clip(np.where(m == 0.5, e - 1, e), -125, 125)
+        e = np.where(safe == 0.0, -125, e)
+        scale = np.ldexp(1.0, e)
+        y = np.where(finite, np.abs(part), 0.0) / scale
+        far = np.abs(y[..., None] - LEVELS)
+        best = far.min(-1, keepdims=True)
+        near = far == best  # one level, or two at a tie: the even one
+        idx = np.where(near.sum(-1) > 1, np.where(near, (np.arange(8) % 2 == 0) * 8 + 1, 0).argmax(-1), near.argmax(-1))
+        value = np.copysign(LEVELS[idx] * scale, part)
+        out[:, :, d:d + GROUP] = np.where(finite, value, np.nan)
+    return out.reshape(n, -1)
+
+
+def attention(q, keys, values, dims, first=None, window=0, window_start=0, attn_scalar=None):
+    """Rows q [n, q_heads * hd] over stored rows [len, kv_dim] (64 bits): contexts, and the bound that `tolerance` gives each of
+    their values. Row i is at position len - n + i (or first + i) and sees positions up to its own, through the window."""
+    q_heads, kv_heads, hd = dims
+    q = np.asarray(q, np.float32).reshape(-1, q_heads, hd)
+    k = keys.reshape(-1, kv_heads, hd)
+    v = values.reshape(-1, kv_heads, hd)
+    n = q.shape[0]
+    first = len(k) - n if first is None else first
+    out, tol = np.empty(q.shape), np.empty(q.shape)
+    scale = 1.0 / np.sqrt(attn_scalar or hd)
+    for i in range(n):
+        lo, hi = max(window_start, first + i + 1 - window if window else 0), first + i + 1
+        for h in range(q_heads):
+            kk, vv = k[lo:hi, h * kv_heads // q_heads], v[lo:hi, h * kv_heads // q_heads]
+            x = q[i, h].astype(np.float64) * scale
+            s = kk @ x
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[i, h] = p @ vv
+            tol[i, h] = _bound(x, kk, s) * (p @ np.abs(vv)) + 1e-37
+    return out.reshape(n, -1), tol.reshape(n, -1)
+
+
+def _bound(x, k, s):
+    """Relative to the weighted mean of |v|, how far a context may be off.
+
+    A query value is four terms, the last of which leaves 2^-17 of the first term's power at most, a power that is at least the
+    group's largest value over 7.5 and at most that over 3.75: 2^-18.9 of the largest value, one way or the other, so that dims are
+    off independently of each other and a score by six of its standard deviations at most (the times log2(e) and back of base 2
+    are in the 2^-24 below). Sums of at most 16 products and roundings of the score: 8 halves of a step of 32 bits of the sum of
+    magnitudes. A score off by d moves the weights by 2 d relative to their sum. The weights are two terms of 16 bits, off by 2^-18, the
+    exponential by 2^-22, sums of up to some thousand keys in partials of a few dozen: 2^-20 together."""
+    hd = len(x)
+    var = 0.0
+    for d in range(0, hd, GROUP):
+        step = np.abs(x[d:d + GROUP]).max() * 2.0 ** -18.9
+        var = var + step ** 2 / 3.0 * (k[:, d:d + GROUP] ** 2).sum(-1)
+    ds = 6.0 * np.sqrt(var) + (np.abs(k) @ np.abs(x) + np.abs(s)) * 8 * 2.0 ** -24
+    return 2.0 * ds.max() + 2.0 ** -18 + 2.0 ** -20
