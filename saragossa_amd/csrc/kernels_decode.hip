@@ -1043,6 +1043,7 @@ hipError_t launch_decode_batch(const DecodeBatchArgs &b, int n_seq, hipStream_t 
     hipError_t e = hipErrorInvalidValue;
     const bool w8 = a0.waves == 8;
     if (a0.g.f32) e = launch_f32_split_batch(b, n_seq, max_splits, s);
+    else if (a0.g.fp4) e = launch_fp4_batch(b, n_seq, max_splits, s);
     else switch (a0.g.P) {
     case 512: e = launch_split_batch<512, 4>(b, n_seq, max_splits, s); break;
     case 32: e = w8 ? launch_split_batch<32, 8>(b, n_seq, max_splits, s) : launch_split_batch<32, 4>(b, n_seq, max_splits, s); break;

@@ -1,6 +1,7 @@
 // gfx950 kernels of the 4-bit element (fp4_tile.h): rows stored as codes, read back, and attended.
 #include "append_tile.h"
 #include "fp4_tile.h"
+#include "pre_kv.h"
 
 namespace skv {
 
@@ -220,14 +221,19 @@ __device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
     return (zero >> 7) * 255u;
 }
 
-// LDS: [NB][4 terms][6 words][64 lanes] of the queries, [NB][64] their powers, then the wavefronts' states
+// LDS in words: [NB][4 terms][6 words][64 lanes] of the queries, [NB][64] their powers; of the new rows, per row, K codes, V codes, K
+// powers, V powers; then the wavefronts' states
 template <int P, int WAVES>
 struct Fp4Lds {
     static constexpr int NB = Fp4Tile<P>::NB, QUERIES = NB * 4 * 6 * 64, POWERS = NB * 64;
-    static constexpr size_t bytes(int rows) { return ((size_t)(QUERIES + POWERS) + (size_t)WAVES * rows * (P + 4 + 2)) * 4; }
+    static constexpr int NEW_ROW = P + 2 * (P / 32); // bytes
+    __host__ __device__ static constexpr int states(int new_rows) { return QUERIES + POWERS + (new_rows * NEW_ROW + 15) / 16 * 4; }
+    static constexpr size_t bytes(int rows, int new_rows) { return ((size_t)states(new_rows) + (size_t)WAVES * rows * (P + 4 + 2)) * 4; }
 };
 
-template <int P, int WAVES, bool MQ, bool RING>
+// MQ: more than one query row, or more than 16 heads to a kv head: slots are (row, head) pairs, 16 to a workgroup (grid z). ROWS: the launch
+// stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one.
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false>
 __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const ChunkPages *c, const int split, const int kvh, const int tile_z) {
     using T = Fp4Tile<P>;
     constexpr int THREADS = WAVES * 64, G = T::G, U = T::U, NB = T::NB, VL = T::VL, NT = P / 16, OSTRIDE = P + 4;
@@ -256,24 +262,80 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     const int pb1 = e_lo + (int)(((unsigned)(split + 1) * span) / (unsigned)a.splits);
     // this wavefront's pairs are pb0 + 2 (wave + it * WAVES)
     const int pairs = (pb1 - pb0 + 1) >> 1, n_it = pairs > wave ? (pairs - wave + WAVES - 1) / WAVES : 0;
+    // place of an entry in the table
+    auto place = [&](int e) __attribute__((always_inline)) {
+        int at = a.ring_base + min(e, n_old - 1);
+        if (at >= a.ring_t) at -= a.ring_t;
+        return max(at, 0);
+    };
     // physical pages of the next 32 pairs, one a lane
     int ids = 0;
     auto fetch_ids = [&](int it) __attribute__((always_inline)) {
         const int e = min(pb0 + 2 * (wave + (it + (lane >> 1)) * WAVES) + (lane & 1), e_hi - 1);
-        int at = a.ring_base + min(e, n_old - 1);
-        if (at >= a.ring_t) at -= a.ring_t;
-        const int page = a.table[max(at, 0)];
+        const int page = a.table[place(e)];
         ids = RING && e >= n_old ? e - n_old : page;
     };
 
+    // ---- the rows that the launch stores: every workgroup that walks a page of theirs converts them and keeps the codes in LDS, from where its
+    // wavefronts patch what they load; the last tile of slots, which sees all of them, stores them. An eighth of a group a thread.
+    constexpr bool NEW = !MQ || ROWS;
+    constexpr int NU = ROWS ? (MQ_APPEND_ROWS * 2 * G * 8 + THREADS - 1) / THREADS : 1;
+    static_assert(!NEW || NU * THREADS >= (ROWS ? MQ_APPEND_ROWS : 1) * 2 * G * 8, "every eighth of every new row has a thread");
+    const int C = ROWS ? a.n_queries : 1;
+    const int p_new = a.len - C, e_new = (p_new - pos0) >> 4, e_last = (a.len - 1 - pos0) >> 4;
+    const bool appends = NEW && a.k_new != nullptr && e_last >= pb0 && e_new < pb1;
+    const bool stores = tile == (n_slots - 1) / 16;
+    float nx[NU][4];
+    int page_a = 0, page_b = 0;
+    if constexpr (NEW) {
+        if (appends) { // uniform
+            const bool vec = (g.head_dim & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.k_new) | reinterpret_cast<uintptr_t>(a.v_new)) & 15) == 0;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int idx = (tid + u * THREADS) >> 3, v = idx >= C * G, row = min((idx - v * C * G) / G, C - 1), d = (idx % G) * 32 + (tid & 7) * 4;
+                const float *src = (v ? a.v_new : a.k_new) + ((long)row * g.kv_heads + kvh) * g.head_dim;
+                if (vec) {
+                    const float4_t x = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) nx[u][e] = x[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) nx[u][e] = src[min(d + e, g.head_dim - 1)];
+                }
+            }
+        }
+    }
+    // ---- queries: block b by wavefront b % WAVES, lane (slot n, group j) its 32 dims
+    constexpr int QB = (NB + WAVES - 1) / WAVES;
+    static_assert(QB == 1, "a wavefront converts one block of the queries");
+    const float *qrow = a.q + (MQ ? context_row(g, kvh, my_slot) : (long)(kvh * g.gqa + my_slot)) * g.head_dim;
+    const int d0 = wave * 128 + j * 32;
+    float x[32];
+    if (wave < NB) {
+        if (a.q_vec) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const float4_t v = *reinterpret_cast<const float4_t *>(qrow + min(d0 + e, g.head_dim - 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[e + k] = v[k];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = qrow[min(d0 + e, g.head_dim - 1)];
+        }
+    }
+
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    uint8_t *new_rows = reinterpret_cast<uint8_t *>(lds + Fp4Lds<P, WAVES>::QUERIES + Fp4Lds<P, WAVES>::POWERS);
+    constexpr int NEW_ROW = Fp4Lds<P, WAVES>::NEW_ROW, AT_V = P / 2, AT_KP = P, AT_VP = P + G; // in a new row
     uint32_t *q_codes = lds, *q_powers = lds + Fp4Lds<P, WAVES>::QUERIES;
     uint32_t kc[2][NB][4], kp[2], vc[2][G], vp[2][G];
     const int jk = G < 4 ? min(j, G - 1) : j; // (narrow heads: the lanes past the last group take it again, against queries of zero)
-    auto load_k = [&](int it) __attribute__((always_inline)) {
+    auto page_id = [&](int it, int h) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ids, (2 * it + h) & 63); };
+    auto load_k = [&](int it, int page0, int page1) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int page = __builtin_amdgcn_readlane(ids, (2 * it + h) & 63);
+            const int page = h ? page1 : page0;
             const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->k_new : a.k_pool;
             const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
 #pragma unroll
@@ -283,10 +345,10 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
         }
     };
-    auto load_v = [&](int it) __attribute__((always_inline)) {
+    auto load_v = [&](int it, int page0, int page1) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int page = __builtin_amdgcn_readlane(ids, (2 * it + h) & 63);
+            const int page = h ? page1 : page0;
             const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->v_new : a.v_pool;
             const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
 #pragma unroll
@@ -299,26 +361,58 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             load_words<G>(vp[h], pp + j * G * 4);
         }
     };
-    fetch_ids(0);
-    load_k(0);
-    load_v(0);
-
-    // ---- queries: block b by wavefront b % WAVES, lane (slot n, group j) its 32 dims
-    for (int b = wave; b < NB; b += WAVES) {
-        const int d0 = b * 128 + j * 32;
-        const float *qrow = a.q + (MQ ? context_row(g, kvh, my_slot) : (long)(kvh * g.gqa + my_slot)) * g.head_dim;
-        float x[32];
-        if (a.q_vec) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                const float4_t v = *reinterpret_cast<const float4_t *>(qrow + min(d0 + e, g.head_dim - 4));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[e + k] = v[k];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = qrow[min(d0 + e, g.head_dim - 1)];
+    // The first pair's places come through the scalar unit, counted apart from the loads above: its requests do not wait for them.
+    {
+        const int ea = min(pb0 + 2 * wave, e_hi - 1), eb = min(pb0 + 2 * wave + 1, e_hi - 1);
+        const int pa = RING && ea >= n_old ? ea - n_old : table_entry<true>(a.table, place(ea));
+        const int pb = RING && eb >= n_old ? eb - n_old : table_entry<true>(a.table, place(eb));
+        if constexpr (NEW) {
+            page_a = table_entry<true>(a.table, place(min(max(e_new, 0), e_hi - 1)));
+            page_b = table_entry<true>(a.table, place(min(max(e_last, 0), e_hi - 1)));
         }
+        load_k(0, pa, pb);
+        load_v(0, pa, pb);
+    }
+    fetch_ids(0);
+
+    if constexpr (NEW) {
+        if (appends) { // uniform
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int idx = (tid + u * THREADS) >> 3, v = idx >= C * G, row = (idx - v * C * G) / G, t = idx % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+                const bool real = idx < 2 * C * G;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) nx[u][e] = real && d + e < g.head_dim ? nx[u][e] : 0.0f;
+                uint32_t power;
+                const uint32_t codes = fp4_codes_of(nx[u], power);
+                const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
+                if (!real) continue;
+                uint8_t *to = new_rows + row * NEW_ROW;
+                const int e = (p_new + row - pos0) >> 4, r = (p_new + row) & 15, page = e == e_new ? page_a : page_b;
+                const bool store = stores && e >= pb0 && e < pb1;
+                uint16_t *pool = const_cast<uint16_t *>(v ? a.v_pool : a.k_pool);
+                uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
+                if (!v) {
+                    *reinterpret_cast<uint16_t *>(to + t * 16 + o8 * 2) = (uint16_t)codes;
+                    if (o8 == 0) to[AT_KP + t] = (uint8_t)power;
+                    if (store) {
+                        *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
+                        if (o8 == 0) pp[k4_power(P, r, t)] = (uint8_t)power;
+                    }
+                } else if (o8 < 4) {
+                    const uint32_t word = nibbles_apart(codes) | nibbles_apart(other) << 4;
+                    *reinterpret_cast<uint32_t *>(to + AT_V + t * 16 + o8 * 4) = word;
+                    if (o8 == 0) to[AT_VP + t] = (uint8_t)power;
+                    if (store) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) cp[v4_code(P, r, d + k)] = (uint8_t)(word >> (8 * k));
+                        if (o8 == 0) pp[v4_power(P, r, t)] = (uint8_t)power;
+                    }
+                }
+            }
+        }
+    }
+    if (wave < NB) {
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
@@ -329,14 +423,14 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         int power = 255;
         if (top < 0x7f800000u) power = max((int)((top + 0x0fffffu) >> 23) - 2, 18);
         constexpr int down[4] = {0, 4, 9, 14};
-        if (power < 255) q_powers[b * 64 + lane] = (uint32_t)(power | (power - 4) << 8 | (power - 9) << 16) | (uint32_t)(power - 14) << 24;
-        else q_powers[b * 64 + lane] = 0xffffffffu;
+        if (power < 255) q_powers[wave * 64 + lane] = (uint32_t)(power | (power - 4) << 8 | (power - 9) << 16) | (uint32_t)(power - 14) << 24;
+        else q_powers[wave * 64 + lane] = 0xffffffffu;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const float scale = __uint_as_float((uint32_t)(power - down[t]) << 23);
             const u6 codes = to_fp6(x, scale);
 #pragma unroll
-            for (int w = 0; w < 6; ++w) q_codes[((b * 4 + t) * 6 + w) * 64 + lane] = codes[w];
+            for (int w = 0; w < 6; ++w) q_codes[((wave * 4 + t) * 6 + w) * 64 + lane] = codes[w];
             if (t < 3) {
                 const float32_t back = from_fp6(codes, scale);
 #pragma unroll
@@ -366,6 +460,38 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     for (int it = 0; it < n_it; ++it) {
         const int e0 = pb0 + 2 * (wave + it * WAVES);
         const int ea = entry_pos(e0), eb = entry_pos(min(e0 + 1, e_hi - 1));
+        if constexpr (NEW) { // the new rows' codes, from LDS
+            if (appends && e0 + 1 >= e_new && e0 <= e_last) { // uniform
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int from = entry_pos(e0 + h) - p_new, row = from + n;
+                    if (row >= 0 && row < C) {
+                        const uint8_t *to = new_rows + row * NEW_ROW;
+                        uint32_t powers = 0;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const u2 *c2 = reinterpret_cast<const u2 *>(to + (4 * b + jk) * 16);
+                            const u2 c0 = c2[0], c1 = c2[1];
+                            kc[h][b][0] = c0[0], kc[h][b][1] = c0[1], kc[h][b][2] = c1[0], kc[h][b][3] = c1[1];
+                            powers |= (uint32_t)to[AT_KP + 4 * b + jk] << (8 * b);
+                        }
+                        kp[h] = powers;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int vrow = from + j * 4 + i;
+                        if (vrow < 0 || vrow >= C) continue;
+                        const uint8_t *to = new_rows + vrow * NEW_ROW;
+                        const uint32_t keep = ~(255u << (8 * i));
+#pragma unroll
+                        for (int t = 0; t < G; ++t) {
+                            vc[h][t] = (vc[h][t] & keep) | (uint32_t)to[AT_V + t * 16 + n] << (8 * i);
+                            vp[h][t] = (vp[h][t] & keep) | (uint32_t)to[AT_VP + t] << (8 * i);
+                        }
+                    }
+                }
+            }
+        }
         // ---- scores of the pair: keys 4j .. 4j + 3 of slot n, of page a, then b
         float4_t s[2];
 #pragma unroll
@@ -383,7 +509,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         }
         if (it + 1 < n_it) {
             if (((it + 1) & 31) == 0) fetch_ids(it + 1);
-            load_k(it + 1);
+            load_k(it + 1, page_id(it + 1, 0), page_id(it + 1, 1));
         }
         // ---- softmax in base 2; keys outside the slot's range get no weight, and where no slot of the workgroup attends them (rows past the
         // length, before the window, of a page that is not there) V's powers are cleared as well: 0 x NaN is NaN
@@ -462,13 +588,13 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * t], 0, 0, 0);
             o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * t + 1], 0, 0, 0);
         }
-        if (it + 1 < n_it) load_v(it + 1);
+        if (it + 1 < n_it) load_v(it + 1, page_id(it + 1, 0), page_id(it + 1, 1));
     }
     l_run = rows_sum(l_run);
 
     // ---- the wavefronts' states meet in LDS, four columns a thread
-    float *xo = reinterpret_cast<float *>(lds + Fp4Lds<P, WAVES>::QUERIES + Fp4Lds<P, WAVES>::POWERS); // [WAVES][rows][OSTRIDE]
-    float *xm = xo + WAVES * rows * OSTRIDE, *xl = xm + WAVES * rows;                                  // [WAVES][rows]
+    float *xo = reinterpret_cast<float *>(lds + Fp4Lds<P, WAVES>::states(NEW ? C : 0)); // [WAVES][rows][OSTRIDE]
+    float *xm = xo + WAVES * rows * OSTRIDE, *xl = xm + WAVES * rows;                   // [WAVES][rows]
     if (n < rows) {
         float *dst = xo + (wave * rows + n) * OSTRIDE + j * 4;
 #pragma unroll
@@ -522,33 +648,42 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     }
 }
 
-template <int P, int WAVES, bool MQ, bool RING>
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS>
 __global__ __launch_bounds__(WAVES * 64) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
-    fp4_attention_body<P, WAVES, MQ, RING>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
+    fp4_attention_body<P, WAVES, MQ, RING, ROWS>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
-template <int P, int WAVES, bool MQ, bool RING>
+// Several sequences of the same model layer: grid z is the sequence, grid x covers the largest number of splits
+template <int P, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void fp4_attention_batch_kernel(DecodeBatchArgs b) {
+    const DecodeArgs &a = b.seq[blockIdx.z];
+    if ((int)blockIdx.x >= a.splits) return;
+    fp4_attention_body<P, WAVES, false, false>(a, nullptr, blockIdx.x, blockIdx.y, 0);
+}
+
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false>
 static hipError_t launch_fp4_of(const DecodeArgs &a, const ChunkPages &c, hipStream_t s) {
     static std::atomic<uint64_t> lds_ok{0}; // per instantiation
     {
-        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_kernel<P, WAVES, MQ, RING>), lds_ok);
+        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_kernel<P, WAVES, MQ, RING, ROWS>), lds_ok);
         if (e != hipSuccess) return e;
     }
     const int n_slots = a.n_queries * a.g.gqa;
     const dim3 grid((unsigned)a.splits, (unsigned)a.g.kv_heads, (unsigned)((n_slots + 15) / 16));
-    const size_t lds = Fp4Lds<P, WAVES>::bytes(n_slots < 16 ? n_slots : 16);
-    hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING>), grid, dim3(WAVES * 64), lds, s, a, c);
+    const size_t lds = Fp4Lds<P, WAVES>::bytes(n_slots < 16 ? n_slots : 16, ROWS ? a.n_queries : MQ ? 0 : 1);
+    hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING, ROWS>), grid, dim3(WAVES * 64), lds, s, a, c);
     return hipGetLastError();
 }
 template <int P, int WAVES>
 static hipError_t launch_fp4(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
+    if (a.k_new && (c || a.n_queries > MQ_APPEND_ROWS)) return hipErrorInvalidValue;
     if (c) return launch_fp4_of<P, WAVES, true, true>(a, *c, s);
-    if (a.n_queries * a.g.gqa > 16 || a.n_queries > 1) return launch_fp4_of<P, WAVES, true, false>(a, ChunkPages{}, s);
-    return launch_fp4_of<P, WAVES, false, false>(a, ChunkPages{}, s);
+    if (a.n_queries == 1 && a.g.gqa <= 16) return launch_fp4_of<P, WAVES, false, false>(a, ChunkPages{}, s);
+    return a.k_new ? launch_fp4_of<P, WAVES, true, false, true>(a, ChunkPages{}, s) : launch_fp4_of<P, WAVES, true, false>(a, ChunkPages{}, s);
 }
 
 hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
-    if (a.pre || a.k_new || a.split_base != 0) return hipErrorInvalidValue;
+    if (a.pre || a.split_base != 0) return hipErrorInvalidValue;
     switch (a.g.P) {
     case 32: return launch_fp4<32, 8>(a, c, s);
     case 64: return launch_fp4<64, 8>(a, c, s);
@@ -556,6 +691,32 @@ hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStr
     case 128: return launch_fp4<128, 8>(a, c, s);
     case 256: return launch_fp4<256, 8>(a, c, s);
     case 512: return launch_fp4<512, 4>(a, c, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+template <int P, int WAVES>
+static hipError_t launch_fp4_batch_of(const DecodeBatchArgs &b, int n_seq, int max_splits, hipStream_t s) {
+    static std::atomic<uint64_t> lds_ok{0}; // per instantiation
+    {
+        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_batch_kernel<P, WAVES>), lds_ok);
+        if (e != hipSuccess) return e;
+    }
+    const Geom &g = b.seq[0].g;
+    const dim3 grid((unsigned)max_splits, (unsigned)g.kv_heads, (unsigned)n_seq);
+    const size_t lds = Fp4Lds<P, WAVES>::bytes(g.gqa, 1);
+    hipLaunchKernelGGL((fp4_attention_batch_kernel<P, WAVES>), grid, dim3(WAVES * 64), lds, s, b);
+    return hipGetLastError();
+}
+// One geometry, one query row a sequence, at most 16 heads a kv head (checked by the caller)
+hipError_t launch_fp4_batch(const DecodeBatchArgs &b, int n_seq, int max_splits, hipStream_t s) {
+    switch (b.seq[0].g.P) {
+    case 32: return launch_fp4_batch_of<32, 8>(b, n_seq, max_splits, s);
+    case 64: return launch_fp4_batch_of<64, 8>(b, n_seq, max_splits, s);
+    case 96: return launch_fp4_batch_of<96, 8>(b, n_seq, max_splits, s);
+    case 128: return launch_fp4_batch_of<128, 8>(b, n_seq, max_splits, s);
+    case 256: return launch_fp4_batch_of<256, 8>(b, n_seq, max_splits, s);
+    case 512: return launch_fp4_batch_of<512, 4>(b, n_seq, max_splits, s);
     default: return hipErrorInvalidValue;
     }
 }

@@ -406,7 +406,7 @@ bool over_rows(const Geom &g, const float *out, const float *rows, size_t n) {
 // 10.0/10.6, 16 over 380 16.3/15.1, 16 over 3000 69.8/71.6.)
 // The line in pages, 0 = none stays whole.
 int whole_step_pages(const Geom &g, int batch_wgs) {
-    if (!may_stay_whole() || g.f32 || g.P > 256) return 0;
+    if (!may_stay_whole() || g.f32 || g.fp4 || g.P > 256) return 0;
     return g.P <= 96 ? 24 + batch_wgs / 5 : g.P <= 128 ? 16 + batch_wgs / 5 : 10 + std::max(batch_wgs - 32, 0) / 6;
 }
 // Chunks in the multi-query mode, of `tiles` tiles of all kv heads: the more there are, the fewer splits would share the device. Split / whole, us of GPU
@@ -463,10 +463,10 @@ size_t row_bytes(const Geom &g) {
     return g.fp4 ? (hd + 1) / 2 + (hd + 31) / 32 : hd * (g.f32 ? 4 : 2);
 }
 bool uses_flash(const skv_layer *L) { return skv_flag_flash_sdpa_enabled() && L->g.P <= 512; }
-// The attention launch of a decode step can append the row itself: always on bf16 layers,
+// The attention launch of a decode step can append the row itself: always on bf16 and 4-bit layers,
 // on f32 layers where the f32 decode kernel serves the shape (head_dim up to 256, at most 16
 // heads per group).
-bool fused_append_built(const skv_layer *L) { return !L->g.fp4 && (!L->g.f32 || (L->g.P <= 256 && L->g.gqa <= 16)); }
+bool fused_append_built(const skv_layer *L) { return !L->g.f32 || (L->g.P <= 256 && L->g.gqa <= 16); }
 // The fused pre-KV step is built for bf16 layers up to head_dim 512 and for f32 layers up to
 // head_dim 256; wide f32 heads take the separate norm/rotation launches.
 bool wide_f32_heads(const skv_layer *L) { return L->g.f32 && L->g.P > 256; }
@@ -529,8 +529,9 @@ void fill_decode_args(const skv_layer *L, const float *q_dev, float *out_dev, si
 // The same for the 4-bit element, whose kernel walks the pages that the queries can see as a list in the order of positions: a.page_first is the
 // first one's number, a.ring_base its place in the table, a.ring_t where the table comes round. A wavefront takes a pair of pages at a
 // time; no split leaves one without.
-void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_t window_start, size_t n_queries, DecodeArgs &a) {
-    fill_decode_args(L, q_dev, out_dev, window_start, nullptr, nullptr, n_queries, decode_target_wgs(), a);
+void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_t window_start, const float *k_new, const float *v_new,
+                   size_t n_queries, size_t target_wgs, DecodeArgs &a) {
+    fill_decode_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, target_wgs, a);
     const Geom &g = L->g;
     // (a decode step's window_start is the caller's, who may want less than the layer's window or all that a ring holds)
     const size_t first = (n_queries > 1 ? std::max(window_start, skv_window_start(L->len - n_queries, L->window)) : window_start) / 16;
@@ -540,7 +541,7 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.ring_t = ring_pages > 0 ? ring_pages : INT32_MAX;
     a.n_pages = (int)((L->len + 15) / 16 - first);
     a.waves = g.P > 256 ? 4 : 8;
-    a.splits = choose_splits(L, (a.n_pages + 1) / 2, L->len - window_start, a.waves, decode_target_wgs());
+    a.splits = choose_splits(L, (a.n_pages + 1) / 2, L->len - window_start, a.waves, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
         a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(512 / tiles, 1));
@@ -878,9 +879,9 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
     }
     const bool use_flash = uses_flash(L) || n_queries > 1;
     if (g.fp4 && use_flash) {
-        if (k_new || v_new || pre) return fail(SKV_ERR_CONFIG, "KV 4 bits: étape fusionnée non construite pour cette forme");
+        if (pre) return fail(SKV_ERR_CONFIG, "KV 4 bits: étape fusionnée non construite pour cette forme");
         DecodeArgs a{};
-        fill_fp4_args(L, q_dev, out_dev, window_start, n_queries, a);
+        fill_fp4_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, decode_target_wgs(), a);
         if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
         if (n_queries > 1 && a.splits > 1) {
             rc = multi_query_partials(L, s, (size_t)a.splits, n_queries, a, lease);
@@ -893,7 +894,7 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         rc = place(a.splits, a.out);
         if (rc) return rc;
         SKV_HIP(launch_fp4_attention(a, nullptr, s));
-        if (a.splits > 1) SKV_HIP(n_queries > 1 ? launch_merge_rows(a, s) : launch_merge(a, s));
+        if (a.splits > 1) SKV_HIP(a.splits <= 4 && n_queries > 1 ? launch_merge_rows(a, s) : launch_merge(a, s));
         return settle();
     }
     if (!use_flash) {
@@ -1703,8 +1704,8 @@ int32_t skv_prefill_chunk_device(skv_layer *L, skv_stream stream, const float *q
         }
         // a few rows over a full bf16 layer (a speculative verify, the rest of a prompt): the multi-query launch
         // appends them itself, as a decode step's does (its last query tile, which sees all of them, stores them)
-        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && !L->g.fp4 && tuning().fused_append &&
-            !context_over_rows(L, c, out, k, v) && !takes_tile_kernel(L->g, c, (L->len + c + 15) / 16)) {
+        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && tuning().fused_append &&
+            !context_over_rows(L, c, out, k, v) && (L->g.fp4 || !takes_tile_kernel(L->g, c, (L->len + c + 15) / 16))) {
             RowsAhead ahead(L, c);
             rc = encode_attention(L, as_stream(stream), q, out, 0, k, v, c);
             if (rc) return rc;
@@ -2183,9 +2184,9 @@ int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_s
             const size_t rows = L->g.ring_rows > 0 ? std::min<size_t>(L->len, (size_t)L->g.ring_rows) : L->len - ws;
             const size_t share = std::max<size_t>(decode_target_wgs() * ((rows + 15) / 16) / std::max<size_t>(pages_total, 1),
                                                   (size_t)L->g.kv_heads);
-            fill_decode_args(L, q_dev[first + i], out_dev[first + i], ws,
-                             reinterpret_cast<const float *>(k_dev[first + i]),
-                             reinterpret_cast<const float *>(v_dev[first + i]), 1, share, b.seq[i], false, whole_ok, wgs);
+            const float *k = reinterpret_cast<const float *>(k_dev[first + i]), *v = reinterpret_cast<const float *>(v_dev[first + i]);
+            if (L->g.fp4) fill_fp4_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i]);
+            else fill_decode_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], false, whole_ok, wgs);
         };
         bool split = false, unsplit = false;
         for (size_t i = 0; i < n; ++i) {
@@ -2369,7 +2370,7 @@ int32_t skv_probe_merge_device(skv_layer *L, skv_stream stream, float *out_dev) 
     if (!uses_flash(L)) return fail(SKV_ERR_CONFIG, "probe: noyau matriciel seulement");
     DecodeArgs a{};
     const size_t ws = skv_window_start(L->len - 1, L->window);
-    if (L->g.fp4) fill_fp4_args(L, nullptr, out_dev, ws, 1, a);
+    if (L->g.fp4) fill_fp4_args(L, nullptr, out_dev, ws, nullptr, nullptr, 1, decode_target_wgs(), a);
     else fill_decode_args(L, nullptr, out_dev, ws, nullptr, nullptr, 1, decode_target_wgs(), a, false, true);
     if (a.splits > 1) SKV_HIP(launch_merge(a, as_stream(stream)));
     return SKV_OK;

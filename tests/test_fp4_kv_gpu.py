@@ -206,3 +206,51 @@ def test_chunks(state, dims, base, n):
     p.chunk(n)
     p.step()
     p.check_rows()
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512), (40, 2, 128)], ids=str)
+def test_batches_of_sequences(state, dims):
+    """Each sequence's context is its own, whatever lies beside it: lengths from none to some thousand, more than a launch takes."""
+    lengths = [0, 1, 15, 16, 17, 300, 2000, 31, 5, 900, 64, 33, 48, 7, 129, 640, 3, 255]
+    seqs = [Pair(state, dims, n + 4, seed=i) for i, n in enumerate(lengths)]
+    for p, n in zip(seqs, lengths):
+        p.append(n)
+    for _ in range(2):
+        rows = [p.new(1) for p in seqs]
+        dev = [[_dev(a) for a in r] for r in rows]
+        outs = [torch.full((p.q_dim,), float("nan"), device="cuda") for p in seqs]
+        skv.encode_decode_step_batch([p.kv for p in seqs], _stream(), [d[0].data_ptr() for d in dev], [d[1].data_ptr() for d in dev],
+                                     [d[2].data_ptr() for d in dev], [o.data_ptr() for o in outs])
+        torch.cuda.synchronize()
+        for p, (k, v, q), o in zip(seqs, rows, outs):
+            p.holds(k, v)
+            p.check(q, o.cpu().numpy()[None])
+    for p in seqs:
+        p.check_rows()
+
+
+def test_batches_over_wrapped_rings(state):
+    dims = (16, 8, 256)
+    lengths = [200, 10, 64, 131]
+    seqs = [Pair(state, dims, 300, seed=i, window=48, rollback=0) for i in range(4)]
+    for p, n in zip(seqs, lengths):
+        p.append(n)
+    for _ in range(3):
+        rows = [p.new(1) for p in seqs]
+        dev = [[_dev(a) for a in r] for r in rows]
+        outs = [torch.full((p.q_dim,), float("nan"), device="cuda") for p in seqs]
+        skv.encode_decode_step_batch([p.kv for p in seqs], _stream(), *([d[i].data_ptr() for d in dev] for i in range(3)),
+                                     [o.data_ptr() for o in outs])
+        torch.cuda.synchronize()
+        for p, (k, v, q), o in zip(seqs, rows, outs):
+            p.holds(k, v)
+            p.check(q, o.cpu().numpy()[None])
+
+
+def test_steps_that_may_not_allocate(state):
+    for dims, rows in (((32, 8, 128), 3000), ((16, 2, 256), 700), ((40, 2, 64), 90)):
+        p = Pair(state, dims, rows + 3, seed=rows)
+        p.append(rows)
+        for _ in range(3):
+            p.step(p.kv.encode_decode_step_static)
+        p.check_rows(rows - 8)
