@@ -1,7 +1,7 @@
 // gfx950 kernels of the 4-bit element (fp4_tile.h): rows stored as codes, read back, and attended.
 #include "append_tile.h"
 #include "fp4_tile.h"
-#include "pre_kv.h"
+#include "lds_copy.h"
 
 namespace skv {
 
@@ -9,7 +9,6 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float float4_t;
 typedef __attribute__((ext_vector_type(16))) float float16_t;
-typedef __attribute__((ext_vector_type(32))) float float32_t;
 typedef __attribute__((ext_vector_type(2))) uint32_t u2;
 typedef __attribute__((ext_vector_type(4))) uint32_t u4;
 typedef __attribute__((ext_vector_type(6))) uint32_t u6;
@@ -25,24 +24,14 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(power), B));
 }
 
-// 32 values as e2m3 codes of x / scale, and the codes' values. These conversions take several passes and write their results as they go: a result
-// register that is also an operand is read back changed (seen: the scale in the first result register, the values after the first few wrong),
-// and the compiler does not know. Operands are kept alive behind the instruction, so that they have registers of their own.
-__device__ __forceinline__ u6 to_fp6(const float (&x)[32], float scale) {
-    float16_t even, odd; // they take turns in the result
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        even[e] = x[2 * e];
-        odd[e] = x[2 * e + 1];
-    }
-    u6 codes = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
-    asm volatile("" : "+v"(codes) : "v"(even), "v"(odd), "v"(scale));
-    return codes;
-}
-__device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
-    float32_t x = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(codes, scale);
-    asm volatile("" : "+v"(x) : "v"(codes), "v"(scale));
-    return x;
+// Four digits between -16 and 16, a byte each and 16 too large, as e2m3 codes of an eighth of them, side by side in 24 bits: sign and magnitude,
+// which for whole eighths up to 2 is the code's last five bits as they stand.
+__device__ __forceinline__ uint32_t fp6_codes_of(uint32_t u) {
+    const uint32_t half = u >> 1, up = ((u | half) & 0x10101010u) >> 4, mask = (up << 8) - up; // not negative: 255
+    const uint32_t pos = (u & 0x0f0f0f0fu) | (half & 0x10101010u), neg = 0x30303030u - u;
+    const uint32_t c = (pos & mask) | (neg & ~mask);
+    const uint32_t two = (c & 0x003f003fu) | (c >> 2 & 0x0fc00fc0u);
+    return (two & 0xfffu) | (two >> 4 & 0xfff000u);
 }
 
 } // namespace
@@ -183,9 +172,9 @@ hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
 // context. The wavefronts of a workgroup hold the same slots and walk the page pairs in turn.
 //
 // S^T = K . Q^T takes the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4 with K as e2m1 (a lane's 16 bytes are a row's 32 dims of
-// a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as four terms in e2m3 with a power a group and term.
-// A term leaves at most 2^-3, then 2^-7, 2^-12, 2^-17 of the group's power, 2^-19 of its largest value: what two
-// bf16 terms leave of each value. Four such products of 128 dims take 64 cycles, two of bf16 (eight instructions of 32 dims) 128, and
+// a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as four terms in e2m3 with a power a group and term:
+// digits of base 32 of the values as whole numbers of 20 bits, off by at most 2^-19 of the group's largest value, about what two bf16 terms
+// leave of each value. Four such products of 128 dims take 64 cycles, two of bf16 (eight instructions of 32 dims) 128, and
 // the codes would have to be converted.
 // O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to bf16 (exact) in registers, per page and group of dims
 // four conversions, four scales and four byte selections for eight values a lane, and P is two bf16 terms; a pair of pages is the 32 keys of
@@ -221,15 +210,33 @@ __device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
     return (zero >> 7) * 255u;
 }
 
-// LDS in words: [NB][4 terms][6 words][64 lanes] of the queries, [NB][64] their powers; of the new rows, per row, K codes, V codes, K
-// powers, V powers; then the wavefronts' states
+// LDS in bytes: the queries' terms ([NB][4 terms][64 lanes][6 words]) and powers ([NB][64]); of the new rows, per row, K codes, V codes, K
+// powers, V powers; then per wavefront DEPTH pairs of pages, and in their place, when all are consumed, its state.
 template <int P, int WAVES>
 struct Fp4Lds {
-    static constexpr int NB = Fp4Tile<P>::NB, QUERIES = NB * 4 * 6 * 64, POWERS = NB * 64;
-    static constexpr int NEW_ROW = P + 2 * (P / 32); // bytes
-    __host__ __device__ static constexpr int states(int new_rows) { return QUERIES + POWERS + (new_rows * NEW_ROW + 15) / 16 * 4; }
-    static constexpr size_t bytes(int rows, int new_rows) { return ((size_t)states(new_rows) + (size_t)WAVES * rows * (P + 4 + 2)) * 4; }
+    static constexpr int NB = Fp4Tile<P>::NB, BLOCK = (4 * 6 + 1) * 64 * 4;
+    static constexpr int DEPTH = P <= 128 ? 4 : 2;
+    static constexpr int PAIR = 34 * P; // codes of K a, K b, V a, V b, then their powers
+    static constexpr int STATE = 16 * (P + 6) * 4; // [16 slots][P + 4], m, l
+    static constexpr int WAVE = DEPTH * PAIR > STATE ? DEPTH * PAIR : STATE;
+    static constexpr int NEW_ROW = P + 2 * (P / 32);
+    // (heads above 256 dims: no room for the queries beside the pairs, they lie in the wavefronts' second pairs until all have read them)
+    static constexpr bool SHARED = P > 256;
+    static_assert(!SHARED || (NB <= WAVES && BLOCK <= PAIR && DEPTH == 2), "a block of the queries in a wavefront's second pair");
+    __host__ __device__ static constexpr int pairs(int new_rows) { return (SHARED ? 0 : NB * BLOCK) + (new_rows * NEW_ROW + 15) / 16 * 16; }
+    __host__ __device__ static constexpr int block(int b, int new_rows) { return SHARED ? pairs(new_rows) + b * WAVE + PAIR : b * BLOCK; }
+    static constexpr size_t bytes(int new_rows) { return (size_t)pairs(new_rows) + (size_t)WAVES * WAVE; }
+    static_assert((SHARED ? 0 : NB * BLOCK) + MQ_APPEND_ROWS * NEW_ROW + 16 + WAVES * WAVE <= 160 * 1024, "it all fits a compute unit's LDS");
 };
+// 64 lanes' 16 (4) bytes, each from an address of its own, to lds + 16 (4) l (`lds` the same in every lane): see copy_to_lds
+__device__ __forceinline__ void gather_to_lds(const void *from, uint32_t lds) {
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
+}
+__device__ __forceinline__ void gather_words_to_lds(const void *from, uint32_t lds) {
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0");
+}
 
 // MQ: more than one query row, or more than 16 heads to a kv head: slots are (row, head) pairs, 16 to a workgroup (grid z). ROWS: the launch
 // stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one.
@@ -275,24 +282,30 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         const int page = a.table[place(e)];
         ids = RING && e >= n_old ? e - n_old : page;
     };
+    fetch_ids(0);
 
-    // ---- the rows that the launch stores: every workgroup that walks a page of theirs converts them and keeps the codes in LDS, from where its
-    // wavefronts patch what they load; the last tile of slots, which sees all of them, stores them. An eighth of a group a thread.
+    // ---- the rows that the launch stores. A decode step's one: the wavefront that walks its page converts it, an eighth of a group a lane.
+    // A chunk's: every workgroup that walks a page of theirs converts them all, and the last tile of slots, which sees all of them, stores
+    // them. The codes stay in LDS, from where a wavefront patches what it has loaded.
+    using L = Fp4Lds<P, WAVES>;
     constexpr bool NEW = !MQ || ROWS;
-    constexpr int NU = ROWS ? (MQ_APPEND_ROWS * 2 * G * 8 + THREADS - 1) / THREADS : 1;
-    static_assert(!NEW || NU * THREADS >= (ROWS ? MQ_APPEND_ROWS : 1) * 2 * G * 8, "every eighth of every new row has a thread");
+    constexpr int BY = ROWS ? THREADS : 64, MOST = ROWS ? MQ_APPEND_ROWS : 1, NU = (MOST * 2 * G * 8 + BY - 1) / BY;
     const int C = ROWS ? a.n_queries : 1;
     const int p_new = a.len - C, e_new = (p_new - pos0) >> 4, e_last = (a.len - 1 - pos0) >> 4;
     const bool appends = NEW && a.k_new != nullptr && e_last >= pb0 && e_new < pb1;
-    const bool stores = tile == (n_slots - 1) / 16;
+    const int w_new = ((e_new - pb0) >> 1) % WAVES; // (of a step)
+    const bool converts = appends && (ROWS || wave == w_new), stores = tile == (n_slots - 1) / 16;
+    const int by = ROWS ? tid : lane;
     float nx[NU][4];
     int page_a = 0, page_b = 0;
     if constexpr (NEW) {
-        if (appends) { // uniform
+        if (converts) { // uniform
             const bool vec = (g.head_dim & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.k_new) | reinterpret_cast<uintptr_t>(a.v_new)) & 15) == 0;
+            page_a = a.table[place(min(max(e_new, 0), e_hi - 1))];
+            page_b = ROWS ? a.table[place(min(max(e_last, 0), e_hi - 1))] : page_a;
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                const int idx = (tid + u * THREADS) >> 3, v = idx >= C * G, row = min((idx - v * C * G) / G, C - 1), d = (idx % G) * 32 + (tid & 7) * 4;
+                const int idx = (by + u * BY) >> 3, v = idx >= C * G, row = min((idx - v * C * G) / G, C - 1), d = (idx % G) * 32 + (tid & 7) * 4;
                 const float *src = (v ? a.v_new : a.k_new) + ((long)row * g.kv_heads + kvh) * g.head_dim;
                 if (vec) {
                     const float4_t x = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
@@ -305,151 +318,191 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             }
         }
     }
-    // ---- queries: block b by wavefront b % WAVES, lane (slot n, group j) its 32 dims
-    constexpr int QB = (NB + WAVES - 1) / WAVES;
-    static_assert(QB == 1, "a wavefront converts one block of the queries");
-    const float *qrow = a.q + (MQ ? context_row(g, kvh, my_slot) : (long)(kvh * g.gqa + my_slot)) * g.head_dim;
-    const int d0 = wave * 128 + j * 32;
-    float x[32];
-    if (wave < NB) {
-        if (a.q_vec) {
+    // ---- queries: four dims of a slot a thread, as eighths of a group (loads side by side: with a lane's 32 dims loaded by the lane, every lane
+    // on lines of its own, such loads were 1 to 2 us of a step)
+    constexpr int QU = (16 * P / 4 + THREADS - 1) / THREADS;
+    float4_t x[QU];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                const float4_t v = *reinterpret_cast<const float4_t *>(qrow + min(d0 + e, g.head_dim - 4));
+    for (int u = 0; u < QU; ++u) {
+        const int idx = tid + u * THREADS, slot = (idx >> 3) / G, d = (idx >> 3) % G * 32 + (tid & 7) * 4;
+        x[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (slot < rows) {
+            const float *qrow = a.q + (MQ ? context_row(g, kvh, tile * 16 + slot) : (long)(kvh * g.gqa + slot)) * g.head_dim;
+            if (a.q_vec) {
+                x[u] = *reinterpret_cast<const float4_t *>(qrow + min(d, g.head_dim - 4));
+            } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[e + k] = v[k];
+                for (int e = 0; e < 4; ++e) x[u][e] = qrow[min(d + e, g.head_dim - 1)];
+            }
+        }
+    }
+
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    uint8_t *new_rows = lds + (L::SHARED ? 0 : NB * L::BLOCK);
+    constexpr int NEW_ROW = L::NEW_ROW, AT_V = P / 2, AT_KP = P, AT_VP = P + G; // in a new row
+    const int n_new = NEW ? C : 0;
+    uint8_t *const mine = lds + L::pairs(n_new) + wave * L::WAVE; // this wavefront's pairs
+    const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + (uint32_t)(L::pairs(n_new) + wave * L::WAVE);
+    const int jk = G < 4 ? min(j, G - 1) : j; // (narrow heads: the lanes past the last group take it again, against queries of zero)
+
+    // A pair's copies to LDS: COPIES instructions. The heads' codes are whole KiBs from 128 dims on; below, and the powers always, a lane of an instruction
+    // may belong to any of the four tiles (K a, K b, V a, V b).
+    constexpr int CODE_COPIES = P >= 128 ? 4 * NB : P / 32, POWER_WORDS = P / 8, POWER_COPIES = (4 * POWER_WORDS + 63) / 64;
+    constexpr int COPIES = CODE_COPIES + POWER_COPIES;
+    const uint32_t page_bytes = (uint32_t)g.page_elems * 2;
+    const size_t codes_at = (size_t)kvh * fp4_code_bytes(P), powers_at = (size_t)g.kv_heads * fp4_code_bytes(P) + (size_t)kvh * fp4_power_bytes(P);
+    // where a lane's part of an instruction lies: in page a or b, so far from the page's start, of K's pool or V's
+    struct Part {
+        const uint8_t *from;
+        bool second, v;
+    };
+    auto part = [&](int u, int units, int bytes, size_t at) __attribute__((always_inline)) {
+        const int t = u / units;
+        const bool v = t >= 2;
+        return Part{reinterpret_cast<const uint8_t *>(v ? a.v_pool : a.k_pool) + at + (u - t * units) * bytes, (t & 1) != 0, v};
+    };
+    Part code_part[P >= 128 ? 1 : CODE_COPIES], power_part[POWER_COPIES];
+    if constexpr (P < 128) {
+#pragma unroll
+        for (int i = 0; i < CODE_COPIES; ++i) code_part[i] = part(i * 64 + lane, P / 2, 16, codes_at);
+    }
+#pragma unroll
+    for (int i = 0; i < POWER_COPIES; ++i) power_part[i] = part(min(i * 64 + lane, 4 * POWER_WORDS - 1), POWER_WORDS, 4, powers_at);
+    auto copy_pair = [&](int it) __attribute__((always_inline)) {
+        const uint32_t pa = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it) & 63), pb = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it + 1) & 63);
+        const int e0 = pb0 + 2 * (wave + it * WAVES);
+        const bool new_a = RING && min(e0, e_hi - 1) >= n_old, new_b = RING && min(e0 + 1, e_hi - 1) >= n_old;
+        const uint32_t to = mine_at + (uint32_t)((it % L::DEPTH) * L::PAIR);
+        const auto address = [&](const Part &p) __attribute__((always_inline)) {
+            const uint8_t *from = p.from + (uint64_t)(p.second ? pb : pa) * page_bytes;
+            if constexpr (RING) {
+                if (p.second ? new_b : new_a) from += p.v ? (const uint8_t *)c->v_new - (const uint8_t *)a.v_pool : (const uint8_t *)c->k_new - (const uint8_t *)a.k_pool;
+            }
+            return from;
+        };
+        if constexpr (P >= 128) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const bool is_new = t & 1 ? new_b : new_a;
+                const uint16_t *pool = t >= 2 ? (is_new ? c->v_new : a.v_pool) : (is_new ? c->k_new : a.k_pool);
+                const uint8_t *from = reinterpret_cast<const uint8_t *>(pool) + codes_at + (uint64_t)(t & 1 ? pb : pa) * page_bytes;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) MQ ? copy_to_lds(from, (uint32_t)lane * 16, to + t * 8 * P, b) : copy_to_lds_once(from, (uint32_t)lane * 16, to + t * 8 * P, b);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = qrow[min(d0 + e, g.head_dim - 1)];
+            for (int i = 0; i < CODE_COPIES; ++i) gather_to_lds(address(code_part[i]), to + i * 1024);
         }
-    }
-
-    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    uint8_t *new_rows = reinterpret_cast<uint8_t *>(lds + Fp4Lds<P, WAVES>::QUERIES + Fp4Lds<P, WAVES>::POWERS);
-    constexpr int NEW_ROW = Fp4Lds<P, WAVES>::NEW_ROW, AT_V = P / 2, AT_KP = P, AT_VP = P + G; // in a new row
-    uint32_t *q_codes = lds, *q_powers = lds + Fp4Lds<P, WAVES>::QUERIES;
-    uint32_t kc[2][NB][4], kp[2], vc[2][G], vp[2][G];
-    const int jk = G < 4 ? min(j, G - 1) : j; // (narrow heads: the lanes past the last group take it again, against queries of zero)
-    auto page_id = [&](int it, int h) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ids, (2 * it + h) & 63); };
-    auto load_k = [&](int it, int page0, int page1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int page = h ? page1 : page0;
-            const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->k_new : a.k_pool;
-            const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) load_words<4>(kc[h][b], cp + ((4 * b + jk) * 16 + n) * 16);
-            if constexpr (NB == 1) kp[h] = pp[jk * 16 + n];
-            else if constexpr (NB == 2) kp[h] = reinterpret_cast<const uint16_t *>(pp)[j * 16 + n];
-            else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
-        }
+        for (int i = 0; i < POWER_COPIES; ++i)
+            if (i * 64 + 64 <= 4 * POWER_WORDS || i * 64 + lane < 4 * POWER_WORDS) gather_words_to_lds(address(power_part[i]), to + 32 * P + i * 256);
     };
-    auto load_v = [&](int it, int page0, int page1) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int page = h ? page1 : page0;
-            const uint16_t *pool = RING && min(pb0 + 2 * (wave + it * WAVES) + h, e_hi - 1) >= n_old ? c->v_new : a.v_pool;
-            const uint8_t *cp = fp4_codes(pool, g, page, kvh), *pp = fp4_powers(pool, g, page, kvh);
-#pragma unroll
-            for (int v = 0; v < VL; ++v) {
-                uint32_t w[U];
-                load_words<U>(w, cp + (v * 64 + lane) * U * 4);
-#pragma unroll
-                for (int u = 0; u < U; ++u) vc[h][v * U + u] = w[u];
-            }
-            load_words<G>(vp[h], pp + j * G * 4);
-        }
-    };
-    // The first pair's places come through the scalar unit, counted apart from the loads above: its requests do not wait for them.
-    {
-        const int ea = min(pb0 + 2 * wave, e_hi - 1), eb = min(pb0 + 2 * wave + 1, e_hi - 1);
-        const int pa = RING && ea >= n_old ? ea - n_old : table_entry<true>(a.table, place(ea));
-        const int pb = RING && eb >= n_old ? eb - n_old : table_entry<true>(a.table, place(eb));
-        if constexpr (NEW) {
-            page_a = table_entry<true>(a.table, place(min(max(e_new, 0), e_hi - 1)));
-            page_b = table_entry<true>(a.table, place(min(max(e_last, 0), e_hi - 1)));
-        }
-        load_k(0, pa, pb);
-        load_v(0, pa, pb);
-    }
-    fetch_ids(0);
-
+    // everything asked for so far has arrived (the compiler does not know of the copies: a wait of its own behind them would be for all of them)
+    asm volatile("" : "+v"(ids), "+v"(page_a), "+v"(page_b));
     if constexpr (NEW) {
-        if (appends) { // uniform
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const int idx = (tid + u * THREADS) >> 3, v = idx >= C * G, row = (idx - v * C * G) / G, t = idx % G, o8 = tid & 7, d = t * 32 + o8 * 4;
-                const bool real = idx < 2 * C * G;
+        for (int u = 0; u < NU; ++u) asm volatile("" : "+v"(nx[u][0]), "+v"(nx[u][1]), "+v"(nx[u][2]), "+v"(nx[u][3]));
+    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) nx[u][e] = real && d + e < g.head_dim ? nx[u][e] : 0.0f;
-                uint32_t power;
-                const uint32_t codes = fp4_codes_of(nx[u], power);
-                const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
-                if (!real) continue;
-                uint8_t *to = new_rows + row * NEW_ROW;
-                const int e = (p_new + row - pos0) >> 4, r = (p_new + row) & 15, page = e == e_new ? page_a : page_b;
-                const bool store = stores && e >= pb0 && e < pb1;
-                uint16_t *pool = const_cast<uint16_t *>(v ? a.v_pool : a.k_pool);
-                uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
-                if (!v) {
-                    *reinterpret_cast<uint16_t *>(to + t * 16 + o8 * 2) = (uint16_t)codes;
-                    if (o8 == 0) to[AT_KP + t] = (uint8_t)power;
-                    if (store) {
-                        *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
-                        if (o8 == 0) pp[k4_power(P, r, t)] = (uint8_t)power;
-                    }
-                } else if (o8 < 4) {
-                    const uint32_t word = nibbles_apart(codes) | nibbles_apart(other) << 4;
-                    *reinterpret_cast<uint32_t *>(to + AT_V + t * 16 + o8 * 4) = word;
-                    if (o8 == 0) to[AT_VP + t] = (uint8_t)power;
-                    if (store) {
+    for (int u = 0; u < QU; ++u) asm volatile("" : "+v"(x[u]));
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) cp[v4_code(P, r, d + k)] = (uint8_t)(word >> (8 * k));
-                        if (o8 == 0) pp[v4_power(P, r, t)] = (uint8_t)power;
-                    }
+    for (int i = 0; i < (L::SHARED ? 1 : L::DEPTH); ++i)
+        if (i < n_it) copy_pair(i); // uniform
+
+    auto convert_rows = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int idx = (by + u * BY) >> 3, v = idx >= C * G, row = (idx - v * C * G) / G, t = idx % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+            const bool real = idx < 2 * C * G;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nx[u][e] = real && d + e < g.head_dim ? nx[u][e] : 0.0f;
+            uint32_t power;
+            const uint32_t codes = fp4_codes_of(nx[u], power);
+            const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
+            if (!real) continue;
+            uint8_t *to = new_rows + row * NEW_ROW;
+            const int e = (p_new + row - pos0) >> 4, r = (p_new + row) & 15, page = e == e_new ? page_a : page_b;
+            const bool store = stores && e >= pb0 && e < pb1;
+            uint16_t *pool = const_cast<uint16_t *>(v ? a.v_pool : a.k_pool);
+            uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
+            if (!v) {
+                *reinterpret_cast<uint16_t *>(to + t * 16 + o8 * 2) = (uint16_t)codes;
+                if (o8 == 0) to[AT_KP + t] = (uint8_t)power;
+                if (store) {
+                    *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
+                    if (o8 == 0) pp[k4_power(P, r, t)] = (uint8_t)power;
+                }
+            } else if (o8 < 4) {
+                const uint32_t word = nibbles_apart(codes) | nibbles_apart(other) << 4;
+                *reinterpret_cast<uint32_t *>(to + AT_V + t * 16 + o8 * 4) = word;
+                if (o8 == 0) to[AT_VP + t] = (uint8_t)power;
+                if (store) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) cp[v4_code(P, r, d + k)] = (uint8_t)(word >> (8 * k));
+                    if (o8 == 0) pp[v4_power(P, r, t)] = (uint8_t)power;
                 }
             }
         }
+    };
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+        const int idx = tid + u * THREADS, slot = (idx >> 3) / G, t = (idx >> 3) % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+        uint32_t *const to = reinterpret_cast<uint32_t *>(lds + L::block(t >> 2, n_new)); // of the block, lane (slot, t % 4)
+        const int at = (t & 3) * 16 + slot;
+        if (slot >= rows) {
+            if (slot < 16 && o8 == 0) to[4 * 6 * 64 + at] = 0; // (nothing reads what becomes of it)
+            continue;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[u][e] = d + e < g.head_dim ? x[u][e] : 0.0f;
+            top = __uint_as_float(max(__float_as_uint(top), magnitude(x[u][e])));
+        }
+        const uint32_t most = max_of_8(magnitude(top * a.qscale));
+        // the values as whole numbers X of 20 bits, |X| <= 2^19, in digits of base 32 between -16 and 15 (the first: 16). A float at
+        // 1.5 * 2^23 + (X + 16 (1 + 32 + 1024)) holds them in its last bits, 16 too large but for the first.
+        const int power = max((int)(most >> 23), 18);
+        const float scale = a.qscale * __uint_as_float((uint32_t)(272 - power) << 23);
+        uint32_t digits[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) digits[e] = __float_as_uint(__builtin_fmaf(x[u][e], scale, 12582912.0f + 16912.0f));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t four = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four |= (k == 0 ? (digits[e] >> 15 & 255u) - 112u : digits[e] >> (15 - 5 * k) & 31u) << (8 * e);
+            const uint32_t codes = fp6_codes_of(four); // 24 bits; four lanes' are three words
+            const uint32_t next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)codes, 0xf9, 0xf, 0xf, false); // of the lane after
+            const int o4 = o8 & 3;
+            if (o4 < 3) to[(k * 64 + at) * 6 + (o8 >> 2) * 3 + o4] = codes >> (8 * o4) | next << (24 - 8 * o4);
+        }
+        if (o8 == 0)
+            to[4 * 6 * 64 + at] = most >= 0x7f800000u ? 0xffffffffu : (uint32_t)(power | (power - 5) << 8 | (power - 10) << 16) | (uint32_t)(power - 15) << 24;
     }
-    if (wave < NB) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            x[e] = n < rows && d0 + e < g.head_dim ? x[e] * a.qscale : 0.0f;
-            top = max(top, magnitude(x[e]));
-        }
-        // the first term's power is the smallest with the largest value <= 7.5 of it
-        int power = 255;
-        if (top < 0x7f800000u) power = max((int)((top + 0x0fffffu) >> 23) - 2, 18);
-        constexpr int down[4] = {0, 4, 9, 14};
-        if (power < 255) q_powers[wave * 64 + lane] = (uint32_t)(power | (power - 4) << 8 | (power - 9) << 16) | (uint32_t)(power - 14) << 24;
-        else q_powers[wave * 64 + lane] = 0xffffffffu;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const float scale = __uint_as_float((uint32_t)(power - down[t]) << 23);
-            const u6 codes = to_fp6(x, scale);
-#pragma unroll
-            for (int w = 0; w < 6; ++w) q_codes[((wave * 4 + t) * 6 + w) * 64 + lane] = codes[w];
-            if (t < 3) {
-                const float32_t back = from_fp6(codes, scale);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] -= back[e];
-            }
-        }
+    if constexpr (ROWS) {
+        if (converts) convert_rows(); // uniform
     }
     __syncthreads();
+    if constexpr (NEW && !ROWS) {
+        if (converts) convert_rows(); // uniform (for itself)
+    }
     int8v_t q_term[NB][4];
     uint32_t q_power[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        q_power[b] = q_powers[b * 64 + lane];
+        const uint32_t *terms = reinterpret_cast<const uint32_t *>(lds + L::block(b, n_new));
+        q_power[b] = G >= 4 || j < G ? terms[4 * 6 * 64 + lane] : 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int w = 0; w < 6; ++w) q_term[b][t][w] = (int)q_codes[((b * 4 + t) * 6 + w) * 64 + lane];
+            for (int w = 0; w < 6; ++w) q_term[b][t][w] = G >= 4 || j < G ? (int)terms[(t * 64 + lane) * 6 + w] : 0;
             q_term[b][t][6] = q_term[b][t][7] = 0;
         }
+    }
+    if constexpr (L::SHARED) {
+        __syncthreads();
+        if (1 < n_it) copy_pair(1);
     }
 
     float4_t o[NT];
@@ -460,6 +513,28 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     for (int it = 0; it < n_it; ++it) {
         const int e0 = pb0 + 2 * (wave + it * WAVES);
         const int ea = entry_pos(e0), eb = entry_pos(min(e0 + 1, e_hi - 1));
+        // ---- the pair, from LDS: the copies behind its own may still be on their way
+        if (it + L::DEPTH <= n_it) copies_left<(L::DEPTH - 1) * COPIES>(); // uniform
+        else copies_landed();
+        const uint8_t *const pair = mine + (it % L::DEPTH) * L::PAIR;
+        uint32_t kc[2][NB][4], kp[2], vc[2][G], vp[2][G];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) load_words<4>(kc[h][b], pair + h * 8 * P + ((4 * b + jk) * 16 + n) * 16);
+            const uint8_t *pp = pair + 32 * P + h * (P / 2);
+            if constexpr (NB == 1) kp[h] = pp[jk * 16 + n];
+            else if constexpr (NB == 2) kp[h] = reinterpret_cast<const uint16_t *>(pp)[j * 16 + n];
+            else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
+#pragma unroll
+            for (int v = 0; v < VL; ++v) {
+                uint32_t w[U];
+                load_words<U>(w, pair + (2 + h) * 8 * P + (v * 64 + lane) * U * 4);
+#pragma unroll
+                for (int u = 0; u < U; ++u) vc[h][v * U + u] = w[u];
+            }
+            load_words<G>(vp[h], pair + 33 * P + h * (P / 2) + j * G * 4);
+        }
         if constexpr (NEW) { // the new rows' codes, from LDS
             if (appends && e0 + 1 >= e_new && e0 <= e_last) { // uniform
 #pragma unroll
@@ -506,10 +581,6 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][1], s[h], 4, 2, 0, kpow, 1, (int)q_power[b]);
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][0], s[h], 4, 2, 0, kpow, 0, (int)q_power[b]);
             }
-        }
-        if (it + 1 < n_it) {
-            if (((it + 1) & 31) == 0) fetch_ids(it + 1);
-            load_k(it + 1, page_id(it + 1, 0), page_id(it + 1, 1));
         }
         // ---- softmax in base 2; keys outside the slot's range get no weight, and where no slot of the workgroup attends them (rows past the
         // length, before the window, of a page that is not there) V's powers are cleared as well: 0 x NaN is NaN
@@ -588,20 +659,29 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * t], 0, 0, 0);
             o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * t + 1], 0, 0, 0);
         }
-        if (it + 1 < n_it) load_v(it + 1, page_id(it + 1, 0), page_id(it + 1, 1));
+        // its place is free for the pair DEPTH further
+        if (it + L::DEPTH < n_it) {
+            if (((it + L::DEPTH) & 31) == 0) {
+                fetch_ids(it + L::DEPTH);
+                asm volatile("" : "+v"(ids)); // (waited for here: where the paths join it would be for every pair's copies)
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (all of it is read)
+            copy_pair(it + L::DEPTH);
+        }
     }
     l_run = rows_sum(l_run);
 
     // ---- the wavefronts' states meet in LDS, four columns a thread
-    float *xo = reinterpret_cast<float *>(lds + Fp4Lds<P, WAVES>::states(NEW ? C : 0)); // [WAVES][rows][OSTRIDE]
-    float *xm = xo + WAVES * rows * OSTRIDE, *xl = xm + WAVES * rows;                   // [WAVES][rows]
+    // [WAVES] of [rows][OSTRIDE], m [rows], l [rows]
+    constexpr int STATE = L::WAVE / 4; // floats from one wavefront's to the next's
+    float *const x0 = reinterpret_cast<float *>(lds + L::pairs(n_new)), *const xm = x0 + rows * OSTRIDE, *const xl = xm + rows;
     if (n < rows) {
-        float *dst = xo + (wave * rows + n) * OSTRIDE + j * 4;
+        float *dst = x0 + wave * STATE + n * OSTRIDE + j * 4;
 #pragma unroll
         for (int t = 0; t < NT; ++t) *reinterpret_cast<float4_t *>(dst + t * 16) = o[t];
         if (j == 0) {
-            xm[wave * rows + n] = m_run;
-            xl[wave * rows + n] = l_run;
+            xm[wave * STATE + n] = m_run;
+            xl[wave * STATE + n] = l_run;
         }
     }
     __syncthreads();
@@ -612,7 +692,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         float mw[WAVES], mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            mw[w] = xm[w * rows + row];
+            mw[w] = xm[w * STATE + row];
             mx = fmaxf(mx, mw[w]);
         }
         const float m_safe = mx == -INFINITY ? 0.0f : mx;
@@ -621,8 +701,8 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             const float wgt = fast_exp2(mw[w] - m_safe);
-            acc += wgt * *reinterpret_cast<const float4_t *>(&xo[(w * rows + row) * OSTRIDE + c4]);
-            lsum += wgt * xl[w * rows + row];
+            acc += wgt * *reinterpret_cast<const float4_t *>(&x0[w * STATE + row * OSTRIDE + c4]);
+            lsum += wgt * xl[w * STATE + row];
         }
         if (c4 >= g.head_dim) continue;
         const int slot = tile * 16 + row;
@@ -670,7 +750,7 @@ static hipError_t launch_fp4_of(const DecodeArgs &a, const ChunkPages &c, hipStr
     }
     const int n_slots = a.n_queries * a.g.gqa;
     const dim3 grid((unsigned)a.splits, (unsigned)a.g.kv_heads, (unsigned)((n_slots + 15) / 16));
-    const size_t lds = Fp4Lds<P, WAVES>::bytes(n_slots < 16 ? n_slots : 16, ROWS ? a.n_queries : MQ ? 0 : 1);
+    const size_t lds = Fp4Lds<P, WAVES>::bytes(ROWS ? a.n_queries : MQ ? 0 : 1);
     hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING, ROWS>), grid, dim3(WAVES * 64), lds, s, a, c);
     return hipGetLastError();
 }
@@ -684,12 +764,13 @@ static hipError_t launch_fp4(const DecodeArgs &a, const ChunkPages *c, hipStream
 
 hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
     if (a.pre || a.split_base != 0) return hipErrorInvalidValue;
+    const bool w8 = a.waves == 8;
     switch (a.g.P) {
-    case 32: return launch_fp4<32, 8>(a, c, s);
-    case 64: return launch_fp4<64, 8>(a, c, s);
-    case 96: return launch_fp4<96, 8>(a, c, s);
-    case 128: return launch_fp4<128, 8>(a, c, s);
-    case 256: return launch_fp4<256, 8>(a, c, s);
+    case 32: return w8 ? launch_fp4<32, 8>(a, c, s) : launch_fp4<32, 4>(a, c, s);
+    case 64: return w8 ? launch_fp4<64, 8>(a, c, s) : launch_fp4<64, 4>(a, c, s);
+    case 96: return w8 ? launch_fp4<96, 8>(a, c, s) : launch_fp4<96, 4>(a, c, s);
+    case 128: return w8 ? launch_fp4<128, 8>(a, c, s) : launch_fp4<128, 4>(a, c, s);
+    case 256: return w8 ? launch_fp4<256, 8>(a, c, s) : launch_fp4<256, 4>(a, c, s);
     case 512: return launch_fp4<512, 4>(a, c, s);
     default: return hipErrorInvalidValue;
     }
@@ -704,18 +785,19 @@ static hipError_t launch_fp4_batch_of(const DecodeBatchArgs &b, int n_seq, int m
     }
     const Geom &g = b.seq[0].g;
     const dim3 grid((unsigned)max_splits, (unsigned)g.kv_heads, (unsigned)n_seq);
-    const size_t lds = Fp4Lds<P, WAVES>::bytes(g.gqa, 1);
+    const size_t lds = Fp4Lds<P, WAVES>::bytes(1);
     hipLaunchKernelGGL((fp4_attention_batch_kernel<P, WAVES>), grid, dim3(WAVES * 64), lds, s, b);
     return hipGetLastError();
 }
 // One geometry, one query row a sequence, at most 16 heads a kv head (checked by the caller)
 hipError_t launch_fp4_batch(const DecodeBatchArgs &b, int n_seq, int max_splits, hipStream_t s) {
+    const bool w8 = b.seq[0].waves == 8;
     switch (b.seq[0].g.P) {
-    case 32: return launch_fp4_batch_of<32, 8>(b, n_seq, max_splits, s);
-    case 64: return launch_fp4_batch_of<64, 8>(b, n_seq, max_splits, s);
-    case 96: return launch_fp4_batch_of<96, 8>(b, n_seq, max_splits, s);
-    case 128: return launch_fp4_batch_of<128, 8>(b, n_seq, max_splits, s);
-    case 256: return launch_fp4_batch_of<256, 8>(b, n_seq, max_splits, s);
+    case 32: return w8 ? launch_fp4_batch_of<32, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<32, 4>(b, n_seq, max_splits, s);
+    case 64: return w8 ? launch_fp4_batch_of<64, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<64, 4>(b, n_seq, max_splits, s);
+    case 96: return w8 ? launch_fp4_batch_of<96, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<96, 4>(b, n_seq, max_splits, s);
+    case 128: return w8 ? launch_fp4_batch_of<128, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<128, 4>(b, n_seq, max_splits, s);
+    case 256: return w8 ? launch_fp4_batch_of<256, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<256, 4>(b, n_seq, max_splits, s);
     case 512: return launch_fp4_batch_of<512, 4>(b, n_seq, max_splits, s);
     default: return hipErrorInvalidValue;
     }

@@ -540,7 +540,8 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.ring_base = ring_pages > 0 ? (int)(first % (size_t)ring_pages) : (int)first;
     a.ring_t = ring_pages > 0 ? ring_pages : INT32_MAX;
     a.n_pages = (int)((L->len + 15) / 16 - first);
-    a.waves = g.P > 256 ? 4 : 8;
+    const size_t forced = tuning().forced_waves;
+    a.waves = g.P > 256 ? 4 : forced == 4 || forced == 8 ? (int)forced : 8;
     a.splits = choose_splits(L, (a.n_pages + 1) / 2, L->len - window_start, a.waves, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;

@@ -24,6 +24,20 @@ __device__ __forceinline__ void copy_to_lds(const void *base, uint32_t lane_offs
     default: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
     }
 }
+// The same for what is read once: not kept in the caches.
+__device__ __forceinline__ void copy_to_lds_once(const void *base, uint32_t lane_offset, uint32_t lds, int kib = 0) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+    const uint64_t from = ((uint64_t)hi << 32) | lo;
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    switch (kib) {
+    case 0: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
+    case 1: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024 nt" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
+    case 2: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:2048 nt" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
+    default: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072 nt" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
+    }
+}
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // all but the wavefront's last N copies have landed
 template <int N>
