@@ -215,7 +215,7 @@ __device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
 template <int P, int WAVES>
 struct Fp4Lds {
     static constexpr int NB = Fp4Tile<P>::NB, BLOCK = (4 * 6 + 1) * 64 * 4;
-    static constexpr int DEPTH = P <= 128 ? 4 : 2;
+    static constexpr int DEPTH = 2;
     static constexpr int PAIR = 34 * P; // codes of K a, K b, V a, V b, then their powers
     static constexpr int STATE = 16 * (P + 6) * 4; // [16 slots][P + 4], m, l
     static constexpr int WAVE = DEPTH * PAIR > STATE ? DEPTH * PAIR : STATE;
@@ -405,9 +405,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     }
 #pragma unroll
     for (int u = 0; u < QU; ++u) asm volatile("" : "+v"(x[u]));
-#pragma unroll
-    for (int i = 0; i < (L::SHARED ? 1 : L::DEPTH); ++i)
-        if (i < n_it) copy_pair(i); // uniform
+    if (0 < n_it) copy_pair(0); // uniform
 
     auto convert_rows = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -500,16 +498,26 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             q_term[b][t][6] = q_term[b][t][7] = 0;
         }
     }
-    if constexpr (L::SHARED) {
-        __syncthreads();
-        if (1 < n_it) copy_pair(1);
-    }
+    if constexpr (L::SHARED) __syncthreads();
+    // (not with the first pair: a compute unit accepts requests as fast as memory answers, and no wavefront passes the barrier before its own
+    // are accepted)
+    if (1 < n_it) copy_pair(1);
 
     float4_t o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.0f;
 
+    // a pair whose place in LDS has been read
+    auto next_pair = [&](int it) __attribute__((always_inline)) {
+        if (it >= n_it) return; // uniform
+        if (((it) & 31) == 0) {
+            fetch_ids(it);
+            asm volatile("" : "+v"(ids)); // (waited for here: where the paths join it would be for every pair's copies)
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (all of this one is read)
+        copy_pair(it);
+    };
     for (int it = 0; it < n_it; ++it) {
         const int e0 = pb0 + 2 * (wave + it * WAVES);
         const int ea = entry_pos(e0), eb = entry_pos(min(e0 + 1, e_hi - 1));
@@ -582,6 +590,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][0], s[h], 4, 2, 0, kpow, 0, (int)q_power[b]);
             }
         }
+        if constexpr (P <= 128) next_pair(it + L::DEPTH);
         // ---- softmax in base 2; keys outside the slot's range get no weight, and where no slot of the workgroup attends them (rows past the
         // length, before the window, of a page that is not there) V's powers are cleared as well: 0 x NaN is NaN
         const int lo_b = RING ? (e0 + 1 >= n_old ? c->new_pos0 : INT32_MIN) : INT32_MIN;
@@ -659,15 +668,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * t], 0, 0, 0);
             o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * t + 1], 0, 0, 0);
         }
-        // its place is free for the pair DEPTH further
-        if (it + L::DEPTH < n_it) {
-            if (((it + L::DEPTH) & 31) == 0) {
-                fetch_ids(it + L::DEPTH);
-                asm volatile("" : "+v"(ids)); // (waited for here: where the paths join it would be for every pair's copies)
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (all of it is read)
-            copy_pair(it + L::DEPTH);
-        }
+        if constexpr (P > 128) next_pair(it + L::DEPTH);
     }
     l_run = rows_sum(l_run);
 
@@ -764,13 +765,12 @@ static hipError_t launch_fp4(const DecodeArgs &a, const ChunkPages *c, hipStream
 
 hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
     if (a.pre || a.split_base != 0) return hipErrorInvalidValue;
-    const bool w8 = a.waves == 8;
     switch (a.g.P) {
-    case 32: return w8 ? launch_fp4<32, 8>(a, c, s) : launch_fp4<32, 4>(a, c, s);
-    case 64: return w8 ? launch_fp4<64, 8>(a, c, s) : launch_fp4<64, 4>(a, c, s);
-    case 96: return w8 ? launch_fp4<96, 8>(a, c, s) : launch_fp4<96, 4>(a, c, s);
-    case 128: return w8 ? launch_fp4<128, 8>(a, c, s) : launch_fp4<128, 4>(a, c, s);
-    case 256: return w8 ? launch_fp4<256, 8>(a, c, s) : launch_fp4<256, 4>(a, c, s);
+    case 32: return launch_fp4<32, 8>(a, c, s);
+    case 64: return launch_fp4<64, 8>(a, c, s);
+    case 96: return launch_fp4<96, 8>(a, c, s);
+    case 128: return launch_fp4<128, 8>(a, c, s);
+    case 256: return launch_fp4<256, 8>(a, c, s);
     case 512: return launch_fp4<512, 4>(a, c, s);
     default: return hipErrorInvalidValue;
     }
@@ -791,13 +791,12 @@ static hipError_t launch_fp4_batch_of(const DecodeBatchArgs &b, int n_seq, int m
 }
 // One geometry, one query row a sequence, at most 16 heads a kv head (checked by the caller)
 hipError_t launch_fp4_batch(const DecodeBatchArgs &b, int n_seq, int max_splits, hipStream_t s) {
-    const bool w8 = b.seq[0].waves == 8;
     switch (b.seq[0].g.P) {
-    case 32: return w8 ? launch_fp4_batch_of<32, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<32, 4>(b, n_seq, max_splits, s);
-    case 64: return w8 ? launch_fp4_batch_of<64, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<64, 4>(b, n_seq, max_splits, s);
-    case 96: return w8 ? launch_fp4_batch_of<96, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<96, 4>(b, n_seq, max_splits, s);
-    case 128: return w8 ? launch_fp4_batch_of<128, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<128, 4>(b, n_seq, max_splits, s);
-    case 256: return w8 ? launch_fp4_batch_of<256, 8>(b, n_seq, max_splits, s) : launch_fp4_batch_of<256, 4>(b, n_seq, max_splits, s);
+    case 32: return launch_fp4_batch_of<32, 8>(b, n_seq, max_splits, s);
+    case 64: return launch_fp4_batch_of<64, 8>(b, n_seq, max_splits, s);
+    case 96: return launch_fp4_batch_of<96, 8>(b, n_seq, max_splits, s);
+    case 128: return launch_fp4_batch_of<128, 8>(b, n_seq, max_splits, s);
+    case 256: return launch_fp4_batch_of<256, 8>(b, n_seq, max_splits, s);
     case 512: return launch_fp4_batch_of<512, 4>(b, n_seq, max_splits, s);
     default: return hipErrorInvalidValue;
     }

@@ -540,9 +540,12 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.ring_base = ring_pages > 0 ? (int)(first % (size_t)ring_pages) : (int)first;
     a.ring_t = ring_pages > 0 ? ring_pages : INT32_MAX;
     a.n_pages = (int)((L->len + 15) / 16 - first);
-    const size_t forced = tuning().forced_waves;
-    a.waves = g.P > 256 ? 4 : forced == 4 || forced == 8 ? (int)forced : 8;
-    a.splits = choose_splits(L, (a.n_pages + 1) / 2, L->len - window_start, a.waves, target_wgs);
+    a.waves = g.P > 256 ? 4 : 8;
+    // A pair to each of half the wavefronts, where there are not more: with all eight busy a step takes longer, in us over 600, 2000 rows of
+    // q32/kv8/hd128 8.0/7.3, 8.2/7.3, of q16/kv8/hd256 9.8/8.4, 10.0/8.6; with two or three to a split as with four, but more partials.
+    // Whole while one pair each does it: over 250 rows 5.6/7.2, 7.7/8.1 (a second one each, over 400, 8.0/7.2, 9.7/8.2).
+    const int pairs = (a.n_pages + 1) / 2;
+    a.splits = pairs <= a.waves && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
         a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(512 / tiles, 1));
