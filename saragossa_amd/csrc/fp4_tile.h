@@ -74,6 +74,42 @@ __device__ __forceinline__ uint32_t nibbles_apart(uint32_t c) {
     c = (c | c << 8) & 0x00ff00ffu;
     return (c | c << 4) & 0x0f0f0f0fu;
 }
+// N words from p, as wide as its alignment (16 bytes of a multiple of four words, else 4 times their number) allows
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t *p) {
+    typedef __attribute__((ext_vector_type(2))) uint32_t u2;
+    typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) {
+        const u4 v = *reinterpret_cast<const u4 *>(p + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+    }
+    if constexpr (N == 3) { // (12 bytes apart: words)
+        typedef __attribute__((ext_vector_type(3), aligned(4))) uint32_t u3;
+        const u3 v = *reinterpret_cast<const u3 *>(p);
+        x[0] = v[0], x[1] = v[1], x[2] = v[2];
+    } else if constexpr (N == 2) {
+        const u2 v = *reinterpret_cast<const u2 *>(p);
+        x[0] = v[0], x[1] = v[1];
+    } else if constexpr (N == 1) {
+        x[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+// 255 in the bytes of w that are
+__device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
+    const uint32_t x = ~w, zero = ~(((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x | 0x7f7f7f7fu); // the top bit of the bytes of x that are 0
+    return (zero >> 7) * 255u;
+}
+
+// Byte B of two codes as two bf16 values, the low nibble's in the low half; `power` has the group's byte in its exponent field (the rest of
+// it is not looked at)
+template <int B>
+__device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(power), B));
+}
+
 #endif
 
 } // namespace skv

@@ -17,13 +17,6 @@ typedef __attribute__((ext_vector_type(8))) int int8v_t;
 namespace {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-// Byte B of two codes as two bf16 values, the low nibble's in the low half; `power` has the group's byte in its exponent field (the rest of
-// it is not looked at)
-template <int B>
-__device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(power), B));
-}
-
 // Four digits between -16 and 16, a byte each and 16 too large, as e2m3 codes of an eighth of them, side by side in 24 bits: sign and magnitude,
 // which for whole eighths up to 2 is the code's last five bits as they stand.
 __device__ __forceinline__ uint32_t fp6_codes_of(uint32_t u) {
@@ -184,32 +177,6 @@ template <int P>
 struct Fp4Tile {
     static constexpr int G = P / 32, U = fp4_quad(P), NB = (P + 127) / 128, VL = G / U;
 };
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t *p) {
-#pragma unroll
-    for (int i = 0; i + 4 <= N; i += 4) {
-        const u4 v = *reinterpret_cast<const u4 *>(p + 4 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i + e] = v[e];
-    }
-    if constexpr (N == 3) { // (12 bytes apart: words)
-        typedef __attribute__((ext_vector_type(3), aligned(4))) uint32_t u3;
-        const u3 v = *reinterpret_cast<const u3 *>(p);
-        x[0] = v[0], x[1] = v[1], x[2] = v[2];
-    } else if constexpr (N == 2) {
-        const u2 v = *reinterpret_cast<const u2 *>(p);
-        x[0] = v[0], x[1] = v[1];
-    } else if constexpr (N == 1) {
-        x[0] = *reinterpret_cast<const uint32_t *>(p);
-    }
-}
-
-// 255 in the bytes of w that are
-__device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
-    const uint32_t x = ~w, zero = ~(((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x | 0x7f7f7f7fu); // the top bit of the bytes of x that are 0
-    return (zero >> 7) * 255u;
-}
-
 // LDS in bytes: the queries' terms ([NB][4 terms][64 lanes][6 words]) and powers ([NB][64]); of the new rows, per row, K codes, V codes, K
 // powers, V powers; then per wavefront DEPTH pairs of pages, and in their place, when all are consumed, its state.
 template <int P, int WAVES>
@@ -228,16 +195,6 @@ struct Fp4Lds {
     static constexpr size_t bytes(int new_rows) { return (size_t)pairs(new_rows) + (size_t)WAVES * WAVE; }
     static_assert((SHARED ? 0 : NB * BLOCK) + MQ_APPEND_ROWS * NEW_ROW + 16 + WAVES * WAVE <= 160 * 1024, "it all fits a compute unit's LDS");
 };
-// 64 lanes' 16 (4) bytes, each from an address of its own, to lds + 16 (4) l (`lds` the same in every lane): see copy_to_lds
-__device__ __forceinline__ void gather_to_lds(const void *from, uint32_t lds) {
-    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
-}
-__device__ __forceinline__ void gather_words_to_lds(const void *from, uint32_t lds) {
-    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0");
-}
-
 // MQ: more than one query row, or more than 16 heads to a kv head: slots are (row, head) pairs, 16 to a workgroup (grid z). ROWS: the launch
 // stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one.
 template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false>

@@ -320,6 +320,12 @@ bool takes_f32_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
     const size_t walked = n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1;
     return tiles * walked >= line;
 }
+// The same for layers of 4 bits.
+bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) { return takes_tile_kernel(g, n_queries, n_pages); }
+TileShape fp4_chunk_shape(const Geom &g, size_t n_slots, size_t n_pages) {
+    const TileShape shape = prefill_shape(g, n_slots, n_pages);
+    return shape == TileShape::quarters ? TileShape::halves : shape;
+}
 bool f32_halves(const Geom &g, size_t n_slots, size_t n_pages) {
     if (tuning().prefill_tiles2_min_pages >= 0) return false;
     const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, walk = wgs * n_pages;
@@ -887,6 +893,12 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         DecodeArgs a{};
         fill_fp4_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, decode_target_wgs(), a);
         if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
+        const bool by_chunk = n_queries > 1 && !k_new && takes_fp4_chunk_kernel(g, n_queries, (size_t)a.n_pages);
+        TileShape shape = TileShape::one_tile;
+        if (by_chunk) {
+            shape = fp4_chunk_shape(g, n_queries * (size_t)g.gqa, (size_t)a.n_pages);
+            a.splits = a.splits_total = chunk_splits(g, n_queries, (size_t)fp4_chunk_slots(g.P, shape), (size_t)a.n_pages);
+        }
         if (n_queries > 1 && a.splits > 1) {
             rc = multi_query_partials(L, s, (size_t)a.splits, n_queries, a, lease);
             if (rc) return rc;
@@ -897,7 +909,12 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         }
         rc = place(a.splits, a.out);
         if (rc) return rc;
-        SKV_HIP(launch_fp4_attention(a, nullptr, s));
+        if (by_chunk) {
+            const size_t lo = std::max(window_start, skv_window_start(L->len - n_queries, L->window));
+            SKV_HIP(launch_fp4_chunk(a, layer_pages(a.g, lo, L->len), shape, s));
+        } else {
+            SKV_HIP(launch_fp4_attention(a, nullptr, s));
+        }
         if (a.splits > 1) SKV_HIP(a.splits <= 4 && n_queries > 1 ? launch_merge_rows(a, s) : launch_merge(a, s));
         return settle();
     }
@@ -1559,7 +1576,8 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
     // a context over the chunk's own rows is written once they are in the ring, one over its queries once all are read: by the merge, so
     // there has to be one
     const bool late = context_over_rows(L, c, out, k, v) || over_queries(g, out, q, c) || reads_again(g, out, q);
-    const size_t slots = g.f32 ? (size_t)f32_prefill_slots(g.P, halves) : g.fp4 ? 16 : (size_t)prefill_tile_slots(g.P, shape); // of a workgroup
+    const TileShape shape4 = g.fp4 ? fp4_chunk_shape(g, c * (size_t)g.gqa, walked) : shape;
+    const size_t slots = (size_t)(g.f32 ? f32_prefill_slots(g.P, halves) : g.fp4 ? fp4_chunk_slots(g.P, shape4) : prefill_tile_slots(g.P, shape)); // of a workgroup
     StreamScratch::Lease lease;
     void *scratch = nullptr;
     int32_t rc = SKV_OK;
@@ -1599,14 +1617,8 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
         SKV_HIP(launch_append(w, s));
         pages.k_new = w.k_pool;
         pages.v_new = w.v_pool;
-        if (g.fp4) {
-            a.page_first = pages.first_pos / 16;
-            a.ring_base = pages.start;
-            a.ring_t = pages.ring_pages;
-            SKV_HIP(launch_fp4_attention(a, &pages, s));
-        } else {
-            SKV_HIP(g.f32 ? launch_f32_prefill(a, pages, nullptr, halves, s) : launch_prefill_tiles(a, pages, shape, s));
-        }
+        if (g.fp4) SKV_HIP(launch_fp4_chunk(a, pages, shape4, s));
+        else SKV_HIP(g.f32 ? launch_f32_prefill(a, pages, nullptr, halves, s) : launch_prefill_tiles(a, pages, shape, s));
     }
     if (a.splits_total == 1) return encode_append(L, s, k, v, c);
     if (late) {

@@ -38,6 +38,15 @@ __device__ __forceinline__ void copy_to_lds_once(const void *base, uint32_t lane
     default: asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072 nt" ::"s"(to), "v"(lane_offset), "s"(from) : "m0"); break;
     }
 }
+// 64 lanes' 16 (4) bytes, each from an address of its own, to lds + 16 (4) l (`lds` the same in every lane)
+__device__ __forceinline__ void gather_to_lds(const void *from, uint32_t lds) {
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
+}
+__device__ __forceinline__ void gather_words_to_lds(const void *from, uint32_t lds) {
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0");
+}
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // all but the wavefront's last N copies have landed
 template <int N>

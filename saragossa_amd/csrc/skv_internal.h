@@ -448,6 +448,8 @@ hipError_t launch_f32_split(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_store_fp4(const AppendArgs &a, hipStream_t s);
 hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s);
 hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s); // no merge; c null = the layer's own pages
+hipError_t launch_fp4_chunk(const DecodeArgs &a, const ChunkPages &c, TileShape shape, hipStream_t s); // chunked prefill, no merge
+int fp4_chunk_slots(int P, TileShape shape); // query slots of a workgroup
 hipError_t launch_fp4_batch(const DecodeBatchArgs &b, int n_seq, int max_splits, hipStream_t s); // no merge
 bool f32_decode_kernel_serves(const DecodeArgs &a); // the launch takes the kernel that can also append the row
 hipError_t launch_decode(const DecodeArgs &a, hipStream_t s);

@@ -1,6 +1,8 @@
 """The 4-bit element of the cache: rows as codes of 4 bits with a power of two per 32 dims, against the definition in 64
 bits (fp4_reference.py). Rows read back are equal, value for value; contexts are within the bound that `fp4_reference.attention`
 derives from the kernels' roundings."""
+import os
+
 import numpy as np
 import pytest
 
@@ -254,3 +256,70 @@ def test_steps_that_may_not_allocate(state):
         for _ in range(3):
             p.step(p.kv.encode_decode_step_static)
         p.check_rows(rows - 8)
+
+
+# the shapes of the chunk kernel: by the chunk's size, or one for all chunks of 64 query slots and more
+SHAPES = {"by-size": {}, "always": {"SKV_PREFILL_TILES": "2"},
+          "one-tile": {"SKV_PREFILL_TILES": "2", "SKV_PREFILL_TILES2_MIN_PAGES": "1000000"},
+          "two-tiles": {"SKV_PREFILL_TILES": "2", "SKV_PREFILL_TILES2_MIN_PAGES": "0"}, "never": {"SKV_PREFILL_TILES": "0"}}
+
+
+@pytest.fixture(params=SHAPES, ids=str)
+def chunk_shape(request):
+    env = SHAPES[request.param]
+    saved = {k: os.environ.get(k) for k in env}
+    os.environ.update(env)
+    skv.flags.reload()
+    yield request.param
+    for k, v in saved.items():
+        os.environ.pop(k) if v is None else os.environ.__setitem__(k, v)
+    skv.flags.reload()
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512), (12, 4, 96), (5, 1, 33), (4, 2, 32), (40, 2, 128)], ids=str)
+@pytest.mark.parametrize("base,n", [(0, 65), (777, 100), (3000, 37), (129, 300)])
+def test_chunks_in_every_shape(state, chunk_shape, dims, base, n):
+    p = Pair(state, dims, base + n, seed=base + n)
+    p.append(base)
+    p.chunk(n)
+
+
+@pytest.mark.parametrize("dims", [(16, 8, 256), (8, 2, 64), (8, 2, 512), (5, 1, 33), (16, 2, 128)], ids=str)
+def test_chunks_over_rings_in_every_shape(state, chunk_shape, dims):
+    p = Pair(state, dims, 1200, seed=3, window=150, rollback=20)
+    p.append(60)
+    for n in (64, 33, 200, 90, 128):
+        p.chunk(n)
+    p.step()
+    p.check_rows(p.kv.len() - 150)
+
+
+@pytest.mark.parametrize("dims", [(16, 2, 256), (32, 8, 128), (8, 2, 64), (8, 2, 512)], ids=str)
+@pytest.mark.parametrize("n", [7, 40, 150])
+def test_rows_that_are_nan_reach_the_queries_that_attend_them_and_no_other(state, chunk_shape, dims, n):
+    """A padded chunk: rows behind a query's own are NaN or infinite, in K, in V or in some groups of dims."""
+    p = Pair(state, dims, 400, seed=n)
+    p.append(100)
+    k, v, q = p.new(n)
+    bad = n - 3
+    v[bad, :32] = np.nan           # the first group of dims of the first head
+    v[bad + 1, -5] = np.inf        # of the last group of the last head
+    k[bad + 2] = np.nan
+    kd, vd, qd = _dev(k), _dev(v), _dev(q)
+    out = torch.zeros((n, p.q_dim), device="cuda")
+    p.kv.encode_prefill_rows(_stream(), qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), n, out.data_ptr())
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(n, dims[0], dims[2])
+    clean_k, clean_v = k.copy(), v.copy()
+    clean_k[bad + 2], clean_v[bad, :32], clean_v[bad + 1, -32:] = 0, 0, 0
+    keys = np.concatenate([p.k, stored(clean_k, dims[2])])
+    vals = np.concatenate([p.v, stored(clean_v, dims[2])])
+    want, tol = attention(q[:bad + 2], keys[:-1], vals[:-1], dims)
+    want, tol = want.reshape(bad + 2, *got.shape[1:]), tol.reshape(bad + 2, *got.shape[1:])
+    group = dims[0] // dims[1]
+    want[bad:, :group, :32] = np.nan
+    want[bad + 1:, -group:, -min(32, dims[2]):] = np.nan
+    assert np.array_equal(np.isnan(got[:bad + 2]), np.isnan(want))
+    ok = ~np.isnan(want)
+    assert (np.abs(got[:bad + 2] - want)[ok] <= tol[ok]).all()
+    assert np.isnan(got[bad + 2]).all()
