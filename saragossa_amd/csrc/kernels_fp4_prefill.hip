@@ -118,24 +118,32 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         return reinterpret_cast<const uint8_t *>(v ? (is_new ? c.v_new : a.v_pool) : (is_new ? c.k_new : a.k_pool));
     };
     // K of the pages it0 + d0 .. (as many as `pages`), whose physical pages lie in lanes d0 .. of ids, to buffer `buf`
-    auto copy_k = [&](int it0, int d0, int pages, int buf) __attribute__((always_inline)) {
+    auto copy_k = [&](int it0, int d0, auto how_many, int buf) __attribute__((always_inline)) {
+        constexpr int pages = decltype(how_many)::value;
         const uint32_t to = lds0 + (uint32_t)(buf * L::K_BUF);
         if constexpr (P >= 128) {
-            for (int i = wave; i < pages * NB; i += WAVES) { // a KiB each
-                const int d = i / NB, b = i % NB;
+#pragma unroll
+            for (int r = 0; r < (pages * NB + WAVES - 1) / WAVES; ++r) { // a KiB each
+                const int i = wave + r * WAVES, d = i / NB, b = i % NB;
+                if (pages * NB % WAVES != 0 && i >= pages * NB) continue;
                 const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, d0 + d);
                 copy_to_lds(pool_of(it0 + d0 + d, false) + codes_at + (uint64_t)page * page_bytes + b * 1024, (uint32_t)lane * 16, to + d * L::K_PAGE + b * 1024);
             }
         } else {
             constexpr int UNITS = P / 2;
-            for (int i = wave * 64; i < pages * UNITS; i += WAVES * 64) {
+#pragma unroll
+            for (int r = 0; r < (pages * UNITS + WAVES * 64 - 1) / (WAVES * 64); ++r) {
+                const int i = (wave + r * WAVES) * 64;
+                if (i >= pages * UNITS) continue;
                 const int u = i + lane, d = min(u / UNITS, pages - 1);
                 const uint32_t page = (uint32_t)__shfl(ids, d0 + d);
                 if (u < pages * UNITS) gather_to_lds(pool_of(it0 + d0 + d, false) + codes_at + (uint64_t)page * page_bytes + (u - d * UNITS) * 16, to + i * 16);
             }
         }
         constexpr int WORDS = P / 8;
-        for (int i = (WAVES - 1 - wave) * 64; i < pages * WORDS; i += WAVES * 64) {
+        static_assert(pages * WORDS <= WAVES * 64, "powers: a copy a wavefront, from the last one on");
+        const int i = (WAVES - 1 - wave) * 64;
+        if (i < pages * WORDS) {
             const int u = i + lane, d = min(u / WORDS, pages - 1);
             const uint32_t page = (uint32_t)__shfl(ids, d0 + d);
             if (u < pages * WORDS) gather_words_to_lds(pool_of(it0 + d0 + d, false) + powers_at + (uint64_t)page * page_bytes + (u - d * WORDS) * 4, to + PAGES * L::K_PAGE + i * 4);
@@ -272,8 +280,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         }
     }
     ids_here();
-    copy_k(0, 0, GP, 1); // the first group's, into the second buffer
-    copy_k(0, GP, PAGES, 0);
+    copy_k(0, 0, std::integral_constant<int, GP>{}, 1); // the first group's, into the second buffer
+    copy_k(0, GP, std::integral_constant<int, PAGES>{}, 0);
     load_v(0);
     __syncthreads(); // (all have read their queries from V's buffers)
     convert_v(0);
@@ -387,8 +395,14 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
             else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
         }
     };
-    auto scores = [&](auto with_probs) __attribute__((always_inline)) {
+    // V operands are asked for AHEAD of their products
+    constexpr int AHEAD = NT < 4 ? NT : 4;
+    u4 vr[AHEAD];
+    auto ask_v = [&](const uint8_t *vt, int u) __attribute__((always_inline)) { vr[u % AHEAD] = *reinterpret_cast<const u4 *>(vt + u * 1024 + lane * 16); };
+    // scores of the pair whose K is in the registers; the settled pair's probabilities between the products, and its first V operands at the end
+    auto scores = [&](auto with_probs, const uint8_t *vt) __attribute__((always_inline)) {
         constexpr bool PROBS = decltype(with_probs)::value;
+        __builtin_amdgcn_s_setprio(1); // (the SIMD's other wavefront is mostly in its second window, products almost alone)
         float4_t ns[2][TILES];
         int q = 0;
 #pragma unroll
@@ -409,6 +423,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                     }
                 }
                 if (PROBS) {
+                    if (b == NB - 1) ask_v(vt, (3 - k) % AHEAD);
                     const int until = ((b * 4 + 4 - k) * 9) / (4 * NB); // steps done by the end of this beat
 #pragma unroll
                     for (int s = 0; s < 9; ++s)
@@ -418,13 +433,14 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             sa[t] = ns[0][t];
             sb[t] = ns[1][t];
         }
     };
-    auto accumulate = [&](const uint8_t *vt) __attribute__((always_inline)) {
+    auto accumulate = [&](const uint8_t *vt, auto next_k) __attribute__((always_inline)) {
         bf16x8_t ph[TILES], pl[TILES];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -433,11 +449,14 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         }
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u4 *>(vt + u * 1024 + lane * 16));
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, vr[u % AHEAD]);
 #pragma unroll
             for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[t], o[t][u], 0, 0, 0);
 #pragma unroll
             for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[t], o[t][u], 0, 0, 0);
+            if (u + AHEAD < NT) ask_v(vt, u + AHEAD);
+            else if (u + AHEAD == NT) next_k();
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // the slots that attend rows that are NaN in the step's V: NaN in those groups of dims
@@ -467,7 +486,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     copies_landed();
     __syncthreads();
     ask_k(1, 0);
-    scores(std::false_type{});
+    scores(std::false_type{}, nullptr);
     mask(half);
     settle();
     ask_ids(PAGES);
@@ -477,17 +496,20 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         const int buf = step & 1;
         if (step + 1 < n_steps) { // uniform
             ids_here();
-            copy_k((step + 1) * PAGES, GP, PAGES, buf ^ 1);
+            copy_k((step + 1) * PAGES, GP, std::integral_constant<int, PAGES>{}, buf ^ 1);
             load_v((step + 1) * PAGES);
             ask_ids((step + 2) * PAGES);
         }
+        ask_k(buf, 0);
 #pragma unroll
         for (int pp = 0; pp < SP; ++pp) {
             const int group = step * SP + pp;
             if (group >= n_groups) continue; // uniform
-            ask_k(buf, pp);
-            scores(std::true_type{});
-            accumulate(lds + L::V_AT + buf * L::V_BUF + (pp * HALVES + half) * 2 * L::V_PAGE);
+            const uint8_t *vt = lds + L::V_AT + buf * L::V_BUF + (pp * HALVES + half) * 2 * L::V_PAGE;
+            scores(std::true_type{}, vt);
+            accumulate(vt, [&]() __attribute__((always_inline)) {
+                if (pp + 1 < SP) ask_k(buf, pp + 1);
+            });
             mask((group + 1) * HALVES + half);
             settle();
         }

@@ -553,8 +553,10 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     const int pairs = (a.n_pages + 1) / 2;
     a.splits = pairs <= a.waves && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
+        // (one workgroup to a compute unit)
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
-        a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(512 / tiles, 1));
+        a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(256 / tiles, 1));
+        if (tiles > (size_t)g.kv_heads) a.splits = xcd_splits(a.splits, g.kv_heads, pairs, a.waves, 10);
     }
     a.splits_total = a.splits;
 }
