@@ -30,72 +30,102 @@ __device__ __forceinline__ uint32_t fp6_codes_of(uint32_t u) {
 } // namespace
 
 // ------------------------------------------------------------------------------------
-// Rows stored: f32 rows -> codes and powers. Eight neighbouring lanes take a group of a row, four dims each (128 bytes side by side), find
-// its largest magnitude among themselves and convert. K: the eight's 16 bits are the lane's 16 bytes of the matrix operand as they stand. V: a
-// byte holds the dims c and c + 16, which lanes four apart exchange, and a word the byte of four rows, which lanes eight apart
-// exchange; a quad of rows that the batch covers is stored as words, one that it shares with older rows as bytes.
-// A workgroup takes 256 such eighths of one (page, kv head) of K or V.
+// Rows stored: f32 rows -> codes and powers. Eight neighbouring lanes take a group of a row, four dims each, find its largest magnitude among
+// themselves and convert; the group beside it is the wavefront's other half, so that rows are read 256 bytes at a time. K: the eight's
+// 16 bits are the lane's 16 bytes of the matrix operand as they stand. V: a byte holds the dims c and c + 16, which lanes four apart exchange, and a
+// word the byte of four rows, which lanes eight apart exchange; a quad of rows that the batch covers is stored as words, one that it
+// shares with older rows as bytes.
+// A workgroup takes PER times 256 such eighths of one (page, kv head), of K and of V, all loads in front of the first conversion.
 // ------------------------------------------------------------------------------------
+struct Fp4Unit { // of a thread: which eighth of which group of which row
+    int o, i, quad, grp;
+    bool real; // (an odd number of groups leaves some of the last part's idle)
+    __device__ __forceinline__ Fp4Unit(int groups, int part) {
+        const int rest = (int)(threadIdx.x >> 5);
+        o = threadIdx.x & 7;
+        i = (threadIdx.x >> 3) & 3;
+        quad = rest >> 1;
+        grp = part * 2 + (rest & 1);
+        real = grp < groups;
+    }
+    __device__ __forceinline__ int row() const { return quad * 4 + i; }
+    __device__ __forceinline__ int dim() const { return grp * 32 + o * 4; }
+};
+constexpr long FP4_WGS = 4096; // workgroups from which each takes twice as much
+static int fp4_parts(int P) { return (P / 32 + 1) / 2; }
+
+template <int PER>
 __global__ __launch_bounds__(256) void store_fp4_kernel(AppendArgs a) {
     const Geom g = a.g;
-    const int groups = g.P >> 5, parts = (groups + 1) >> 1;
-    const bool is_v = (int)blockIdx.z >= parts;
-    const int part = (int)blockIdx.z - (is_v ? parts : 0), kvh = blockIdx.y;
+    const int groups = g.P >> 5, kvh = blockIdx.y;
+    // (the page's place by a vector load, in front of the rows: see append_tile)
     int logical = a.first_page + (int)blockIdx.x;
     if (a.ring_pages > 0 && logical >= a.ring_pages) logical -= a.ring_pages;
-    const int page = a.table ? a.table[logical] : logical;
+    int at = a.table ? logical : 0;
+    asm("" : "+v"(at));
+    const int asked = (a.table ? a.table : reinterpret_cast<const int32_t *>(a.k_src))[at]; // (no table: some valid address)
     const int row0 = (int)blockIdx.x * 16 - a.first_row; // batch row of the page's first row
     const int r_lo = max(-row0, 0), r_hi = min(16, a.n_rows - row0); // rows of the page in the batch
-
-    const int lane = threadIdx.x & 63, o = threadIdx.x & 7, i = (threadIdx.x >> 3) & 3;
-    const int rest = (int)(threadIdx.x >> 5) + part * 8, quad = rest & 3, grp = rest >> 2;
-    const int r = quad * 4 + i, d = grp * 32 + o * 4;
-    const int row = min(max(r, r_lo), r_hi - 1); // clamped: every lane takes part in the exchanges
-    const int kv_dim = g.kv_heads * g.head_dim;
-    const float *src = (is_v ? a.v_src : a.k_src) + (long)(row0 + row) * kv_dim + kvh * g.head_dim;
-    float x[4];
-    if (a.vec) { // uniform
-        const float4_t v = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
+    const int kv_dim = g.kv_heads * g.head_dim, lane = threadIdx.x & 63;
+    float x[2][PER][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = d < g.head_dim ? v[e] : 0.0f;
-    } else {
+    for (int p = 0; p < PER; ++p) {
+        const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
+        const int row = min(max(u.row(), r_lo), r_hi - 1), d = u.dim(); // clamped: every lane takes part in the exchanges
+        const long from = (long)(row0 + row) * kv_dim + kvh * g.head_dim;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float v = src[min(d + e, g.head_dim - 1)];
-            x[e] = d + e < g.head_dim ? v : 0.0f;
+        for (int v = 0; v < 2; ++v) {
+            const float *src = (v ? a.v_src : a.k_src) + from;
+            if (a.vec) { // uniform
+                const float4_t y = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[v][p][e] = y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[v][p][e] = src[min(d + e, g.head_dim - 1)];
+            }
         }
     }
-    uint32_t power;
-    const uint32_t codes = fp4_codes_of(x, power);
-    const bool real = grp < groups; // (an odd number of groups fills half of its last workgroup)
-    const bool in = real && r >= r_lo && r < r_hi;
-    uint16_t *pool = is_v ? a.v_pool : a.k_pool;
-    uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
-    if (!is_v) { // uniform
+    const int page = __builtin_amdgcn_readfirstlane(a.table ? asked : logical);
+    uint8_t *const kp = const_cast<uint8_t *>(fp4_powers(a.k_pool, g, page, kvh)), *const vp = const_cast<uint8_t *>(fp4_powers(a.v_pool, g, page, kvh));
+    uint8_t *const kc = const_cast<uint8_t *>(fp4_codes(a.k_pool, g, page, kvh)), *const vc = const_cast<uint8_t *>(fp4_codes(a.v_pool, g, page, kvh));
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
+        const int r = u.row(), d = u.dim();
+        const bool in = u.real && r >= r_lo && r < r_hi;
+        uint32_t codes[2], power[2];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[v][p][e] = d + e < g.head_dim ? x[v][p][e] : 0.0f;
+            codes[v] = fp4_codes_of(x[v][p], power[v]);
+        }
         if (in) {
-            *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
-            if (o == 0) pp[k4_power(g.P, r, grp)] = (uint8_t)power;
+            *reinterpret_cast<uint16_t *>(kc + k4_code(r, d)) = (uint16_t)codes[0];
+            if (u.o == 0) {
+                kp[k4_power(g.P, r, u.grp)] = (uint8_t)power[0];
+                vp[v4_power(g.P, r, u.grp)] = (uint8_t)power[1];
+            }
         }
-        return;
-    }
-    const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
-    const uint32_t low = o < 4 ? codes : other, high = o < 4 ? other : codes;
-    const uint32_t mine = nibbles_apart(low) | nibbles_apart(high) << 4; // dims 4 (o % 4) .. of the row, each with the one 16 further
-    uint32_t word = 0; // column 4 (o % 4) + i: byte q is row q of the quad
+        const uint32_t other = (uint32_t)__shfl_xor((int)codes[1], 4);
+        const uint32_t low = u.o < 4 ? codes[1] : other, high = u.o < 4 ? other : codes[1];
+        const uint32_t mine = nibbles_apart(low) | nibbles_apart(high) << 4; // dims 4 (o % 4) .. of the row, each with the one 16 further
+        uint32_t word = 0; // column 4 (o % 4) + i: byte q is row q of the quad
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const uint32_t of_row = (uint32_t)__shfl((int)mine, (lane & ~24) | q << 3);
-        word |= (of_row >> (8 * i) & 255u) << (8 * q);
-    }
-    if (in && o == 0) pp[v4_power(g.P, r, grp)] = (uint8_t)power;
-    if (o >= 4 || !real) return;
-    uint8_t *dst = cp + v4_code(g.P, quad * 4, grp * 32 + o * 4 + i);
-    if (quad * 4 >= r_lo && quad * 4 + 4 <= r_hi) {
-        *reinterpret_cast<uint32_t *>(dst) = word;
-    } else {
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t of_row = (uint32_t)__shfl((int)mine, (lane & ~24) | q << 3);
+            word |= (of_row >> (8 * u.i) & 255u) << (8 * q);
+        }
+        if (u.o >= 4 || !u.real) continue;
+        uint8_t *dst = vc + v4_code(g.P, u.quad * 4, d + u.i);
+        if (u.quad * 4 >= r_lo && u.quad * 4 + 4 <= r_hi) {
+            *reinterpret_cast<uint32_t *>(dst) = word;
+        } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (quad * 4 + q >= r_lo && quad * 4 + q < r_hi) dst[q] = (uint8_t)(word >> (8 * q));
+            for (int q = 0; q < 4; ++q)
+                if (u.quad * 4 + q >= r_lo && u.quad * 4 + q < r_hi) dst[q] = (uint8_t)(word >> (8 * q));
+        }
     }
 }
 
@@ -104,50 +134,63 @@ hipError_t launch_store_fp4(const AppendArgs &a, hipStream_t s) {
     AppendArgs b = append_placed(a);
     b.vec = b.vec && ((uintptr_t)a.v_src & 15) == 0;
     const long pages = (a.first_pos + a.n_rows + 15) / 16 - a.first_pos / 16;
-    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(2 * ((a.g.P / 32 + 1) / 2)));
-    hipLaunchKernelGGL(store_fp4_kernel, grid, dim3(256), 0, s, b);
+    const int parts = fp4_parts(a.g.P);
+    const bool two = parts % 2 == 0 && pages * a.g.kv_heads * parts > FP4_WGS;
+    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(two ? parts / 2 : parts));
+    if (two) hipLaunchKernelGGL(store_fp4_kernel<2>, grid, dim3(256), 0, s, b);
+    else hipLaunchKernelGGL(store_fp4_kernel<1>, grid, dim3(256), 0, s, b);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------
 // Rows read back as bf16, which holds every value exactly: the store's steps the other way round, with the same division of the work.
 // ------------------------------------------------------------------------------------
+template <int PER>
 __global__ __launch_bounds__(256) void load_fp4_kernel(GatherArgs a, int vec) {
     const Geom g = a.g;
-    const int groups = g.P >> 5, parts = (groups + 1) >> 1;
-    const bool is_v = (int)blockIdx.z >= parts;
-    const int part = (int)blockIdx.z - (is_v ? parts : 0), kvh = blockIdx.y;
-    uint16_t *out = is_v ? a.v_dst : a.k_dst;
-    if (!out) return;
+    const int groups = g.P >> 5, kvh = blockIdx.y, lane = threadIdx.x & 63;
     const long pos0 = (a.first_pos / 16 + blockIdx.x) * 16;
     const int page = a.table[slot_of(pos0, g.ring_rows) >> 4];
-    const int lane = threadIdx.x & 63, o = threadIdx.x & 7, i = (threadIdx.x >> 3) & 3;
-    const int rest = (int)(threadIdx.x >> 5) + part * 8, quad = rest & 3, grp = min(rest >> 2, groups - 1);
-    const int r = quad * 4 + i, d = grp * 32 + o * 4;
-    const uint8_t *cp = fp4_codes(is_v ? a.v_pool : a.k_pool, g, page, kvh), *pp = fp4_powers(is_v ? a.v_pool : a.k_pool, g, page, kvh);
-    const uint32_t power = (uint32_t)pp[is_v ? v4_power(g.P, r, grp) : k4_power(g.P, r, grp)] << 23;
-    uint32_t codes = 0;
-    if (is_v) { // uniform
-        const uint32_t word = *reinterpret_cast<const uint32_t *>(cp + v4_code(g.P, quad * 4, grp * 32 + (o & 3) * 4 + i));
-        const int half = o < 4 ? 0 : 4;
+    const uint8_t *const kc = fp4_codes(a.k_pool, g, page, kvh), *const vc = fp4_codes(a.v_pool, g, page, kvh);
+    const uint8_t *const kp = fp4_powers(a.k_pool, g, page, kvh), *const vp = fp4_powers(a.v_pool, g, page, kvh);
+    uint32_t codes[2][PER], power[2][PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
+        const int grp = min(u.grp, groups - 1), d = grp * 32 + u.o * 4;
+        codes[0][p] = *reinterpret_cast<const uint16_t *>(kc + k4_code(u.row(), d));
+        codes[1][p] = *reinterpret_cast<const uint32_t *>(vc + v4_code(g.P, u.quad * 4, grp * 32 + (u.o & 3) * 4 + u.i)); // column 4 (o % 4) + i: byte q is row q
+        power[0][p] = kp[k4_power(g.P, u.row(), grp)];
+        power[1][p] = vp[v4_power(g.P, u.row(), grp)];
+    }
+    const int kv_dim = g.kv_heads * g.head_dim;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
+        const int d = u.dim();
+        uint32_t mine = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t col = (uint32_t)__shfl((int)word, (lane & ~24) | k << 3);
-            codes |= (col >> (8 * i + half) & 15u) << (4 * k);
+            const uint32_t col = (uint32_t)__shfl((int)codes[1][p], (lane & ~24) | k << 3);
+            mine |= (col >> (8 * u.i + (u.o < 4 ? 0 : 4)) & 15u) << (4 * k);
         }
-    } else {
-        codes = *reinterpret_cast<const uint16_t *>(cp + k4_code(r, d));
-    }
-    const long row = pos0 + r - a.first_pos;
-    if (rest >> 2 >= groups || row < 0 || row >= a.n_rows || d >= g.head_dim) return;
-    const uint32_t v[2] = {code_pair<0>(codes, power), code_pair<1>(codes, power)};
-    uint16_t *dst = out + row * g.kv_heads * g.head_dim + kvh * g.head_dim + d;
-    if (vec) { // uniform
-        *reinterpret_cast<u2 *>(dst) = u2{v[0], v[1]};
-    } else {
+        codes[1][p] = mine;
+        const long row = pos0 + u.row() - a.first_pos;
+        if (!u.real || row < 0 || row >= a.n_rows || d >= g.head_dim) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < g.head_dim) dst[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+        for (int v = 0; v < 2; ++v) {
+            uint16_t *out = v ? a.v_dst : a.k_dst;
+            if (!out) continue; // uniform
+            const uint32_t e4 = power[v][p] << 23, w[2] = {code_pair<0>(codes[v][p], e4), code_pair<1>(codes[v][p], e4)};
+            uint16_t *dst = out + row * kv_dim + kvh * g.head_dim + d;
+            if (vec) { // uniform
+                __builtin_nontemporal_store(u2{w[0], w[1]}, reinterpret_cast<u2 *>(dst));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < g.head_dim) dst[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            }
+        }
     }
 }
 
@@ -155,8 +198,11 @@ hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
     if (a.n_rows <= 0) return hipSuccess;
     const int vec = a.g.head_dim % 4 == 0 && (((uintptr_t)a.k_dst | (uintptr_t)a.v_dst) & 7) == 0;
     const long pages = (a.first_pos + a.n_rows + 15) / 16 - a.first_pos / 16;
-    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(2 * ((a.g.P / 32 + 1) / 2)));
-    hipLaunchKernelGGL(load_fp4_kernel, grid, dim3(256), 0, s, a, vec);
+    const int parts = fp4_parts(a.g.P);
+    const bool two = parts % 2 == 0 && pages * a.g.kv_heads * parts > FP4_WGS;
+    const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(two ? parts / 2 : parts));
+    if (two) hipLaunchKernelGGL(load_fp4_kernel<2>, grid, dim3(256), 0, s, a, vec);
+    else hipLaunchKernelGGL(load_fp4_kernel<1>, grid, dim3(256), 0, s, a, vec);
     return hipGetLastError();
 }
 

@@ -26,13 +26,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return __built
 // 32 values as e2m3 codes of x / scale, and the codes' values. These conversions take several passes and write their results as they go: a
 // result register that is also an operand is read back changed (seen: the scale in the first result register, the values after the first
 // few wrong), and the compiler does not know. Operands are kept alive behind the instruction, so that they have registers of their own.
-__device__ __forceinline__ u6 to_fp6(const float (&x)[32], float scale) {
-    float16_t even, odd; // they take turns in the result
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        even[e] = x[2 * e];
-        odd[e] = x[2 * e + 1];
-    }
+__device__ __forceinline__ u6 to_fp6(float16_t even, float16_t odd, float scale) { // (they take turns in the result)
     u6 codes = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
     asm volatile("" : "+v"(codes) : "v"(even), "v"(odd), "v"(scale));
     return codes;
@@ -216,8 +210,11 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     int8v_t q_term[TILES][NB][4];
     uint32_t q_power[TILES][NB];
     float4_t *const raw = reinterpret_cast<float4_t *>(lds + L::V_AT) + wave * 16 * L::ROW;
+    constexpr int ROW = L::ROW, LANES = ROW == 24 ? 32 : ROW, AT_ONCE = 64 / LANES, QL = 16 / AT_ONCE; // lanes of a row, rows of an instruction
+    const int unit = lane % LANES;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
+        float4_t qv[NB][QL]; // every load of the tile in front of the first conversion
         const int s0 = wg_slot0 + (tw * TILES + t) * 16;
         t_on[t] = s0 < n_slots;
         const int my_slot = min(s0 + n, n_slots - 1);
@@ -226,39 +223,42 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         t_lim_lo[t] = limit_of(min(s0, n_slots - 1));
         t_ws_hi[t] = ws_of(min(s0 + 15, n_slots - 1));
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            constexpr int ROW = L::ROW, LANES = ROW == 24 ? 32 : ROW, AT_ONCE = 64 / LANES; // lanes of a row, rows of an instruction
-            float4_t v[16 / AT_ONCE];
-            const int unit = lane % LANES, d = b * 128 + unit * 4;
+        for (int i = 0; i < QL; ++i) {
+            const float *qrow = a.q + context_row(g, kvh, min(s0 + i * AT_ONCE + lane / LANES, n_slots - 1)) * g.head_dim;
 #pragma unroll
-            for (int i = 0; i < 16 / AT_ONCE; ++i) {
-                const float *qrow = a.q + context_row(g, kvh, min(s0 + i * AT_ONCE + lane / LANES, n_slots - 1)) * g.head_dim;
+            for (int b = 0; b < NB; ++b) {
+                const int d = b * 128 + unit * 4;
                 if (a.q_vec) {
-                    v[i] = *reinterpret_cast<const float4_t *>(qrow + min(d, g.head_dim - 4));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i][e] = d < g.head_dim ? v[i][e] : 0.0f;
+                    qv[b][i] = *reinterpret_cast<const float4_t *>(qrow + min(d, g.head_dim - 4));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i][e] = qrow[min(d + e, g.head_dim - 1)];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i][e] = d + e < g.head_dim ? v[i][e] : 0.0f;
+                    for (int e = 0; e < 4; ++e) qv[b][i][e] = qrow[min(d + e, g.head_dim - 1)];
                 }
             }
+        }
 #pragma unroll
-            for (int i = 0; i < 16 / AT_ONCE; ++i) {
+        for (int b = 0; b < NB; ++b) {
+            const int d = b * 128 + unit * 4;
+#pragma unroll
+            for (int i = 0; i < QL; ++i) {
                 const int row = i * AT_ONCE + lane / LANES;
-                if (LANES == ROW || unit < ROW) raw[row * ROW + (unit ^ (row & 7))] = v[i];
+                float4_t v = qv[b][i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = d + e < g.head_dim ? v[e] * a.qscale : 0.0f;
+                if (LANES == ROW || unit < ROW) raw[row * ROW + (unit ^ (row & 7))] = v;
             }
-            float x[32];
+            float16_t even, odd;
+            uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float4_t y = raw[n * ROW + ((min(j * 8, ROW - 8) + i) ^ (n & 7))];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * i + e] = G >= 4 || j < G ? y[e] * a.qscale : 0.0f;
+                for (int e = 0; e < 2; ++e) {
+                    even[2 * i + e] = G >= 4 || j < G ? y[2 * e] : 0.0f;
+                    odd[2 * i + e] = G >= 4 || j < G ? y[2 * e + 1] : 0.0f;
+                    top = max(top, max(magnitude(even[2 * i + e]), magnitude(odd[2 * i + e])));
+                }
             }
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) top = max(top, magnitude(x[e]));
             // the first term's power is the smallest with the largest value <= 7.5 of it; a term leaves at most 2^-2, then 2^-7, 2^-12, 2^-17 of it, 2^-18.9
             // of the largest value
             const int power = max((int)((top + 0x0fffffu) >> 23) - 2, 18);
@@ -267,14 +267,17 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float scale = __uint_as_float((uint32_t)(power - down[k]) << 23);
-                const u6 codes = to_fp6(x, scale);
+                const u6 codes = to_fp6(even, odd, scale);
 #pragma unroll
                 for (int w = 0; w < 6; ++w) q_term[t][b][k][w] = (int)codes[w];
                 q_term[t][b][k][6] = q_term[t][b][k][7] = 0;
                 if (k < 3) {
                     const float32_t back = from_fp6(codes, scale);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] -= back[e];
+                    for (int e = 0; e < 16; ++e) {
+                        even[e] -= back[2 * e];
+                        odd[e] -= back[2 * e + 1];
+                    }
                 }
             }
         }
