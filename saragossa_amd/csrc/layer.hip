@@ -320,11 +320,43 @@ bool takes_f32_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
     const size_t walked = n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1;
     return tiles * walked >= line;
 }
-// The same for layers of 4 bits.
-bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) { return takes_tile_kernel(g, n_queries, n_pages); }
-TileShape fp4_chunk_shape(const Geom &g, size_t n_slots, size_t n_pages) {
-    const TileShape shape = prefill_shape(g, n_slots, n_pages);
-    return shape == TileShape::quarters ? TileShape::halves : shape;
+// The same for layers of 4 bits: the streaming kernel or the one that shares pages and V's conversion among 64 to 256 slots. The streaming
+// one has no prologue to speak of and converts V anew for every 16 slots; the other's start is the queries' conversion (3 us at
+// head_dim 128, 5 at 256). From 193 workgroups of 64 slots on that needs neither splits nor a merge and is the faster one everywhere. Over 3510
+// chunks of 4 to 1024 rows in nine geometries, on layers in no cache, kernel and shape chosen are 0.6 % slower than the best on the
+// average. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
+// 16.7/23.8, 256 (70) 25.7/31.5, 64 over 8000 (65) 28.5/28.2, 512 over 512 (49, 256 workgroups) 24.8/23.2; q16/kv2/hd256, 64 over 8192 (33)
+// 28.7/35.8, 128 (66) 43.6/47.6, q16/kv8/hd256, 256 over 8000 (131) 70.4/68.3; q8/kv2/hd512 loses in the mean from 16 on.
+bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
+    const size_t n_slots = n_queries * (size_t)g.gqa;
+    if (tuning().prefill_tiles != 1 || n_slots < 64) return tuning().prefill_tiles > 1 && n_slots >= 64;
+    const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, tiles = (n_slots + 15) / 16 * (size_t)g.kv_heads;
+    const size_t walked = n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1;
+    return wgs > 192 || tiles * walked >= (g.P > 256 ? 17000u : g.P > 128 ? 48000u : 70000u);
+}
+// Slots of a workgroup of that kernel: 64 (two wavefronts to a tile), 128, or 256 (heads to 128 dims). Wider ones convert a page of V for
+// more slots, narrower ones fill the device sooner, and where the causal triangle is most of the work (`own`) they also share it out more
+// evenly. Lines in the same pairs. 64 / 128 / 256 slots, in us: q32/kv8/hd128, 512 rows over 0 (16) 17.0/26.5/32.8, over 4700 (313)
+// 74.8/71.4/73.2, 600 over 3763 111.3/93.3/76.4 (128 slots: 150 workgroups for 256 compute units); q16/kv2/hd256, 512 over 0
+// 29.5/33.2, 4096 72/68.6, 1761 over 0 (98) 61/81, 2442 over 998 (339) 171/142.
+TileShape fp4_chunk_shape(const Geom &g, size_t n_queries, size_t n_pages) {
+    if (g.P > 256) return TileShape::one_tile;
+    const long knob = tuning().prefill_tiles2_min_pages;
+    if (knob >= 0) return g.P <= 128 && (long)n_pages >= knob ? TileShape::two_tiles : TileShape::one_tile;
+    const size_t n_slots = n_queries * (size_t)g.gqa;
+    const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, tiles = (n_slots + 15) / 16 * (size_t)g.kv_heads;
+    const size_t pairs = tiles * (n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1);
+    if (g.P > 128) {
+        const size_t one = wgs <= 128 ? 120000 : wgs <= 192 ? 50000 : wgs <= 256 ? 150000 : wgs <= 512 ? 340000 : 180000;
+        return pairs < one ? TileShape::halves : TileShape::one_tile;
+    }
+    if (wgs > 512) return pairs >= (wgs <= 1024 ? 900000u : 500000u) ? TileShape::two_tiles : TileShape::one_tile;
+    if (wgs > 256) {
+        const bool own = n_queries / 8 >= n_pages;
+        if (wgs <= 340 && pairs >= 150000 && !own) return TileShape::two_tiles;
+        return pairs < (own ? 300000u : 120000u) ? TileShape::halves : pairs < 450000 ? TileShape::one_tile : TileShape::two_tiles;
+    }
+    return pairs < (wgs <= 128 ? 120000u : wgs <= 192 ? 75000u : 180000u) ? TileShape::halves : TileShape::one_tile;
 }
 bool f32_halves(const Geom &g, size_t n_slots, size_t n_pages) {
     if (tuning().prefill_tiles2_min_pages >= 0) return false;
@@ -898,7 +930,7 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         const bool by_chunk = n_queries > 1 && !k_new && takes_fp4_chunk_kernel(g, n_queries, (size_t)a.n_pages);
         TileShape shape = TileShape::one_tile;
         if (by_chunk) {
-            shape = fp4_chunk_shape(g, n_queries * (size_t)g.gqa, (size_t)a.n_pages);
+            shape = fp4_chunk_shape(g, n_queries, (size_t)a.n_pages);
             a.splits = a.splits_total = chunk_splits(g, n_queries, (size_t)fp4_chunk_slots(g.P, shape), (size_t)a.n_pages);
         }
         if (n_queries > 1 && a.splits > 1) {
@@ -1578,7 +1610,8 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
     // a context over the chunk's own rows is written once they are in the ring, one over its queries once all are read: by the merge, so
     // there has to be one
     const bool late = context_over_rows(L, c, out, k, v) || over_queries(g, out, q, c) || reads_again(g, out, q);
-    const TileShape shape4 = g.fp4 ? fp4_chunk_shape(g, c * (size_t)g.gqa, walked) : shape;
+    const TileShape shape4 = g.fp4 ? fp4_chunk_shape(g, c, walked) : shape;
+    const bool streams = g.fp4 && !takes_fp4_chunk_kernel(g, c, walked);
     const size_t slots = (size_t)(g.f32 ? f32_prefill_slots(g.P, halves) : g.fp4 ? fp4_chunk_slots(g.P, shape4) : prefill_tile_slots(g.P, shape)); // of a workgroup
     StreamScratch::Lease lease;
     void *scratch = nullptr;
@@ -1598,6 +1631,12 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
     }
     if (!made) {
         a.splits = chunk_splits(g, c, slots, walked);
+        if (streams) {
+            RowsAhead ahead(L, c);
+            fill_fp4_args(L, q, out, L->floor_pos, nullptr, nullptr, c, tuning().prefill_wgs, a);
+            a.n_pages = pages.n_old + (int)n_new;
+            a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(walked / 8, 1));
+        }
         if (late) a.splits = std::max(a.splits, 2);
         a.splits_total = a.splits;
         rc = multi_query_partials(L, s, a.splits > 1 ? (size_t)a.splits : 0, c, a, lease, 2 * pool_bytes, &scratch);
@@ -1619,18 +1658,19 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
         SKV_HIP(launch_append(w, s));
         pages.k_new = w.k_pool;
         pages.v_new = w.v_pool;
-        if (g.fp4) SKV_HIP(launch_fp4_chunk(a, pages, shape4, s));
+        if (g.fp4) SKV_HIP(streams ? launch_fp4_attention(a, &pages, s) : launch_fp4_chunk(a, pages, shape4, s));
         else SKV_HIP(g.f32 ? launch_f32_prefill(a, pages, nullptr, halves, s) : launch_prefill_tiles(a, pages, shape, s));
     }
     if (a.splits_total == 1) return encode_append(L, s, k, v, c);
+    auto merge = [&] { return a.splits_total > 4 && streams ? launch_merge(a, s) : launch_merge_rows(a, s); };
     if (late) {
         rc = encode_append(L, s, k, v, c);
         if (rc) return rc;
-        SKV_HIP(launch_merge_rows(a, s));
+        SKV_HIP(merge());
         return SKV_OK;
     }
     if (g.fp4) {
-        SKV_HIP(launch_merge_rows(a, s));
+        SKV_HIP(merge());
         return encode_append(L, s, k, v, c);
     }
     SKV_HIP(launch_merge_append(a, append_args(L, k, v, c), s)); // (the caller has checked the capacity)
