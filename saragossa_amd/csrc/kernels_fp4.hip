@@ -2,6 +2,7 @@
 #include "append_tile.h"
 #include "fp4_tile.h"
 #include "lds_copy.h"
+#include "pre_kv.h"
 
 namespace skv {
 
@@ -242,8 +243,12 @@ struct Fp4Lds {
     static_assert((SHARED ? 0 : NB * BLOCK) + MQ_APPEND_ROWS * NEW_ROW + 16 + WAVES * WAVE <= 160 * 1024, "it all fits a compute unit's LDS");
 };
 // MQ: more than one query row, or more than 16 heads to a kv head: slots are (row, head) pairs, 16 to a workgroup (grid z). ROWS: the launch
-// stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one.
-template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false>
+// stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one. PRE: a step whose queries and new K row are
+// normed and rotated here, from LDS that belongs to the wavefronts' second pairs until the first barrier behind it (the
+// pairs lie by depth then, the states of the wavefronts over both behind one more barrier). A step of q32/kv8/hd128 over 2000 rows from its
+// projections: 9.5 us, 14.1 with norm, rotation and append as launches of their own; of q16/kv2/hd256, gated, 11.7 and 17.8. (The
+// step alone: 7.4 and 8.8. The chain load, ordered sum, rotation, digits is longer than the first pages' way.)
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false, bool PRE = false>
 __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const ChunkPages *c, const int split, const int kvh, const int tile_z) {
     using T = Fp4Tile<P>;
     constexpr int THREADS = WAVES * 64, G = T::G, U = T::U, NB = T::NB, VL = T::VL, NT = P / 16, OSTRIDE = P + 4;
@@ -292,7 +297,8 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     // them. The codes stay in LDS, from where a wavefront patches what it has loaded.
     using L = Fp4Lds<P, WAVES>;
     constexpr bool NEW = !MQ || ROWS;
-    constexpr int BY = ROWS ? THREADS : 64, MOST = ROWS ? MQ_APPEND_ROWS : 1, NU = (MOST * 2 * G * 8 + BY - 1) / BY;
+    // (PRE: V's groups alone, behind K's)
+    constexpr int BY = ROWS ? THREADS : 64, MOST = ROWS ? MQ_APPEND_ROWS : 1, FIRST = PRE ? G : 0, NU = ((MOST * 2 * G - FIRST) * 8 + BY - 1) / BY;
     const int C = ROWS ? a.n_queries : 1;
     const int p_new = a.len - C, e_new = (p_new - pos0) >> 4, e_last = (a.len - 1 - pos0) >> 4;
     const bool appends = NEW && a.k_new != nullptr && e_last >= pb0 && e_new < pb1;
@@ -301,14 +307,26 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     const int by = ROWS ? tid : lane;
     float nx[NU][4];
     int page_a = 0, page_b = 0;
+    using Pre = PreKvStage<P, THREADS>;
+    Pre pre;
+    float k_row[Pre::NE];
+    if constexpr (PRE) {
+        if (appends) page_a = a.table[place(min(max(e_new, 0), e_hi - 1))]; // uniform
+#pragma unroll
+        for (int u = 0; u < Pre::NE; ++u) {
+            k_row[u] = 0.0f;
+            if (appends && tid + u * THREADS < g.head_dim) k_row[u] = a.k_new[kvh * g.head_dim + tid + u * THREADS];
+        }
+        pre.load(a, kvh, rows, a.q_head_stride > 0 ? a.q_head_stride : g.head_dim, tid);
+    }
     if constexpr (NEW) {
         if (converts) { // uniform
             const bool vec = (g.head_dim & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.k_new) | reinterpret_cast<uintptr_t>(a.v_new)) & 15) == 0;
-            page_a = a.table[place(min(max(e_new, 0), e_hi - 1))];
+            if (!PRE) page_a = a.table[place(min(max(e_new, 0), e_hi - 1))];
             page_b = ROWS ? a.table[place(min(max(e_last, 0), e_hi - 1))] : page_a;
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                const int idx = (by + u * BY) >> 3, v = idx >= C * G, row = min((idx - v * C * G) / G, C - 1), d = (idx % G) * 32 + (tid & 7) * 4;
+                const int idx = FIRST + ((by + u * BY) >> 3), v = idx >= C * G, row = min((idx - v * C * G) / G, C - 1), d = (idx % G) * 32 + (tid & 7) * 4;
                 const float *src = (v ? a.v_new : a.k_new) + ((long)row * g.kv_heads + kvh) * g.head_dim;
                 if (vec) {
                     const float4_t x = *reinterpret_cast<const float4_t *>(src + min(d, g.head_dim - 4));
@@ -326,7 +344,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     constexpr int QU = (16 * P / 4 + THREADS - 1) / THREADS;
     float4_t x[QU];
 #pragma unroll
-    for (int u = 0; u < QU; ++u) {
+    for (int u = 0; u < (PRE ? 0 : QU); ++u) {
         const int idx = tid + u * THREADS, slot = (idx >> 3) / G, d = (idx >> 3) % G * 32 + (tid & 7) * 4;
         x[u] = float4_t{0.f, 0.f, 0.f, 0.f};
         if (slot < rows) {
@@ -344,8 +362,11 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     uint8_t *new_rows = lds + (L::SHARED ? 0 : NB * L::BLOCK);
     constexpr int NEW_ROW = L::NEW_ROW, AT_V = P / 2, AT_KP = P, AT_VP = P + G; // in a new row
     const int n_new = NEW ? C : 0;
-    uint8_t *const mine = lds + L::pairs(n_new) + wave * L::WAVE; // this wavefront's pairs
-    const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + (uint32_t)(L::pairs(n_new) + wave * L::WAVE);
+    constexpr int STEP = PRE ? WAVES * L::PAIR : L::PAIR; // from one of a wavefront's pairs to the next
+    const int mine_off = L::pairs(n_new) + wave * (PRE ? L::PAIR : L::WAVE);
+    uint8_t *const mine = lds + mine_off; // this wavefront's pairs
+    const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + (uint32_t)mine_off;
+    static_assert(!PRE || (!MQ && !L::SHARED && Pre::LDS_FLOATS * 4 <= (size_t)WAVES * L::PAIR), "norm and rotation in the second pairs' place");
     const int jk = G < 4 ? min(j, G - 1) : j; // (narrow heads: the lanes past the last group take it again, against queries of zero)
 
     // A pair's copies to LDS: COPIES instructions. The heads' codes are whole KiBs from 128 dims on; below, and the powers always, a lane of an instruction
@@ -375,7 +396,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         const uint32_t pa = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it) & 63), pb = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it + 1) & 63);
         const int e0 = pb0 + 2 * (wave + it * WAVES);
         const bool new_a = RING && min(e0, e_hi - 1) >= n_old, new_b = RING && min(e0 + 1, e_hi - 1) >= n_old;
-        const uint32_t to = mine_at + (uint32_t)((it % L::DEPTH) * L::PAIR);
+        const uint32_t to = mine_at + (uint32_t)((it % L::DEPTH) * STEP);
         const auto address = [&](const Part &p) __attribute__((always_inline)) {
             const uint8_t *from = p.from + (uint64_t)(p.second ? pb : pa) * page_bytes;
             if constexpr (RING) {
@@ -406,14 +427,53 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 #pragma unroll
         for (int u = 0; u < NU; ++u) asm volatile("" : "+v"(nx[u][0]), "+v"(nx[u][1]), "+v"(nx[u][2]), "+v"(nx[u][3]));
     }
+    if constexpr (PRE) {
 #pragma unroll
-    for (int u = 0; u < QU; ++u) asm volatile("" : "+v"(x[u]));
+        for (int u = 0; u < Pre::U; ++u) asm volatile("" : "+v"(pre.q[u]));
+#pragma unroll
+        for (int u = 0; u < Pre::NE; ++u) asm volatile("" : "+v"(pre.wq[u]), "+v"(pre.wk[u]), "+v"(pre.rot[u]), "+v"(k_row[u]));
+    } else {
+#pragma unroll
+        for (int u = 0; u < QU; ++u) asm volatile("" : "+v"(x[u]));
+    }
     if (0 < n_it) copy_pair(0); // uniform
 
+    // an eighth of a group of a new row, to LDS and, from the tile that stores, to the page: K's, V's
+    auto row_pool = [&](int v, int row, uint8_t *&codes, uint8_t *&powers) __attribute__((always_inline)) {
+        const int e = (p_new + row - pos0) >> 4, page = e == e_new ? page_a : page_b;
+        uint16_t *pool = const_cast<uint16_t *>(v ? a.v_pool : a.k_pool);
+        codes = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), powers = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
+        return stores && e >= pb0 && e < pb1;
+    };
+    auto k_eighth = [&](int row, int t, int o8, uint32_t codes, uint32_t power) __attribute__((always_inline)) {
+        uint8_t *cp, *pp, *to = new_rows + row * NEW_ROW;
+        const bool store = row_pool(0, row, cp, pp);
+        const int r = (p_new + row) & 15;
+        *reinterpret_cast<uint16_t *>(to + t * 16 + o8 * 2) = (uint16_t)codes;
+        if (o8 == 0) to[AT_KP + t] = (uint8_t)power;
+        if (store) {
+            *reinterpret_cast<uint16_t *>(cp + k4_code(r, t * 32 + o8 * 4)) = (uint16_t)codes;
+            if (o8 == 0) pp[k4_power(P, r, t)] = (uint8_t)power;
+        }
+    };
+    auto v_eighth = [&](int row, int t, int o8, uint32_t codes, uint32_t other, uint32_t power) __attribute__((always_inline)) {
+        if (o8 >= 4) return;
+        uint8_t *cp, *pp, *to = new_rows + row * NEW_ROW;
+        const bool store = row_pool(1, row, cp, pp);
+        const int r = (p_new + row) & 15;
+        const uint32_t word = nibbles_apart(codes) | nibbles_apart(other) << 4;
+        *reinterpret_cast<uint32_t *>(to + AT_V + t * 16 + o8 * 4) = word;
+        if (o8 == 0) to[AT_VP + t] = (uint8_t)power;
+        if (store) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) cp[v4_code(P, r, t * 32 + o8 * 4 + k)] = (uint8_t)(word >> (8 * k));
+            if (o8 == 0) pp[v4_power(P, r, t)] = (uint8_t)power;
+        }
+    };
     auto convert_rows = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int idx = (by + u * BY) >> 3, v = idx >= C * G, row = (idx - v * C * G) / G, t = idx % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+            const int idx = FIRST + ((by + u * BY) >> 3), v = idx >= C * G, row = (idx - v * C * G) / G, t = idx % G, o8 = tid & 7, d = t * 32 + o8 * 4;
             const bool real = idx < 2 * C * G;
 #pragma unroll
             for (int e = 0; e < 4; ++e) nx[u][e] = real && d + e < g.head_dim ? nx[u][e] : 0.0f;
@@ -421,45 +481,20 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             const uint32_t codes = fp4_codes_of(nx[u], power);
             const uint32_t other = (uint32_t)__shfl_xor((int)codes, 4);
             if (!real) continue;
-            uint8_t *to = new_rows + row * NEW_ROW;
-            const int e = (p_new + row - pos0) >> 4, r = (p_new + row) & 15, page = e == e_new ? page_a : page_b;
-            const bool store = stores && e >= pb0 && e < pb1;
-            uint16_t *pool = const_cast<uint16_t *>(v ? a.v_pool : a.k_pool);
-            uint8_t *cp = const_cast<uint8_t *>(fp4_codes(pool, g, page, kvh)), *pp = const_cast<uint8_t *>(fp4_powers(pool, g, page, kvh));
-            if (!v) {
-                *reinterpret_cast<uint16_t *>(to + t * 16 + o8 * 2) = (uint16_t)codes;
-                if (o8 == 0) to[AT_KP + t] = (uint8_t)power;
-                if (store) {
-                    *reinterpret_cast<uint16_t *>(cp + k4_code(r, d)) = (uint16_t)codes;
-                    if (o8 == 0) pp[k4_power(P, r, t)] = (uint8_t)power;
-                }
-            } else if (o8 < 4) {
-                const uint32_t word = nibbles_apart(codes) | nibbles_apart(other) << 4;
-                *reinterpret_cast<uint32_t *>(to + AT_V + t * 16 + o8 * 4) = word;
-                if (o8 == 0) to[AT_VP + t] = (uint8_t)power;
-                if (store) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) cp[v4_code(P, r, d + k)] = (uint8_t)(word >> (8 * k));
-                    if (o8 == 0) pp[v4_power(P, r, t)] = (uint8_t)power;
-                }
-            }
+            if (!v) k_eighth(row, t, o8, codes, power);
+            else v_eighth(row, t, o8, codes, other, power);
         }
     };
-#pragma unroll
-    for (int u = 0; u < QU; ++u) {
-        const int idx = tid + u * THREADS, slot = (idx >> 3) / G, t = (idx >> 3) % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+    auto no_query = [&](int slot, int t) __attribute__((always_inline)) { // (nothing reads what becomes of it)
+        reinterpret_cast<uint32_t *>(lds + L::block(t >> 2, n_new))[4 * 6 * 64 + (t & 3) * 16 + slot] = 0;
+    };
+    // an eighth of a group of a slot's queries, to its place among the terms
+    auto query_eighth = [&](int slot, int t, int o8, float4_t y) __attribute__((always_inline)) {
         uint32_t *const to = reinterpret_cast<uint32_t *>(lds + L::block(t >> 2, n_new)); // of the block, lane (slot, t % 4)
         const int at = (t & 3) * 16 + slot;
-        if (slot >= rows) {
-            if (slot < 16 && o8 == 0) to[4 * 6 * 64 + at] = 0; // (nothing reads what becomes of it)
-            continue;
-        }
         float top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[u][e] = d + e < g.head_dim ? x[u][e] : 0.0f;
-            top = __uint_as_float(max(__float_as_uint(top), magnitude(x[u][e])));
-        }
+        for (int e = 0; e < 4; ++e) top = __uint_as_float(max(__float_as_uint(top), magnitude(y[e])));
         const uint32_t most = max_of_8(magnitude(top * a.qscale));
         // the values as whole numbers X of 20 bits, |X| <= 2^19, in digits of base 32 between -16 and 15 (the first: 16). A float at
         // 1.5 * 2^23 + (X + 16 (1 + 32 + 1024)) holds them in its last bits, 16 too large but for the first.
@@ -467,7 +502,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         const float scale = a.qscale * __uint_as_float((uint32_t)(272 - power) << 23);
         uint32_t digits[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) digits[e] = __float_as_uint(__builtin_fmaf(x[u][e], scale, 12582912.0f + 16912.0f));
+        for (int e = 0; e < 4; ++e) digits[e] = __float_as_uint(__builtin_fmaf(y[e], scale, 12582912.0f + 16912.0f));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint32_t four = 0;
@@ -480,6 +515,37 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         }
         if (o8 == 0)
             to[4 * 6 * 64 + at] = most >= 0x7f800000u ? 0xffffffffu : (uint32_t)(power | (power - 5) << 8 | (power - 10) << 16) | (uint32_t)(power - 15) << 24;
+    };
+    if constexpr (PRE) {
+        float *const pre_lds = reinterpret_cast<float *>(lds + L::pairs(n_new) + WAVES * L::PAIR);
+        pre.stage(pre_lds, a, rows, k_row, tid);
+        for (int i = rows * G + tid; i < 16 * G; i += THREADS) no_query(i / G, i % G);
+        const int n_rows = rows + (appends ? 1 : 0);
+        __syncthreads();
+        Pre::scales(pre_lds, a, rows, n_rows, tid);
+        __syncthreads();
+        Pre::each(pre_lds, a, rows, n_rows, tid, [&](int r, int c4, float4_t y) __attribute__((always_inline)) {
+            if (r < rows) { // (eight lanes alike)
+                query_eighth(r, c4 >> 3, c4 & 7, y);
+            } else {
+                float z[4] = {y[0], y[1], y[2], y[3]};
+                uint32_t power;
+                const uint32_t codes = fp4_codes_of(z, power);
+                k_eighth(0, c4 >> 3, c4 & 7, codes, power);
+            }
+        });
+    } else {
+#pragma unroll
+        for (int u = 0; u < QU; ++u) {
+            const int idx = tid + u * THREADS, slot = (idx >> 3) / G, t = (idx >> 3) % G, o8 = tid & 7, d = t * 32 + o8 * 4;
+            if (slot >= rows) {
+                if (slot < 16 && o8 == 0) no_query(slot, t);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] = d + e < g.head_dim ? x[u][e] : 0.0f;
+            query_eighth(slot, t, o8, x[u]);
+        }
     }
     if constexpr (ROWS) {
         if (converts) convert_rows(); // uniform
@@ -527,7 +593,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         // ---- the pair, from LDS: the copies behind its own may still be on their way
         if (it + L::DEPTH <= n_it) copies_left<(L::DEPTH - 1) * COPIES>(); // uniform
         else copies_landed();
-        const uint8_t *const pair = mine + (it % L::DEPTH) * L::PAIR;
+        const uint8_t *const pair = mine + (it % L::DEPTH) * STEP;
         uint32_t kc[2][NB][4], kp[2], vc[2][G], vp[2][G];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -674,6 +740,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         if constexpr (P > 128) next_pair(it + L::DEPTH);
     }
     l_run = rows_sum(l_run);
+    if constexpr (PRE) __syncthreads(); // (a state lies over other wavefronts' pairs)
 
     // ---- the wavefronts' states meet in LDS, four columns a thread
     // [WAVES] of [rows][OSTRIDE], m [rows], l [rows]
@@ -713,6 +780,14 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         float *dst;
         if (a.splits_total == 1) {
             acc *= 1.0f / lsum;
+            if constexpr (PRE) {
+                if (a.gate) {
+                    const float *gate = a.gate + (long)(kvh * g.gqa + slot) * (a.q_head_stride > 0 ? a.q_head_stride : g.head_dim) + c4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c4 + i < g.head_dim) acc[i] *= sigmoid_gate(gate[i]);
+                }
+            }
             dst = a.out + (MQ ? context_row(g, kvh, slot) : (long)(kvh * g.gqa + slot)) * g.head_dim + c4;
         } else {
             const long pidx = ((long)kvh * a.splits_total + split) * n_slots + slot;
@@ -732,9 +807,9 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     }
 }
 
-template <int P, int WAVES, bool MQ, bool RING, bool ROWS>
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS, bool PRE>
 __global__ __launch_bounds__(WAVES * 64) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
-    fp4_attention_body<P, WAVES, MQ, RING, ROWS>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
+    fp4_attention_body<P, WAVES, MQ, RING, ROWS, PRE>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // Several sequences of the same model layer: grid z is the sequence, grid x covers the largest number of splits
@@ -745,29 +820,33 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_attention_batch_kernel(DecodeB
     fp4_attention_body<P, WAVES, false, false>(a, nullptr, blockIdx.x, blockIdx.y, 0);
 }
 
-template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false>
+template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false, bool PRE = false>
 static hipError_t launch_fp4_of(const DecodeArgs &a, const ChunkPages &c, hipStream_t s) {
     static std::atomic<uint64_t> lds_ok{0}; // per instantiation
     {
-        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_kernel<P, WAVES, MQ, RING, ROWS>), lds_ok);
+        hipError_t e = allow_full_lds(reinterpret_cast<const void *>(&fp4_attention_kernel<P, WAVES, MQ, RING, ROWS, PRE>), lds_ok);
         if (e != hipSuccess) return e;
     }
     const int n_slots = a.n_queries * a.g.gqa;
     const dim3 grid((unsigned)a.splits, (unsigned)a.g.kv_heads, (unsigned)((n_slots + 15) / 16));
     const size_t lds = Fp4Lds<P, WAVES>::bytes(ROWS ? a.n_queries : MQ ? 0 : 1);
-    hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING, ROWS>), grid, dim3(WAVES * 64), lds, s, a, c);
+    hipLaunchKernelGGL((fp4_attention_kernel<P, WAVES, MQ, RING, ROWS, PRE>), grid, dim3(WAVES * 64), lds, s, a, c);
     return hipGetLastError();
 }
 template <int P, int WAVES>
 static hipError_t launch_fp4(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
     if (a.k_new && (c || a.n_queries > MQ_APPEND_ROWS)) return hipErrorInvalidValue;
+    if (a.pre) {
+        if constexpr (P > 256) return hipErrorInvalidValue; // the caller sends these through separate launches
+        else return c || a.n_queries > 1 || a.g.gqa > 16 || !a.k_new ? hipErrorInvalidValue : launch_fp4_of<P, WAVES, false, false, false, true>(a, ChunkPages{}, s);
+    }
     if (c) return launch_fp4_of<P, WAVES, true, true>(a, *c, s);
     if (a.n_queries == 1 && a.g.gqa <= 16) return launch_fp4_of<P, WAVES, false, false>(a, ChunkPages{}, s);
     return a.k_new ? launch_fp4_of<P, WAVES, true, false, true>(a, ChunkPages{}, s) : launch_fp4_of<P, WAVES, true, false>(a, ChunkPages{}, s);
 }
 
 hipError_t launch_fp4_attention(const DecodeArgs &a, const ChunkPages *c, hipStream_t s) {
-    if (a.pre || a.split_base != 0) return hipErrorInvalidValue;
+    if (a.split_base != 0) return hipErrorInvalidValue;
     switch (a.g.P) {
     case 32: return launch_fp4<32, 8>(a, c, s);
     case 64: return launch_fp4<64, 8>(a, c, s);

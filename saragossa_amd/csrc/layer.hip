@@ -777,6 +777,18 @@ struct PreKv {
     int q_head_stride;  // elements between the heads of q and of gate (0 = head_dim)
 };
 
+void with_pre(DecodeArgs &a, const PreKv &pre) {
+    a.pre = 1;
+    a.rope = pre.rope;
+    a.q_norm_w = pre.q_norm_w;
+    a.k_norm_w = pre.k_norm_w;
+    a.eps = pre.eps;
+    a.rope_dims = pre.rope ? pre.rope_dims : 0;
+    a.rope_style = pre.rope_style;
+    a.gate = pre.gate;
+    a.q_head_stride = pre.q_head_stride;
+}
+
 // Points the launch's split partials at `buf` instead of the layer's own buffers
 // (decode, one query row): [kv_heads][splits][gqa] of (o[head_dim], m, l).
 int32_t partials_in(void *buf, size_t buf_bytes, DecodeArgs &a) {
@@ -835,17 +847,7 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
         fill_decode_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, decode_target_wgs(), a);
         if ((k_new || v_new || pre) && n_queries == 1 && !f32_decode_kernel_serves(a))
             return fail(SKV_ERR_CONFIG, "KV f32: étape fusionnée non construite pour cette forme");
-        if (pre) {
-            a.pre = 1;
-            a.rope = pre->rope;
-            a.q_norm_w = pre->q_norm_w;
-            a.k_norm_w = pre->k_norm_w;
-            a.eps = pre->eps;
-            a.rope_dims = pre->rope ? pre->rope_dims : 0;
-            a.rope_style = pre->rope_style;
-            a.gate = pre->gate;
-            a.q_head_stride = pre->q_head_stride;
-        }
+        if (pre) with_pre(a, *pre);
         if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
         const bool by_terms = n_queries > 1 && takes_f32_chunk_kernel(g, n_queries, (size_t)a.n_pages);
         const auto store_rows = [&]() -> int32_t { // rows that the terms' launch would have stored
@@ -923,9 +925,9 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
     }
     const bool use_flash = uses_flash(L) || n_queries > 1;
     if (g.fp4 && use_flash) {
-        if (pre) return fail(SKV_ERR_CONFIG, "KV 4 bits: étape fusionnée non construite pour cette forme");
         DecodeArgs a{};
         fill_fp4_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, decode_target_wgs(), a);
+        if (pre) with_pre(a, *pre);
         if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
         const bool by_chunk = n_queries > 1 && !k_new && takes_fp4_chunk_kernel(g, n_queries, (size_t)a.n_pages);
         TileShape shape = TileShape::one_tile;
@@ -983,17 +985,7 @@ int32_t encode_attention(skv_layer *L, hipStream_t s, const float *q_dev, float 
     DecodeArgs a{};
     fill_decode_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, decode_target_wgs(), a, false, !over);
     if (attn_scalar > 0.0f) a.qscale = (1.0f / std::sqrt(attn_scalar)) * 1.4426950408889634f;
-    if (pre) {
-        a.pre = 1;
-        a.rope = pre->rope;
-        a.q_norm_w = pre->q_norm_w;
-        a.k_norm_w = pre->k_norm_w;
-        a.eps = pre->eps;
-        a.rope_dims = pre->rope ? pre->rope_dims : 0;
-        a.rope_style = pre->rope_style;
-        a.gate = pre->gate;
-        a.q_head_stride = pre->q_head_stride;
-    }
+    if (pre) with_pre(a, *pre);
     const bool use_tiles = n_queries > 1 && takes_tile_kernel(a.g, n_queries, (size_t)a.n_pages);
     TileShape shape = TileShape::one_tile;
     if (n_queries > 1) {
@@ -2035,7 +2027,7 @@ static int32_t prekv_step(skv_layer *L, skv_stream stream, const skv_rope *rope,
                                            std::to_string(L->capacity) + " atteinte (overflow)");
     hipStream_t s = as_stream(stream);
     const bool fused = tuning().fused_append;
-    if (!fused || !uses_flash(L) || wide_f32_heads(L) || L->g.fp4 || L->g.gqa > 16) {
+    if (!fused || !uses_flash(L) || wide_f32_heads(L) || (L->g.fp4 && L->g.P > 256) || L->g.gqa > 16) {
         // the same step as separate launches: norm + rotation of q and k, append, attention, gate
         NormRopeArgs n{};
         n.x = q;
