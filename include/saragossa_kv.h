@@ -16,7 +16,8 @@
  * block table; logical row r of the reference's contiguous cache is
  * (block_table[r / 16], r % 16) here. A layer's elements are bf16, rounded from
  * f32 with the reference's integer formula (src/decode_resident/utils.rs:55-60),
- * or f32 kept verbatim (GpuElement, src/decode_resident/attention.rs:26-45).
+ * or f32 kept verbatim (GpuElement, src/decode_resident/attention.rs:26-45), or codes of
+ * 4 bits, which the reference does not have (skv_layer_create).
  */
 #ifndef SARAGOSSA_KV_H
 #define SARAGOSSA_KV_H
@@ -94,7 +95,7 @@ size_t skv_sdpa_2pass_blocks(size_t len);         /* utils.rs:282-286 */
 /* Rows below which this library never splits the context of a decode launch: RETI_RUST_SDPA_2PASS_MIN_LEN
  * when it is set (the reference's parse, default 2048 when unparsable), and then it splits from there on; else 128.
  * While neither it nor SKV_DECODE_WGS, SKV_PREFILL_WGS, SKV_DECODE_MIN_PAGES or SKV_DECODE_WAVES is set, contexts that are
- * faster whole stay so for longer: steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
+ * faster whole stay so for longer: steps of 4-bit layers up to 256 rows (heads above 256 dims 128), steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
  * batches further the more sequences and kv heads they have (16 sequences of 8 kv heads 784, 656, 416), chunks of up to some
  * hundred rows up to 400 to 1500. The reference's
  * own default (2048, utils.rs:270-278) is what skv_flag_sdpa_2pass_min_len reports; it was tuned
@@ -178,8 +179,13 @@ int32_t skv_ctx_synchronize(skv_ctx *ctx);
  * src/decoder/attention_cache.rs:72-100); 0 keeps all `capacity` rows in pages.
  * `dtype` is what the pages hold: SKV_DTYPE_BF16 (rows rounded to nearest even at append,
  * room for pages of kv_heads * P * 32 bytes per tensor, P = head_dim rounded up to a power of two) or
- * SKV_DTYPE_F32 (rows verbatim; pages twice the bytes). head_dim up to 512 in both. Every
- * entry point below serves both; where they differ it says so. */
+ * SKV_DTYPE_F32 (rows verbatim; pages twice the bytes), or SKV_DTYPE_FP4: per row and 32 dims of a head (a group;
+ * a head's last one may be shorter) a power 2^e and the dims as codes e2m1, 4 bits each, 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with
+ * a sign, times it: 4.25 bits a value, 17 bytes where bf16 has 64. e is the smallest in [-125, 125] with max |x| <= 7 * 2^e, a
+ * value the nearest code times 2^e, ties to the even code, off by at most 2^e, which is between 1/7 and 2/7 of the group's largest
+ * value. A group that holds a NaN or an infinity reads back as NaN, and is NaN to every query that attends it. Values
+ * read back are exact in bf16. head_dim up to 512 in all. Every
+ * entry point below serves all three; where they differ it says so. */
 int32_t skv_layer_create(skv_ctx *ctx, size_t capacity, size_t q_heads, size_t kv_heads,
                          size_t head_dim, int32_t dtype, size_t window, skv_layer **out);
 /* skv_layer_create with the rollback depth of a ring layer as an argument: the ring keeps
@@ -201,7 +207,7 @@ void skv_layer_destroy(skv_layer *layer);
  * table, split partials, staging rows), after the same checks: what a host adds up before it
  * creates a model's layers, where the reference adds up 2 * capacity * kv_dim * 4 per layer
  * (check_resident_full_decode_allocation, src/decoder/resident/setup.rs:897-962). A bf16
- * layer takes about half of an f32 one; a ring layer's size follows its window, not capacity. */
+ * layer takes about half of an f32 one, a 4-bit one about 17/64 of a bf16 one; a ring layer's size follows its window, not capacity. */
 int32_t skv_layer_bytes(size_t capacity, size_t q_heads, size_t kv_heads, size_t head_dim, int32_t dtype,
                         size_t window, uint64_t *bytes);
 /* The same for skv_layer_create_ring (no counterpart in the reference, whose caches are never rings). */
@@ -229,7 +235,8 @@ size_t skv_q_heads(const skv_layer *layer);
 size_t skv_kv_heads(const skv_layer *layer);
 size_t skv_head_dim(const skv_layer *layer);
 size_t skv_window(const skv_layer *layer);
-/* keys().byte_len() of the reference for the same capacity (tests.rs:446): capacity*kv_dim*2. */
+/* keys().byte_len() of the reference for the same capacity (tests.rs:446): capacity*kv_dim*2 (f32 layers 4; 4-bit ones
+ * capacity * kv_heads * (ceil(head_dim / 2) + ceil(head_dim / 32))). */
 size_t skv_logical_byte_len(const skv_layer *layer);
 /* truncate(len) (attention.rs:496-505): error if len > capacity. */
 int32_t skv_truncate(skv_layer *layer, size_t len);
@@ -264,7 +271,7 @@ int32_t skv_attention_device(skv_layer *layer, skv_stream stream, const float *q
 /* append + attention of one token in one call (layers.rs:259-288 does the two
  * encodes back to back). window_start is derived from the layer's window. On the GPU it is one
  * launch pair (the attention kernel stores the new row itself) for bf16 layers up to head_dim
- * 512 and for f32 layers up to head_dim 256 with at most 16 query heads per kv head; other
+ * 512, for 4-bit layers, and for f32 layers up to head_dim 256 with at most 16 query heads per kv head; other
  * f32 shapes, and every shape with RETI_RUST_FLASH_SDPA=0, take an append launch first (the
  * f32 kernel for wide heads has no registers to spare: with the append built into it the step
  * takes 48.7 us against 44.1 us at 4096 rows of q16/kv8/hd512, 260 against 253 us at 32768). */
@@ -349,8 +356,8 @@ int32_t skv_rms_norm_rope_decode_host(skv_ctx *ctx, const float *x, const float 
  * attn_scalar is SKV_ERR_CONFIG), append of (k, v) and attention through the layer's
  * window. q_norm_w / k_norm_w: device f32[head_dim], null = that norm is skipped. The
  * finished q is not written back; the appended k row is the CPU path's row bit for bit.
- * (One launch pair on bf16 layers of any head_dim and on f32 layers up to head_dim 256, at
- * most 16 query heads per kv head; on f32 layers with wider heads, or more heads per group,
+ * (One launch pair on bf16 layers of any head_dim and on f32 and 4-bit layers up to head_dim 256, at
+ * most 16 query heads per kv head; on f32 and 4-bit layers with wider heads, or more heads per group,
  * the norm and rotation, the append and the attention are separate launches with the same
  * result. Measured on one MI355X at q16/kv8/hd512: an f32 layer's step as those four launches
  * takes 61 us at 4096 cached rows and 267 us at 32768, its attention launches alone 41 us and
@@ -386,7 +393,7 @@ int32_t skv_attn_gate_device(skv_ctx *ctx, skv_stream stream, const float *ctx_d
  * src/decode_resident/layers.rs:259-288, once per sequence); this is that call applied to
  * a batch, with the same result per sequence. All handles must share the head geometry,
  * the element, the window and the context, and be distinct; nothing is modified when one of
- * them is at capacity. (One launch pair on either element up to 16 query heads per kv head,
+ * them is at capacity. (One launch pair on any element up to 16 query heads per kv head,
  * f32 layers up to head_dim 256; other shapes run a launch pair per sequence.) A context may lie over its own
  * sequence's inputs, as in a step; over another's in a batch of up to 16 that is one launch pair. */
 int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_stream stream,
@@ -405,12 +412,13 @@ int32_t skv_decode_step_layers_device(skv_layer *const *layers, size_t n_layers,
 
 /* Reads logical rows [first, first+n) through the block table as bf16 bits,
  * row-major [n, kv_dim]: the stand-in for reading keys()/values() back
- * (tests.rs:423-428, 469-476). Synchronous. bf16 layers only (SKV_ERR_CONFIG on an f32 one). */
+ * (tests.rs:423-428, 469-476). Synchronous. bf16 layers, and 4-bit ones, whose values bf16 holds exactly
+ * (SKV_ERR_CONFIG on an f32 one). */
 int32_t skv_read_rows(skv_layer *layer, size_t first, size_t n, uint16_t *k_out, uint16_t *v_out);
-/* The same rows as f32, for layers of either element type (bf16 rows widen exactly). */
+/* The same rows as f32, for layers of any element type (bf16 and 4-bit rows widen exactly). */
 int32_t skv_read_rows_f32(skv_layer *layer, size_t first, size_t n, float *k_out, float *v_out);
 /* Same gather, device to device, async on `stream`; the destination rows have the layer's
- * element type (bf16 bits or f32). */
+ * element type (bf16 bits or f32; of a 4-bit layer the values they stand for, as bf16 bits). */
 int32_t skv_gather_device(skv_layer *layer, skv_stream stream, size_t first, size_t n,
                           void *k_dst_dev, void *v_dst_dev);
 

@@ -505,7 +505,7 @@ bool uses_flash(const skv_layer *L) { return skv_flag_flash_sdpa_enabled() && L-
 // on f32 layers where the f32 decode kernel serves the shape (head_dim up to 256, at most 16
 // heads per group).
 bool fused_append_built(const skv_layer *L) { return !L->g.f32 || (L->g.P <= 256 && L->g.gqa <= 16); }
-// The fused pre-KV step is built for bf16 layers up to head_dim 512 and for f32 layers up to
+// The fused pre-KV step is built for bf16 layers up to head_dim 512 and for f32 and 4-bit layers up to
 // head_dim 256; wide f32 heads take the separate norm/rotation launches.
 bool wide_f32_heads(const skv_layer *L) { return L->g.f32 && L->g.P > 256; }
 
