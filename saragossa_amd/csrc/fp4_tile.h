@@ -112,4 +112,13 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
 
 #endif
 
+// Entry e of a ring chunk's list of pages (ChunkPages): whether it lies in the chunk's scratch, and its page there or in the layer's pools.
+__device__ __forceinline__ bool fp4_in_scratch(const ChunkPages &c, int e) { return e >= c.apart_lo && e < c.apart_hi; }
+__device__ __forceinline__ int fp4_ring_page(const DecodeArgs &a, const ChunkPages &c, int e) {
+    int at = e < c.n_old ? c.start + e : c.new_start + min(e - c.n_old, c.ring_pages - 1);
+    if (at >= c.ring_pages) at -= c.ring_pages;
+    const int page = a.table[max(at, 0)]; // (every lane asks for some entry: no load of its own under a condition)
+    return fp4_in_scratch(c, e) ? c.apart_id + e : page;
+}
+
 } // namespace skv

@@ -36,7 +36,8 @@ __device__ __forceinline__ uint32_t fp6_codes_of(uint32_t u) {
 // 16 bits are the lane's 16 bytes of the matrix operand as they stand. V: a byte holds the dims c and c + 16, which lanes four apart exchange, and a
 // word the byte of four rows, which lanes eight apart exchange; a quad of rows that the batch covers is stored as words, one that it
 // shares with older rows as bytes.
-// A workgroup takes PER times 256 such eighths of one (page, kv head), of K and of V, all loads in front of the first conversion.
+// A workgroup takes PER times 256 such eighths of one (page, kv head), of K and of V, all loads in front of the first conversion. SAVE: what the
+// page held goes to a page of its own first, every byte by the thread that writes in its place.
 // ------------------------------------------------------------------------------------
 struct Fp4Unit { // of a thread: which eighth of which group of which row
     int o, i, quad, grp;
@@ -55,7 +56,7 @@ struct Fp4Unit { // of a thread: which eighth of which group of which row
 constexpr long FP4_WGS = 4096; // workgroups from which each takes twice as much
 static int fp4_parts(int P) { return (P / 32 + 1) / 2; }
 
-template <int PER>
+template <int PER, bool SAVE = false>
 __global__ __launch_bounds__(256) void store_fp4_kernel(AppendArgs a) {
     const Geom g = a.g;
     const int groups = g.P >> 5, kvh = blockIdx.y;
@@ -90,11 +91,40 @@ __global__ __launch_bounds__(256) void store_fp4_kernel(AppendArgs a) {
     const int page = __builtin_amdgcn_readfirstlane(a.table ? asked : logical);
     uint8_t *const kp = const_cast<uint8_t *>(fp4_powers(a.k_pool, g, page, kvh)), *const vp = const_cast<uint8_t *>(fp4_powers(a.v_pool, g, page, kvh));
     uint8_t *const kc = const_cast<uint8_t *>(fp4_codes(a.k_pool, g, page, kvh)), *const vc = const_cast<uint8_t *>(fp4_codes(a.v_pool, g, page, kvh));
+    uint32_t held[PER][4]; // SAVE: what is there so far, K's codes, V's, their powers
+    if constexpr (SAVE) {
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
+            const int grp = min(u.grp, groups - 1), d = grp * 32 + u.o * 4;
+            held[p][0] = *reinterpret_cast<const uint16_t *>(kc + k4_code(u.row(), d));
+            held[p][1] = *reinterpret_cast<const uint32_t *>(vc + v4_code(g.P, u.quad * 4, grp * 32 + (u.o & 3) * 4 + u.i));
+            held[p][2] = kp[k4_power(g.P, u.row(), grp)];
+            held[p][3] = vp[v4_power(g.P, u.row(), grp)];
+        }
+    }
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
         const Fp4Unit u(groups, (int)blockIdx.z * PER + p);
         const int r = u.row(), d = u.dim();
         const bool in = u.real && r >= r_lo && r < r_hi;
+        if constexpr (SAVE) {
+            if (u.real) {
+                uint16_t *const pools[2] = {a.k_save, a.v_save};
+                uint8_t *codes[2], *powers[2];
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    codes[v] = const_cast<uint8_t *>(fp4_codes(pools[v], g, blockIdx.x, kvh));
+                    powers[v] = const_cast<uint8_t *>(fp4_powers(pools[v], g, blockIdx.x, kvh));
+                }
+                *reinterpret_cast<uint16_t *>(codes[0] + k4_code(r, d)) = (uint16_t)held[p][0];
+                if (u.o < 4) *reinterpret_cast<uint32_t *>(codes[1] + v4_code(g.P, u.quad * 4, d + u.i)) = held[p][1];
+                if (u.o == 0) {
+                    powers[0][k4_power(g.P, r, u.grp)] = (uint8_t)held[p][2];
+                    powers[1][v4_power(g.P, r, u.grp)] = (uint8_t)held[p][3];
+                }
+            }
+        }
         uint32_t codes[2], power[2];
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
@@ -138,7 +168,8 @@ hipError_t launch_store_fp4(const AppendArgs &a, hipStream_t s) {
     const int parts = fp4_parts(a.g.P);
     const bool two = parts % 2 == 0 && pages * a.g.kv_heads * parts > FP4_WGS;
     const dim3 grid((unsigned)pages, (unsigned)a.g.kv_heads, (unsigned)(two ? parts / 2 : parts));
-    if (two) hipLaunchKernelGGL(store_fp4_kernel<2>, grid, dim3(256), 0, s, b);
+    if (a.k_save) hipLaunchKernelGGL((store_fp4_kernel<1, true>), dim3(grid.x, grid.y, (unsigned)parts), dim3(256), 0, s, b);
+    else if (two) hipLaunchKernelGGL(store_fp4_kernel<2>, grid, dim3(256), 0, s, b);
     else hipLaunchKernelGGL(store_fp4_kernel<1>, grid, dim3(256), 0, s, b);
     return hipGetLastError();
 }
@@ -267,8 +298,9 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     const int ws_lo = start_of(tile * 16), ws_hi = start_of(tile * 16 + rows - 1);
 
     // The pages as a list in the order of positions: entry e < n_old is table[start + e] (less ring_pages past the ring's end), whose first
-    // row has position pos0 + 16 e; behind them (RING) pages outside the layer with the chunk's own rows.
+    // row has position pos0 + 16 e; behind them (RING) those of the chunk's own rows. (Of a ring some lie outside the layer, see ChunkPages.)
     const int pos0 = a.page_first * 16, n_old = RING ? c->n_old : INT32_MAX;
+    const int apart_lo = RING ? c->apart_lo : 0, apart_hi = RING ? c->apart_hi : 0;
     auto entry_pos = [&](int e) { return RING && e >= n_old ? c->new_first + (e - n_old) * 16 : pos0 + e * 16; };
     auto entry_of = [&](int pos) { return RING && pos >= c->new_pos0 ? n_old + ((pos - c->new_first) >> 4) : max(pos - pos0, 0) >> 4; };
     const int e_lo = entry_of(ws_lo), e_hi = entry_of(lim_hi) + 1;
@@ -279,7 +311,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     const int pairs = (pb1 - pb0 + 1) >> 1, n_it = pairs > wave ? (pairs - wave + WAVES - 1) / WAVES : 0;
     // place of an entry in the table
     auto place = [&](int e) __attribute__((always_inline)) {
-        int at = a.ring_base + min(e, n_old - 1);
+        int at = a.ring_base + e;
         if (at >= a.ring_t) at -= a.ring_t;
         return max(at, 0);
     };
@@ -287,8 +319,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     int ids = 0;
     auto fetch_ids = [&](int it) __attribute__((always_inline)) {
         const int e = min(pb0 + 2 * (wave + (it + (lane >> 1)) * WAVES) + (lane & 1), e_hi - 1);
-        const int page = a.table[place(e)];
-        ids = RING && e >= n_old ? e - n_old : page;
+        ids = RING ? fp4_ring_page(a, *c, e) : a.table[place(e)];
     };
     fetch_ids(0);
 
@@ -395,20 +426,21 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     auto copy_pair = [&](int it) __attribute__((always_inline)) {
         const uint32_t pa = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it) & 63), pb = (uint32_t)__builtin_amdgcn_readlane(ids, (2 * it + 1) & 63);
         const int e0 = pb0 + 2 * (wave + it * WAVES);
-        const bool new_a = RING && min(e0, e_hi - 1) >= n_old, new_b = RING && min(e0 + 1, e_hi - 1) >= n_old;
+        const int ea = min(e0, e_hi - 1), eb = min(e0 + 1, e_hi - 1);
+        const bool apart_a = RING && ea >= apart_lo && ea < apart_hi, apart_b = RING && eb >= apart_lo && eb < apart_hi;
         const uint32_t to = mine_at + (uint32_t)((it % L::DEPTH) * STEP);
         const auto address = [&](const Part &p) __attribute__((always_inline)) {
             const uint8_t *from = p.from + (uint64_t)(p.second ? pb : pa) * page_bytes;
             if constexpr (RING) {
-                if (p.second ? new_b : new_a) from += p.v ? (const uint8_t *)c->v_new - (const uint8_t *)a.v_pool : (const uint8_t *)c->k_new - (const uint8_t *)a.k_pool;
+                if (p.second ? apart_b : apart_a) from += p.v ? (const uint8_t *)c->v_new - (const uint8_t *)a.v_pool : (const uint8_t *)c->k_new - (const uint8_t *)a.k_pool;
             }
             return from;
         };
         if constexpr (P >= 128) {
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const bool is_new = t & 1 ? new_b : new_a;
-                const uint16_t *pool = t >= 2 ? (is_new ? c->v_new : a.v_pool) : (is_new ? c->k_new : a.k_pool);
+                const bool apart = t & 1 ? apart_b : apart_a;
+                const uint16_t *pool = t >= 2 ? (apart ? c->v_new : a.v_pool) : (apart ? c->k_new : a.k_pool);
                 const uint8_t *from = reinterpret_cast<const uint8_t *>(pool) + codes_at + (uint64_t)(t & 1 ? pb : pa) * page_bytes;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) MQ ? copy_to_lds(from, (uint32_t)lane * 16, to + t * 8 * P, b) : copy_to_lds_once(from, (uint32_t)lane * 16, to + t * 8 * P, b);

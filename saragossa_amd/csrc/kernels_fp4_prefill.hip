@@ -103,13 +103,13 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
 
     // ---- what a step brings: V of its pages, K of the pages a group further (K runs a group ahead). ids: physical pages from the step's first on, one a lane
     int ids;
-    auto ask_ids = [&](int it) __attribute__((always_inline)) { ids = (int)entry_place<RING>(a, c, entry(it + lane)); };
+    auto ask_ids = [&](int it) __attribute__((always_inline)) { ids = RING ? fp4_ring_page(a, c, entry(it + lane)) : (int)entry_place<false>(a, c, entry(it + lane)); };
     const uint32_t page_bytes = (uint32_t)g.page_elems * 2;
     const size_t codes_at = (size_t)kvh * fp4_code_bytes(P), powers_at = (size_t)g.kv_heads * fp4_code_bytes(P) + (size_t)kvh * fp4_power_bytes(P);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     auto pool_of = [&](int it, bool v) __attribute__((always_inline)) {
-        const bool is_new = RING && entry(it) >= c.n_old;
-        return reinterpret_cast<const uint8_t *>(v ? (is_new ? c.v_new : a.v_pool) : (is_new ? c.k_new : a.k_pool));
+        const bool apart = RING && fp4_in_scratch(c, entry(it));
+        return reinterpret_cast<const uint8_t *>(v ? (apart ? c.v_new : a.v_pool) : (apart ? c.k_new : a.k_pool));
     };
     // K of the pages it0 + d0 .. (as many as `pages`), whose physical pages lie in lanes d0 .. of ids, to buffer `buf`
     auto copy_k = [&](int it0, int d0, auto how_many, int buf) __attribute__((always_inline)) {

@@ -120,6 +120,8 @@ struct AppendArgs {
     int first_page; // logical page of the first row, of a ring the one it has come round to
     int first_row;  // of that page
     int ring_pages; // 0 = not a ring
+    uint16_t *k_save; // 4-bit layers: where the pages that the rows go into are copied to as they were, in order (null = nowhere)
+    uint16_t *v_save;
     Geom g;
 };
 
@@ -198,6 +200,11 @@ struct ChunkPages {
     int new_first;       // position of the first new page's first row
     const uint16_t *k_new; // tiles of the new pages, in order (null: their rows lie in the caller's memory, TermPairs)
     const uint16_t *v_new;
+    // 4-bit layers: entries [apart_lo, apart_hi) are pages apart_id + e of k_new, v_new, new ones that are not are table[new_start + e - n_old]
+    int apart_lo;
+    int apart_hi;
+    int apart_id;
+    int new_start;
 };
 
 // Pages of a chunk's list as three bf16 terms a value (f32 layers): pairs [first, first + held) of entries (2i, 2i + 1), per kv head
