@@ -43,20 +43,32 @@ def attention(q, keys, values, dims, first=None, window=0, window_start=0, attn_
     first = len(k) - n if first is None else first
     out, tol = np.empty(q.shape), np.empty(q.shape)
     scale = 1.0 / np.sqrt(attn_scalar or hd)
-    for i in range(n):
-        lo, hi = max(window_start, first + i + 1 - window if window else 0), first + i + 1
-        for h in range(q_heads):
-            kk, vv = k[lo:hi, h * kv_heads // q_heads], v[lo:hi, h * kv_heads // q_heads]
-            x = q[i, h].astype(np.float64) * scale
-            s = kk @ x
-            p = np.exp(s - s.max())
-            p /= p.sum()
-            out[i, h] = p @ vv
-            tol[i, h] = _bound(x, kk, s) * (p @ np.abs(vv)) + 1e-37
+    pos = first + np.arange(n)
+    at = np.arange(len(k))
+    # rows of queries at a time; one where there are NaN, which are not to reach the rows in front of them
+    block = 64 if np.isfinite(k).all() and np.isfinite(v).all() else 1
+    for kh in range(kv_heads):
+        heads = range(kh * q_heads // kv_heads, (kh + 1) * q_heads // kv_heads)
+        for i0 in range(0, n, block):
+            rows = slice(i0, min(i0 + block, n))
+            lo = max(window_start, pos[i0] + 1 - window if window else 0)
+            hi = pos[rows][-1] + 1
+            kk, vv = k[lo:hi, kh], v[lo:hi, kh]
+            seen = (at[None, lo:hi] <= pos[rows, None]) & (at[None, lo:hi] >= window_start)
+            if window:
+                seen &= at[None, lo:hi] > pos[rows, None] - window
+            for h in heads:
+                x = q[rows, h].astype(np.float64) * scale
+                s = x @ kk.T
+                m = np.where(seen, s, -np.inf).max(-1, keepdims=True)
+                p = np.where(seen, np.exp(np.where(seen, s, m) - m), 0.0)
+                p /= p.sum(-1, keepdims=True)
+                out[rows, h] = p @ vv
+                tol[rows, h] = _bound(x, kk, s, seen)[:, None] * (p @ np.abs(vv)) + 1e-37
     return out.reshape(n, -1), tol.reshape(n, -1)
 
 
-def _bound(x, k, s):
+def _bound(x, k, s, seen):
     """Relative to the weighted mean of |v|, how far a context may be off.
 
     A query value is four terms, the last of which leaves 2^-17 of the first term's power at most, a power that is at least the
@@ -65,10 +77,9 @@ def _bound(x, k, s):
     are in the 2^-24 below). Sums of at most 16 products and roundings of the score: 8 halves of a step of 32 bits of the sum of
     magnitudes. A score off by d moves the weights by 2 d relative to their sum. The weights are two terms of 16 bits, off by 2^-18, the
     exponential by 2^-22, sums of up to some thousand keys in partials of a few dozen: 2^-20 together."""
-    hd = len(x)
-    var = 0.0
-    for d in range(0, hd, GROUP):
-        step = np.abs(x[d:d + GROUP]).max() * 2.0 ** -18.9
-        var = var + step ** 2 / 3.0 * (k[:, d:d + GROUP] ** 2).sum(-1)
-    ds = 6.0 * np.sqrt(var) + (np.abs(k) @ np.abs(x) + np.abs(s)) * 8 * 2.0 ** -24
-    return 2.0 * ds.max() + 2.0 ** -18 + 2.0 ** -20
+    var = np.zeros(s.shape)
+    for d in range(0, x.shape[1], GROUP):
+        step = np.abs(x[:, d:d + GROUP]).max(-1) * 2.0 ** -18.9
+        var += step[:, None] ** 2 / 3.0 * (k[:, d:d + GROUP] ** 2).sum(-1)[None]
+    ds = 6.0 * np.sqrt(var) + (np.abs(x) @ np.abs(k).T + np.abs(s)) * 8 * 2.0 ** -24
+    return 2.0 * np.where(seen, ds, 0.0).max(-1) + 2.0 ** -18 + 2.0 ** -20
