@@ -48,9 +48,10 @@ __device__ __forceinline__ const uint8_t *fp4_powers(const uint16_t *pool, const
     return reinterpret_cast<const uint8_t *>(pool) + page * g.page_elems * 2 + g.kv_heads * fp4_code_bytes(g.P) + kvh * fp4_power_bytes(g.P);
 }
 // A group's byte from the bits of its largest magnitude (as integers, NaN and infinities above all numbers): the exponent, one more where the
-// leading bits pass 1.75, less two.
+// leading bits pass 1.75, less two. A group of zeros has the power 1.
 __device__ __forceinline__ uint32_t fp4_power_of(uint32_t top) {
     if (top >= 0x7f800000u) return 255u;
+    if (top == 0) return 127u;
     const int e = (int)((top + 0x1fffffu) >> 23) - 2;
     return (uint32_t)min(max(e, 2), 252);
 }
@@ -108,6 +109,25 @@ __device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
 template <int B>
 __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(power), B));
+}
+
+// V as f16, at 2^-8 of its value, against probabilities at 2^8 of theirs: exact for powers of 2^-15 to 2^16 (codes are multiples of 1/2 up to 6, f16's
+// steps 2^-24, its largest 65504), and two f16 terms hold a probability to 2^-22 of itself, or 2^-33, where two bf16 terms hold 2^-18.
+// Four rows' powers, those above and below it at 255 or below 112: bits in `far`.
+constexpr int V_SHIFT = 8;
+constexpr float P_SCALE = 1.0f / 256.0f; // of the sums of probabilities
+__device__ __forceinline__ uint32_t fp4_far(uint32_t powers) { return ((powers + 0x10101010u) ^ 0x80808080u) & 0xe0e0e0e0u; } // (bytes 112 to 143 have none)
+template <int B>
+__device__ __forceinline__ uint32_t code_pair_f16(uint32_t codes, uint32_t power) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, __uint_as_float(power), B));
+}
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+// x and y as two terms
+__device__ __forceinline__ void f16_terms(float x, float y, uint32_t &hi, uint32_t &lo) {
+    typedef __attribute__((ext_vector_type(2))) float f2;
+    const f16x2_t h = __builtin_convertvector(f2{x, y}, f16x2_t);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x - (float)h[0], y - (float)h[1]}, f16x2_t));
 }
 
 #endif

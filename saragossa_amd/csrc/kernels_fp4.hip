@@ -8,6 +8,7 @@ namespace skv {
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(4))) float float4_t;
 typedef __attribute__((ext_vector_type(16))) float float16_t;
 typedef __attribute__((ext_vector_type(2))) uint32_t u2;
@@ -255,11 +256,11 @@ template <int P>
 struct Fp4Tile {
     static constexpr int G = P / 32, U = fp4_quad(P), NB = (P + 127) / 128, VL = G / U;
 };
-// LDS in bytes: the queries' terms ([NB][4 terms][64 lanes][6 words]) and powers ([NB][64]); of the new rows, per row, K codes, V codes, K
+// LDS in bytes: the queries' terms ([NB][5 terms][64 lanes][6 words]) and powers ([NB][64]); of the new rows, per row, K codes, V codes, K
 // powers, V powers; then per wavefront DEPTH pairs of pages, and in their place, when all are consumed, its state.
 template <int P, int WAVES>
 struct Fp4Lds {
-    static constexpr int NB = Fp4Tile<P>::NB, BLOCK = (4 * 6 + 1) * 64 * 4;
+    static constexpr int NB = Fp4Tile<P>::NB, BLOCK = (5 * 6 + 1) * 64 * 4;
     static constexpr int DEPTH = 2;
     static constexpr int PAIR = 34 * P; // codes of K a, K b, V a, V b, then their powers
     static constexpr int STATE = 16 * (P + 6) * 4; // [16 slots][P + 4], m, l
@@ -518,7 +519,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         }
     };
     auto no_query = [&](int slot, int t) __attribute__((always_inline)) { // (nothing reads what becomes of it)
-        reinterpret_cast<uint32_t *>(lds + L::block(t >> 2, n_new))[4 * 6 * 64 + (t & 3) * 16 + slot] = 0;
+        reinterpret_cast<uint32_t *>(lds + L::block(t >> 2, n_new))[5 * 6 * 64 + (t & 3) * 16 + slot] = 0;
     };
     // an eighth of a group of a slot's queries, to its place among the terms
     auto query_eighth = [&](int slot, int t, int o8, float4_t y) __attribute__((always_inline)) {
@@ -528,25 +529,25 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = __uint_as_float(max(__float_as_uint(top), magnitude(y[e])));
         const uint32_t most = max_of_8(magnitude(top * a.qscale));
-        // the values as whole numbers X of 20 bits, |X| <= 2^19, in digits of base 32 between -16 and 15 (the first: 16). A float at
-        // 1.5 * 2^23 + (X + 16 (1 + 32 + 1024)) holds them in its last bits, 16 too large but for the first.
-        const int power = max((int)(most >> 23), 18);
-        const float scale = a.qscale * __uint_as_float((uint32_t)(272 - power) << 23);
+        // the values as whole numbers of 25 bits, at most 2^24 (a float's own bits), in digits of base 32 between -16 and 15 (the first: 16), here
+        // each 16 too large
+        const int power = max((int)(most >> 23), 23);
+        const float scale = a.qscale * __uint_as_float((uint32_t)(277 - power) << 23);
         uint32_t digits[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) digits[e] = __float_as_uint(__builtin_fmaf(y[e], scale, 12582912.0f + 16912.0f));
+        for (int e = 0; e < 4; ++e) digits[e] = (uint32_t)((int)__builtin_rintf(y[e] * scale) + 16 * (1 + 32 + 1024 + 32768 + 1048576));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 5; ++k) {
             uint32_t four = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) four |= (k == 0 ? (digits[e] >> 15 & 255u) - 112u : digits[e] >> (15 - 5 * k) & 31u) << (8 * e);
+            for (int e = 0; e < 4; ++e) four |= (k == 0 ? digits[e] >> 20 & 63u : digits[e] >> (20 - 5 * k) & 31u) << (8 * e);
             const uint32_t codes = fp6_codes_of(four); // 24 bits; four lanes' are three words
             const uint32_t next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)codes, 0xf9, 0xf, 0xf, false); // of the lane after
             const int o4 = o8 & 3;
             if (o4 < 3) to[(k * 64 + at) * 6 + (o8 >> 2) * 3 + o4] = codes >> (8 * o4) | next << (24 - 8 * o4);
         }
         if (o8 == 0)
-            to[4 * 6 * 64 + at] = most >= 0x7f800000u ? 0xffffffffu : (uint32_t)(power | (power - 5) << 8 | (power - 10) << 16) | (uint32_t)(power - 15) << 24;
+            to[5 * 6 * 64 + at] = most >= 0x7f800000u ? 0xffffffffu : (uint32_t)(power | (power - 5) << 8 | (power - 10) << 16) | (uint32_t)(power - 15) << 24;
     };
     if constexpr (PRE) {
         float *const pre_lds = reinterpret_cast<float *>(lds + L::pairs(n_new) + WAVES * L::PAIR);
@@ -586,14 +587,15 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     if constexpr (NEW && !ROWS) {
         if (converts) convert_rows(); // uniform (for itself)
     }
-    int8v_t q_term[NB][4];
-    uint32_t q_power[NB];
+    int8v_t q_term[NB][5];
+    uint32_t q_power[NB], q_last[NB]; // a byte each for the first four terms, the last one's
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const uint32_t *terms = reinterpret_cast<const uint32_t *>(lds + L::block(b, n_new));
-        q_power[b] = G >= 4 || j < G ? terms[4 * 6 * 64 + lane] : 0;
+        q_power[b] = G >= 4 || j < G ? terms[5 * 6 * 64 + lane] : 0;
+        q_last[b] = q_power[b] == 0xffffffffu ? 255u : (uint32_t)max((int)(q_power[b] & 255u) - 20, 0);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 5; ++t) {
 #pragma unroll
             for (int w = 0; w < 6; ++w) q_term[b][t][w] = G >= 4 || j < G ? (int)terms[(t * 64 + lane) * 6 + w] : 0;
             q_term[b][t][6] = q_term[b][t][7] = 0;
@@ -635,17 +637,44 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             if constexpr (NB == 1) kp[h] = pp[jk * 16 + n];
             else if constexpr (NB == 2) kp[h] = reinterpret_cast<const uint16_t *>(pp)[j * 16 + n];
             else kp[h] = reinterpret_cast<const uint32_t *>(pp)[j * 16 + n];
-#pragma unroll
-            for (int v = 0; v < VL; ++v) {
-                uint32_t w[U];
-                load_words<U>(w, pair + (2 + h) * 8 * P + (v * 64 + lane) * U * 4);
-#pragma unroll
-                for (int u = 0; u < U; ++u) vc[h][v * U + u] = w[u];
-            }
-            load_words<G>(vp[h], pair + 33 * P + h * (P / 2) + j * G * 4);
         }
-        if constexpr (NEW) { // the new rows' codes, from LDS
-            if (appends && e0 + 1 >= e_new && e0 <= e_last) { // uniform
+        const bool patches = NEW && appends && e0 + 1 >= e_new && e0 <= e_last; // uniform: the new rows' codes, from LDS
+        auto take_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int v = 0; v < VL; ++v) {
+                    uint32_t w[U];
+                    load_words<U>(w, pair + (2 + h) * 8 * P + (v * 64 + lane) * U * 4);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) vc[h][v * U + u] = w[u];
+                }
+                load_words<G>(vp[h], pair + 33 * P + h * (P / 2) + j * G * 4);
+            }
+            if constexpr (NEW) {
+                if (patches) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int from = entry_pos(e0 + h) - p_new;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int vrow = from + j * 4 + i;
+                            if (vrow < 0 || vrow >= C) continue;
+                            const uint8_t *to = new_rows + vrow * NEW_ROW;
+                            const uint32_t keep = ~(255u << (8 * i));
+#pragma unroll
+                            for (int t = 0; t < G; ++t) {
+                                vc[h][t] = (vc[h][t] & keep) | (uint32_t)to[AT_V + t * 16 + n] << (8 * i);
+                                vp[h][t] = (vp[h][t] & keep) | (uint32_t)to[AT_VP + t] << (8 * i);
+                            }
+                        }
+                    }
+                }
+            }
+        };
+        if constexpr (P <= 128) take_v();
+        if constexpr (NEW) {
+            if (patches) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int from = entry_pos(e0 + h) - p_new, row = from + n;
@@ -661,18 +690,6 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                         }
                         kp[h] = powers;
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int vrow = from + j * 4 + i;
-                        if (vrow < 0 || vrow >= C) continue;
-                        const uint8_t *to = new_rows + vrow * NEW_ROW;
-                        const uint32_t keep = ~(255u << (8 * i));
-#pragma unroll
-                        for (int t = 0; t < G; ++t) {
-                            vc[h][t] = (vc[h][t] & keep) | (uint32_t)to[AT_V + t * 16 + n] << (8 * i);
-                            vp[h][t] = (vp[h][t] & keep) | (uint32_t)to[AT_VP + t] << (8 * i);
-                        }
-                    }
                 }
             }
         }
@@ -685,13 +702,19 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             for (int b = 0; b < NB; ++b) {
                 const int8v_t k = {(int)kc[h][b][0], (int)kc[h][b][1], (int)kc[h][b][2], (int)kc[h][b][3], 0, 0, 0, 0};
                 const int kpow = (int)(kp[h] >> (8 * b));
+                s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][4], s[h], 4, 2, 0, kpow, 0, (int)q_last[b]);
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][3], s[h], 4, 2, 0, kpow, 3, (int)q_power[b]);
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][2], s[h], 4, 2, 0, kpow, 2, (int)q_power[b]);
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][1], s[h], 4, 2, 0, kpow, 1, (int)q_power[b]);
                 s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q_term[b][0], s[h], 4, 2, 0, kpow, 0, (int)q_power[b]);
             }
         }
-        if constexpr (P <= 128) next_pair(it + L::DEPTH);
+        if constexpr (P <= 128) {
+            next_pair(it + L::DEPTH);
+        } else { // (no registers for V beside K)
+            __builtin_amdgcn_sched_barrier(0);
+            take_v();
+        }
         // ---- softmax in base 2; keys outside the slot's range get no weight, and where no slot of the workgroup attends them (rows past the
         // length, before the window, of a page that is not there) V's powers are cleared as well: 0 x NaN is NaN
         const int lo_b = RING ? (e0 + 1 >= n_old ? c->new_pos0 : INT32_MIN) : INT32_MIN;
@@ -713,7 +736,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                     if (here && pos >= ws_lo && pos <= lim_hi) keep |= 255u << (8 * i);
                 }
 #pragma unroll
-                for (int t = 0; t < G; ++t) vp[h][t] &= keep;
+                for (int t = 0; t < G; ++t) vp[h][t] = (vp[h][t] & keep) | (~keep & 0x7f7f7f7fu);
                 if constexpr (MQ) { // a row that is NaN, attended by some slots and not by others: theirs alone
 #pragma unroll
                     for (int t = 0; t < G; ++t) {
@@ -722,7 +745,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                             const float x = rows_max((nan & seen) != 0 ? 1.0f : 0.0f) > 0.0f ? NAN : 0.0f;
                             o[2 * t] += x;
                             o[2 * t + 1] += x;
-                            vp[h][t] &= ~nan;
+                            vp[h][t] ^= nan & 0x80808080u;
                         }
                     }
                 }
@@ -732,15 +755,11 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         m_blk = rows_max(m_blk);
         const float m_new = fmaxf(m_run, m_blk), m_safe = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = fast_exp2(m_run - m_safe);
-        uint32_t hi[4], lo[4];
-        float psum = 0.0f;
+        float pr[8], psum = 0.0f; // times 2^8
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = fast_exp2(s[i >> 1][2 * (i & 1)] - m_safe), y = fast_exp2(s[i >> 1][2 * (i & 1) + 1] - m_safe);
-            psum += x + y;
-            typedef __attribute__((ext_vector_type(2))) float f2;
-            hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf16x2_t));
-            lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u)}, bf16x2_t));
+        for (int i = 0; i < 8; ++i) {
+            pr[i] = fast_exp2(s[i >> 2][i & 3] - (m_safe - V_SHIFT));
+            psum += pr[i];
         }
         l_run = l_run * alpha + psum;
         const bool rescale = alpha != 1.0f && m_run != -INFINITY; // (a slot without a key so far holds zeros)
@@ -749,29 +768,65 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= alpha;
         }
-        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u4{hi[0], hi[1], hi[2], hi[3]}), pl = __builtin_bit_cast(bf16x8_t, u4{lo[0], lo[1], lo[2], lo[3]});
         // ---- O^T += V^T . P^T
+        uint32_t hi[4], lo[4], far = 0;
 #pragma unroll
-        for (int t = 0; t < G; ++t) {
-            u4 first, second; // dims 32 t + n and 32 t + 16 + n of the 32 keys
+        for (int t = 0; t < G; ++t) far |= fp4_far(vp[0][t]) | fp4_far(vp[1][t]);
+        // dims 32 t + n and 32 t + 16 + n of the 32 keys, from the pairs that c0 .. c3 hold of each page
+        auto products = [&](int t, auto of_page, auto mfma) __attribute__((always_inline)) {
+            u4 first, second;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t w = vc[h][t], e = vp[h][t];
-                const uint32_t c0 = code_pair<0>(w, e << 23), c1 = code_pair<1>(w, e << 15), c2 = code_pair<2>(w, e << 7), c3 = code_pair<3>(w, e >> 1);
-                first[2 * h] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);
-                first[2 * h + 1] = __builtin_amdgcn_perm(c3, c2, 0x05040100u);
-                second[2 * h] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);
-                second[2 * h + 1] = __builtin_amdgcn_perm(c3, c2, 0x07060302u);
+                const u4 c = of_page(vc[h][t], vp[h][t]);
+                first[2 * h] = __builtin_amdgcn_perm(c[1], c[0], 0x05040100u);
+                first[2 * h + 1] = __builtin_amdgcn_perm(c[3], c[2], 0x05040100u);
+                second[2 * h] = __builtin_amdgcn_perm(c[1], c[0], 0x07060302u);
+                second[2 * h + 1] = __builtin_amdgcn_perm(c[3], c[2], 0x07060302u);
             }
-            const bf16x8_t va = __builtin_bit_cast(bf16x8_t, first), vb = __builtin_bit_cast(bf16x8_t, second);
-            o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pl, o[2 * t], 0, 0, 0);
-            o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pl, o[2 * t + 1], 0, 0, 0);
-            o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * t], 0, 0, 0);
-            o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * t + 1], 0, 0, 0);
+            o[2 * t] = mfma(first, lo, o[2 * t]);
+            o[2 * t + 1] = mfma(second, lo, o[2 * t + 1]);
+            o[2 * t] = mfma(first, hi, o[2 * t]);
+            o[2 * t + 1] = mfma(second, hi, o[2 * t + 1]);
+        };
+        if (__builtin_amdgcn_ballot_w64(far != 0)) { // uniform: powers that f16 does not have, or NaN
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                typedef __attribute__((ext_vector_type(2))) float f2;
+                const float x = pr[2 * i] * P_SCALE, y = pr[2 * i + 1] * P_SCALE;
+                hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf16x2_t));
+                lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u)}, bf16x2_t));
+            }
+#pragma unroll
+            for (int t = 0; t < G; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                products(
+                    t, [](uint32_t w, uint32_t e) __attribute__((always_inline)) { return u4{code_pair<0>(w, e << 23), code_pair<1>(w, e << 15), code_pair<2>(w, e << 7), code_pair<3>(w, e >> 1)}; },
+                    [](u4 v, const uint32_t(&x)[4], float4_t to) __attribute__((always_inline)) {
+                        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, u4{x[0], x[1], x[2], x[3]}), to, 0, 0, 0);
+                    });
+                vc[0][t] = vc[1][t] = 0; // (f16's products then add zeros: with a path of their own, o would be in two places)
+                vp[0][t] = vp[1][t] = 0x7f7f7f7fu;
+            }
+        }
+        {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f16_terms(pr[2 * i], pr[2 * i + 1], hi[i], lo[i]);
+#pragma unroll
+            for (int t = 0; t < G; ++t) {
+                __builtin_amdgcn_sched_barrier(0); // (a group's conversions behind the products of the one in front of it: registers)
+                products(
+                    t, [](uint32_t w, uint32_t e) __attribute__((always_inline)) {
+                        e -= 0x01010101u * V_SHIFT;
+                        return u4{code_pair_f16<0>(w, e << 23), code_pair_f16<1>(w, e << 15), code_pair_f16<2>(w, e << 7), code_pair_f16<3>(w, e >> 1)};
+                    },
+                    [](u4 v, const uint32_t(&x)[4], float4_t to) __attribute__((always_inline)) {
+                        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, v), __builtin_bit_cast(f16x8_t, u4{x[0], x[1], x[2], x[3]}), to, 0, 0, 0);
+                    });
+            }
         }
         if constexpr (P > 128) next_pair(it + L::DEPTH);
     }
-    l_run = rows_sum(l_run);
+    l_run = rows_sum(l_run) * P_SCALE;
     if constexpr (PRE) __syncthreads(); // (a state lies over other wavefronts' pairs)
 
     // ---- the wavefronts' states meet in LDS, four columns a thread

@@ -9,6 +9,7 @@ namespace skv {
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) float float2v_t;
 typedef __attribute__((ext_vector_type(4))) float float4_t;
 typedef __attribute__((ext_vector_type(16))) float float16_t;
@@ -65,8 +66,9 @@ struct Fp4Chunk {
     static constexpr int K_PAGE = 8 * P, K_POWERS = P / 2, K_BUF = PAGES * (K_PAGE + K_POWERS), V_PAGE = 32 * P, V_BUF = PAGES * V_PAGE;
     static constexpr int V_AT = 2 * K_BUF, NAN_AT = V_AT + 2 * V_BUF;
     // of the rows that are NaN: per buffer the step that has some; per (page, part) the step, and per row a bit a group
-    static constexpr int NAN_WORDS = 2 * (1 + PAGES * PARTS * 17);
-    static constexpr size_t LDS = NAN_AT + (NAN_WORDS * 4 + 15) / 16 * 16;
+    // of the powers that f16 does not have: per buffer the step that has some, and per (page, part)
+    static constexpr int NAN_WORDS = 2 * (1 + PAGES * PARTS * 17), FAR_WORDS = 2 * (1 + PAGES * PARTS);
+    static constexpr size_t LDS = NAN_AT + ((NAN_WORDS + FAR_WORDS) * 4 + 15) / 16 * 16;
     static_assert(SP >= 1 && PARTS >= 1 && G % PARTS == 0, "steps of whole groups, whole groups of dims to a wavefront");
     static_assert(LDS <= 160 * 1024, "it fits a compute unit's LDS");
     static constexpr int ROW = P < 128 ? P / 4 : 32; // units of four dims of a block of a query row
@@ -158,6 +160,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         load_words<GW>(vs, at + powers_at + (j * G + vp * GW) * 4);
     };
     uint32_t *const nan_step = reinterpret_cast<uint32_t *>(lds + L::NAN_AT), *const nan_of = nan_step + 2; // [2], [2][PAGES * PARTS][1 + 16]
+    uint32_t *const far_step = nan_step + L::NAN_WORDS, *const far_of = far_step + 2; // [2], [2][PAGES * PARTS]
     const Inner wg_in = inner_entries<RING>(c, pb0, pb1, wg_ws_lo, wg_lim_hi);
     // V of step `step`, loaded, to buffer step & 1: per (pair, group of dims, dims n or n + 16) a KiB, a lane's 4 keys of page a, then of b
     auto convert_v = [&](int step) __attribute__((always_inline)) {
@@ -170,29 +173,42 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
             for (int i = 0; i < 4; ++i)
                 if (it < n_it && pos + i >= lo && pos + i <= hi) keep |= 255u << (8 * i);
 #pragma unroll
-            for (int t = 0; t < GW; ++t) vs[t] &= keep;
+            for (int t = 0; t < GW; ++t) vs[t] = (vs[t] & keep) | (~keep & 0x7f7f7f7fu);
         }
         uint32_t any = 0;
 #pragma unroll
-        for (int t = 0; t < GW; ++t) any |= bytes_255(vs[t]);
-        if (__builtin_amdgcn_ballot_w64(any != 0)) { // rows that are NaN
-            uint32_t *of = nan_of + ((step & 1) * PAGES * PARTS + wave) * 17;
-            if (lane == 0) nan_step[step & 1] = of[0] = (uint32_t)step + 1;
+        for (int t = 0; t < GW; ++t) any |= fp4_far(vs[t]);
+        if (__builtin_amdgcn_ballot_w64(any != 0)) { // uniform: NaN, or powers that f16 does not have
+            any = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t bits = 0;
+            for (int t = 0; t < GW; ++t) any |= bytes_255(vs[t]);
+            if (__builtin_amdgcn_ballot_w64(any != 0)) { // rows that are NaN
+                uint32_t *of = nan_of + ((step & 1) * PAGES * PARTS + wave) * 17;
+                if (lane == 0) nan_step[step & 1] = of[0] = (uint32_t)step + 1;
 #pragma unroll
-                for (int t = 0; t < GW; ++t) bits |= (bytes_255(vs[t]) >> (8 * i) & 1u) << (vp * GW + t);
-                if (n == 0) of[1 + j * 4 + i] = bits;
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int t = 0; t < GW; ++t) bits |= (bytes_255(vs[t]) >> (8 * i) & 1u) << (vp * GW + t);
+                    if (n == 0) of[1 + j * 4 + i] = bits;
+                }
+#pragma unroll
+                for (int t = 0; t < GW; ++t) vs[t] ^= bytes_255(vs[t]) & 0x80808080u;
             }
+            any = 0;
 #pragma unroll
-            for (int t = 0; t < GW; ++t) vs[t] &= ~bytes_255(vs[t]);
+            for (int t = 0; t < GW; ++t) any |= fp4_far(vs[t]);
+            if (__builtin_amdgcn_ballot_w64(any != 0)) { // uniform: far_pages takes all of it, from memory
+                if (lane == 0) far_step[step & 1] = far_of[(step & 1) * PAGES * PARTS + wave] = (uint32_t)step + 1;
+#pragma unroll
+                for (int t = 0; t < GW; ++t) vc[t] = 0, vs[t] = 0x7f7f7f7fu;
+            }
         }
         uint8_t *to = lds + L::V_AT + (step & 1) * L::V_BUF + (vd >> 1) * 2 * L::V_PAGE + lane * 16 + (vd & 1) * 8;
 #pragma unroll
         for (int t = 0; t < GW; ++t) {
-            const uint32_t w = vc[t], e4 = vs[t];
-            const uint32_t c0 = code_pair<0>(w, e4 << 23), c1 = code_pair<1>(w, e4 << 15), c2 = code_pair<2>(w, e4 << 7), c3 = code_pair<3>(w, e4 >> 1);
+            const uint32_t w = vc[t], e4 = vs[t] - 0x01010101u * V_SHIFT;
+            const uint32_t c0 = code_pair_f16<0>(w, e4 << 23), c1 = code_pair_f16<1>(w, e4 << 15), c2 = code_pair_f16<2>(w, e4 << 7), c3 = code_pair_f16<3>(w, e4 >> 1);
             uint8_t *at = to + (vp * GW + t) * 2048;
             *reinterpret_cast<u2 *>(at) = u2{__builtin_amdgcn_perm(c1, c0, 0x05040100u), __builtin_amdgcn_perm(c3, c2, 0x05040100u)};
             *reinterpret_cast<u2 *>(at + 1024) = u2{__builtin_amdgcn_perm(c1, c0, 0x07060302u), __builtin_amdgcn_perm(c3, c2, 0x07060302u)};
@@ -201,14 +217,14 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     // everything asked for with an ordinary load has arrived (the compiler does not know of the copies: see copy_to_lds)
     auto ids_here = [&]() __attribute__((always_inline)) { asm volatile("" : "+v"(ids)); };
     ask_ids(0);
-    if (tid < 2) nan_step[tid] = 0;
-    if (tid < 2 * PAGES * PARTS) nan_of[tid * 17] = 0; // (LDS holds what the launch before left)
+    if (tid < 2) nan_step[tid] = far_step[tid] = 0;
+    if (tid < 2 * PAGES * PARTS) nan_of[tid * 17] = far_of[tid] = 0; // (LDS holds what the launch before left)
 
     // ---- this wavefront's query tiles: rows side by side through LDS (V's buffers), a lane (slot n, group j) then has its 32 dims
     int my_limit[TILES], my_ws[TILES], t_ws_hi[TILES], t_lim_lo[TILES];
     bool t_on[TILES];
-    int8v_t q_term[TILES][NB][4];
-    uint32_t q_power[TILES][NB];
+    int8v_t q_term[TILES][NB][5];
+    uint32_t q_power[TILES][NB], q_last[TILES][NB]; // a byte each for the first four terms, the last one's
     float4_t *const raw = reinterpret_cast<float4_t *>(lds + L::V_AT) + wave * 16 * L::ROW;
     constexpr int ROW = L::ROW, LANES = ROW == 24 ? 32 : ROW, AT_ONCE = 64 / LANES, QL = 16 / AT_ONCE; // lanes of a row, rows of an instruction
     const int unit = lane % LANES;
@@ -259,19 +275,20 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                     top = max(top, max(magnitude(even[2 * i + e]), magnitude(odd[2 * i + e])));
                 }
             }
-            // the first term's power is the smallest with the largest value <= 7.5 of it; a term leaves at most 2^-2, then 2^-7, 2^-12, 2^-17 of it, 2^-18.9
-            // of the largest value
-            const int power = max((int)((top + 0x0fffffu) >> 23) - 2, 18);
-            constexpr int down[4] = {0, 4, 9, 14};
+            // the first term's power is the smallest with the largest value <= 7.5 of it; a term leaves at most 2^-2, then 2^-7, 2^-12, 2^-17, 2^-22 of it,
+            // 2^-23.9 of the largest value
+            const int power = max((int)((top + 0x0fffffu) >> 23) - 2, 23);
+            constexpr int down[5] = {0, 4, 9, 14, 19};
+            q_last[t][b] = top >= 0x7f800000u ? 255u : (uint32_t)(power - 19);
             q_power[t][b] = top >= 0x7f800000u ? 0xffffffffu : (uint32_t)(power | (power - 4) << 8 | (power - 9) << 16) | (uint32_t)(power - 14) << 24;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 5; ++k) {
                 const float scale = __uint_as_float((uint32_t)(power - down[k]) << 23);
                 const u6 codes = to_fp6(even, odd, scale);
 #pragma unroll
                 for (int w = 0; w < 6; ++w) q_term[t][b][k][w] = (int)codes[w];
                 q_term[t][b][k][6] = q_term[t][b][k][7] = 0;
-                if (k < 3) {
+                if (k < 4) {
                     const float32_t back = from_fp6(codes, scale);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -290,7 +307,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     convert_v(0);
 
     float4_t o[TILES][NT], neg_m[TILES];
-    constexpr int UNSEEN = INT32_MIN, SEEN = 1; // a score whose bits reach thr moves the base: any above it, or, of a slot without a key so far, whatever it is
+    // a score whose bits reach thr moves the base: any more than 8 above it, or, of a slot without a key so far, whatever it is
+    constexpr int UNSEEN = INT32_MIN, SEEN = 0x41000001;
     float m_base[TILES], l_run[TILES];
     int thr[TILES];
 #pragma unroll
@@ -345,7 +363,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 const float mx = fmaxf(fmaxf(fmaxf(sa[t][0], sa[t][1]), fmaxf(sa[t][2], sa[t][3])), fmaxf(fmaxf(sb[t][0], sb[t][1]), fmaxf(sb[t][2], sb[t][3])));
                 const float top = rows_max(mx); // of the slot, relative to its base
                 const bool unseen = thr[t] < 0;
-                const float d = top > (unseen ? -INFINITY : 0.0f) ? top + 4.0f : 0.0f;
+                const float d = top > (unseen ? -INFINITY : 8.0f) ? top - 4.0f : 0.0f;
                 const float alpha = unseen ? 1.0f : fast_exp2(-d);
                 m_base[t] += d;
                 neg_m[t] = float4_t{-m_base[t], -m_base[t], -m_base[t], -m_base[t]};
@@ -375,9 +393,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 l_run[t] += prev[t];
                 pr[t][e & 1] = prev[t];
                 if (e & 1) {
-                    const uint32_t hi = bf16_pair(pr[t][0], pr[t][1]);
-                    hi4[t][e >> 1] = hi;
-                    lo4[t][e >> 1] = bf16_pair(pr[t][0] - __uint_as_float(hi << 16), pr[t][1] - __uint_as_float(hi & 0xffff0000u));
+                    f16_terms(pr[t][0], pr[t][1], hi4[t][e >> 1], lo4[t][e >> 1]);
                 }
             }
             if (q < 8) prev[t] = fast_exp2(q < 4 ? sa[t][q & 3] : sb[t][q & 3]);
@@ -411,23 +427,24 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int k = 3; k >= 0; --k) {
+            for (int k = 4; k >= 0; --k) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int8v_t kk = {(int)kc[h][b][0], (int)kc[h][b][1], (int)kc[h][b][2], (int)kc[h][b][3], 0, 0, 0, 0};
                     const int kpow = (int)(kp[h] >> (8 * b));
 #pragma unroll
                     for (int t = 0; t < TILES; ++t) {
-                        const float4_t from = b == 0 && k == 3 ? neg_m[t] : ns[h][t];
-                        ns[h][t] = k == 3   ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][3], from, 4, 2, 0, kpow, 3, (int)q_power[t][b])
+                        const float4_t from = b == 0 && k == 4 ? neg_m[t] : ns[h][t];
+                        ns[h][t] = k == 4   ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][4], from, 4, 2, 0, kpow, 0, (int)q_last[t][b])
+                                   : k == 3 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][3], from, 4, 2, 0, kpow, 3, (int)q_power[t][b])
                                    : k == 2 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][2], from, 4, 2, 0, kpow, 2, (int)q_power[t][b])
                                    : k == 1 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][1], from, 4, 2, 0, kpow, 1, (int)q_power[t][b])
                                             : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, q_term[t][b][0], from, 4, 2, 0, kpow, 0, (int)q_power[t][b]);
                     }
                 }
                 if (PROBS) {
-                    if (b == NB - 1) ask_v(vt, (3 - k) % AHEAD);
-                    const int until = ((b * 4 + 4 - k) * 9) / (4 * NB); // steps done by the end of this beat
+                    if (b == NB - 1 && k < 4) ask_v(vt, (3 - k) % AHEAD);
+                    const int until = ((b * 5 + 5 - k) * 9) / (5 * NB); // steps done by the end of this beat
 #pragma unroll
                     for (int s = 0; s < 9; ++s)
                         if (s >= q && s < until) prob_step(s);
@@ -444,22 +461,75 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
         }
     };
     auto accumulate = [&](const uint8_t *vt, auto next_k) __attribute__((always_inline)) {
-        bf16x8_t ph[TILES], pl[TILES];
+        f16x8_t ph[TILES], pl[TILES];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            ph[t] = __builtin_bit_cast(bf16x8_t, u4{hi4[t][0], hi4[t][1], hi4[t][2], hi4[t][3]});
-            pl[t] = __builtin_bit_cast(bf16x8_t, u4{lo4[t][0], lo4[t][1], lo4[t][2], lo4[t][3]});
+            ph[t] = __builtin_bit_cast(f16x8_t, u4{hi4[t][0], hi4[t][1], hi4[t][2], hi4[t][3]});
+            pl[t] = __builtin_bit_cast(f16x8_t, u4{lo4[t][0], lo4[t][1], lo4[t][2], lo4[t][3]});
         }
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, vr[u % AHEAD]);
+            const f16x8_t v = __builtin_bit_cast(f16x8_t, vr[u % AHEAD]);
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[t], o[t][u], 0, 0, 0);
+            for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t], o[t][u], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[t], o[t][u], 0, 0, 0);
+            for (int t = 0; t < TILES; ++t) o[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[t][u], 0, 0, 0);
             if (u + AHEAD < NT) ask_v(vt, u + AHEAD);
             else if (u + AHEAD == NT) next_k();
             __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // a pair's pages whose V has powers that f16 does not have (convert_v left zeros): as bf16, from memory
+    auto far_pages = [&](int step, int pp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int d = (pp * HALVES + half) * 2 + h, it = step * PAGES + d, e = entry(it);
+            uint32_t ph[TILES][2], pl[TILES][2];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f16x2_t a16 = __builtin_bit_cast(f16x2_t, hi4[t][2 * h + i]), b16 = __builtin_bit_cast(f16x2_t, lo4[t][2 * h + i]);
+                    const float x = ((float)a16[0] + (float)b16[0]) * P_SCALE, y = ((float)a16[1] + (float)b16[1]) * P_SCALE;
+                    ph[t][i] = bf16_pair(x, y);
+                    pl[t][i] = bf16_pair(x - __uint_as_float(ph[t][i] << 16), y - __uint_as_float(ph[t][i] & 0xffff0000u));
+                }
+            }
+            const int pos = entry_pos<RING>(c, e) + j * 4, lo = max(wg_ws_lo, entry_lo<RING>(c, e)), hi = min(wg_lim_hi, entry_hi<RING>(c, e));
+            uint32_t keep = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (it < n_it && pos + i >= lo && pos + i <= hi) keep |= 255u << (8 * i);
+            const uint8_t *at = pool_of(it, true) + (uint64_t)(uint32_t)(RING ? fp4_ring_page(a, c, e) : (int)entry_place<false>(a, c, e)) * page_bytes;
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                if (__builtin_amdgcn_readfirstlane((int)far_of[((step & 1) * PAGES + d) * PARTS + part]) != step + 1) continue;
+#pragma unroll
+                for (int g0 = 0; g0 < GW / U; ++g0) {
+                    uint32_t w[U];
+                    load_words<U>(w, at + codes_at + ((part * (GW / U) + g0) * 64 + lane) * U * 4);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int grp = part * GW + g0 * U + u;
+                        uint32_t e4 = *reinterpret_cast<const uint32_t *>(at + powers_at + (j * G + grp) * 4);
+                        const uint32_t none = ~keep | bytes_255(e4); // (NaN: see nan_rows)
+                        e4 = (e4 & ~none) | (none & 0x7f7f7f7fu);
+                        const uint32_t c0 = code_pair<0>(w[u], e4 << 23), c1 = code_pair<1>(w[u], e4 << 15), c2 = code_pair<2>(w[u], e4 << 7), c3 = code_pair<3>(w[u], e4 >> 1);
+                        // (the other page's keys are zeros)
+                        const u4 first = {__builtin_amdgcn_perm(c1, c0, 0x05040100u), __builtin_amdgcn_perm(c3, c2, 0x05040100u), 0, 0};
+                        const u4 second = {__builtin_amdgcn_perm(c1, c0, 0x07060302u), __builtin_amdgcn_perm(c3, c2, 0x07060302u), 0, 0};
+#pragma unroll
+                        for (int t = 0; t < TILES; ++t) {
+                            const bf16x8_t xh = __builtin_bit_cast(bf16x8_t, u4{ph[t][0], ph[t][1], 0, 0}), xl = __builtin_bit_cast(bf16x8_t, u4{pl[t][0], pl[t][1], 0, 0});
+                            o[t][2 * grp] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), xl, o[t][2 * grp], 0, 0, 0);
+                            o[t][2 * grp] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), xh, o[t][2 * grp], 0, 0, 0);
+                            o[t][2 * grp + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, second), xl, o[t][2 * grp + 1], 0, 0, 0);
+                            o[t][2 * grp + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, second), xh, o[t][2 * grp + 1], 0, 0, 0);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
         }
     };
     // the slots that attend rows that are NaN in the step's V: NaN in those groups of dims
@@ -497,6 +567,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
 
     for (int step = 0; step < n_steps; ++step) {
         const int buf = step & 1;
+        const bool far = __builtin_amdgcn_readfirstlane((int)far_step[buf]) == step + 1;
         if (step + 1 < n_steps) { // uniform
             ids_here();
             copy_k((step + 1) * PAGES, GP, std::integral_constant<int, PAGES>{}, buf ^ 1);
@@ -513,6 +584,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
             accumulate(vt, [&]() __attribute__((always_inline)) {
                 if (pp + 1 < SP) ask_k(buf, pp + 1);
             });
+            if (far) far_pages(step, pp); // uniform
             mask((group + 1) * HALVES + half);
             settle();
         }
@@ -567,7 +639,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     const bool vec_ok = (g.head_dim & 3) == 0 && (a.splits_total > 1 || (reinterpret_cast<uintptr_t>(a.out) & 15) == 0);
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-        const float l = rows_sum(l_run[t]);
+        const float l = rows_sum(l_run[t]) * P_SCALE;
         const int slot = wg_slot0 + (tw * TILES + t) * 16 + n;
         if (!t_on[t] || slot >= n_slots) continue;
         float *dst;

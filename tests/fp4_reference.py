@@ -62,24 +62,32 @@ def attention(q, keys, values, dims, first=None, window=0, window_start=0, attn_
                 s = x @ kk.T
                 m = np.where(seen, s, -np.inf).max(-1, keepdims=True)
                 p = np.where(seen, np.exp(np.where(seen, s, m) - m), 0.0)
-                p /= p.sum(-1, keepdims=True)
+                total = p.sum(-1, keepdims=True)
+                p /= total
                 out[rows, h] = p @ vv
-                tol[rows, h] = _bound(x, kk, s, seen)[:, None] * (p @ np.abs(vv)) + 1e-37
+                tol[rows, h] = _bound(x, kk, s, seen, vv)[:, None] * (p @ np.abs(vv)) + 2.0 ** -29 * (seen @ np.abs(vv)) / total + 1e-37
     return out.reshape(n, -1), tol.reshape(n, -1)
 
 
-def _bound(x, k, s, seen):
+def _bound(x, k, s, seen, v):
     """Relative to the weighted mean of |v|, how far a context may be off.
 
-    A query value is four terms, the last of which leaves 2^-17 of the first term's power at most, a power that is at least the
-    group's largest value over 7.5 and at most that over 3.75: 2^-18.9 of the largest value, one way or the other, so that dims are
+    A query value is five terms. The last of them leaves 2^-22 of the first term's power at most, a power that is at least the
+    group's largest value over 7.5 and at most that over 3.75: 2^-23.9 of the largest value, one way or the other, so that dims are
     off independently of each other and a score by six of its standard deviations at most (the times log2(e) and back of base 2
     are in the 2^-24 below). Sums of at most 16 products and roundings of the score: 8 halves of a step of 32 bits of the sum of
-    magnitudes. A score off by d moves the weights by 2 d relative to their sum. The weights are two terms of 16 bits, off by 2^-18, the
-    exponential by 2^-22, sums of up to some thousand keys in partials of a few dozen: 2^-20 together."""
+    magnitudes. A score off by d moves the weights by 2 d relative to their sum. The weights are two terms of f16, off by half a step of
+    half a step, 2^-22, or, where V has powers outside 2^-15 to 2^16 (largest values in 3.5 times the one to 7 times the other), of
+    bf16, 2^-18. The exponential is off by 2^-22, sums of up to some thousand keys in partials of a few dozen by 2^-20 together.
+
+    Beside that (`attention`): f16's steps end at 2^-24. A weight is held at 2^8 times itself, relative to a base that is at most 2^4
+    above the largest, so that it is off by half of such a step over 2^8, 2^-33, times 2^4: 2^-29 of the largest weight."""
+    top = np.stack([np.abs(v[:, d:d + GROUP]).max(-1) for d in range(0, v.shape[1], GROUP)])
+    top = top[top > 0]
+    far = top.size > 0 and (top.min() <= 3.5 * 2.0 ** -15 or top.max() > 6 * 2.0 ** 16)
     var = np.zeros(s.shape)
     for d in range(0, x.shape[1], GROUP):
-        step = np.abs(x[:, d:d + GROUP]).max(-1) * 2.0 ** -18.9
+        step = np.abs(x[:, d:d + GROUP]).max(-1) * 2.0 ** -23.9
         var += step[:, None] ** 2 / 3.0 * (k[:, d:d + GROUP] ** 2).sum(-1)[None]
     ds = 6.0 * np.sqrt(var) + (np.abs(x) @ np.abs(k).T + np.abs(s)) * 8 * 2.0 ** -24
-    return 2.0 * np.where(seen, ds, 0.0).max(-1) + 2.0 ** -18 + 2.0 ** -20
+    return 2.0 * np.where(seen, ds, 0.0).max(-1) + (2.0 ** -18 if far else 2.0 ** -22) + 2.0 ** -22 + 2.0 ** -20

@@ -132,6 +132,42 @@ def test_chunks_about_as_long_as_their_ring(state, chunk_kernel, dims, window, r
         p.check_rows(p.kv.len() - window)
 
 
+# ---- values of any size --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (12, 4, 96), (8, 2, 512), (5, 1, 33)], ids=str)
+@pytest.mark.parametrize("case", ["tiny", "huge", "some rows", "some groups", "zeros"])
+def test_values_whose_powers_half_precision_does_not_have(state, chunk_kernel, dims, case):
+    """V from 1e-30 to 1e30, whole caches of it, or rows and groups of dims among others; rows of zeros."""
+    p = Pair(state, dims, 700, seed=8)
+    fresh = p.new
+
+    def new(n):
+        k, v, q = fresh(n)
+        v = v.reshape(n, dims[1], dims[2])
+        if case == "tiny":
+            v *= np.float32(1e-12)
+        elif case == "huge":
+            v *= np.float32(1e30)
+        elif case == "some rows":
+            v[::7] *= np.float32(2.0 ** -18)
+            v[3::11] *= np.float32(2.0 ** 17)
+        elif case == "some groups":
+            v[::5, :, :32] *= np.float32(1e-30)
+            v[1::5, -1, -32:] *= np.float32(1e-6)
+        else:
+            v[::2] = 0
+            v[1::4, :, :32] = 0
+        return k, v.reshape(n, -1), q
+
+    p.new = new
+    p.append(333)
+    p.step()
+    for n in (5, 90, 70):
+        p.chunk(n)
+        p.step()
+    p.check_rows()
+
+
 # ---- graphs ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dims,window,base,rows", [((16, 2, 256), 0, 2000, 6), ((8, 2, 64), 0, 900, 130), ((32, 8, 128), 0, 2000, 128),
@@ -192,7 +228,7 @@ def test_captured_chunks_and_steps_replay_the_eager_result(dims, window, base, r
 
 def _apart(kv, first=0):
     """How far two launches over the same rows and queries may be from each other, split differently: they have the same scores, and each rounds
-    its weights by 2^-18 and its exponentials and sums by 2^-20 (fp4_reference.py), relative to the mean of |v|: at most the largest |v|."""
+    its weights by 2^-18 at most and its exponentials and sums by 2^-20 (fp4_reference.py), relative to the mean of |v|: at most the largest |v|."""
     return 2 * (2.0 ** -18 + 2.0 ** -20) * float(np.abs(kv.read_rows_f32(first)[1]).max())
 
 
