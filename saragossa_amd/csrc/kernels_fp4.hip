@@ -813,7 +813,6 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             for (int i = 0; i < 4; ++i) f16_terms(pr[2 * i], pr[2 * i + 1], hi[i], lo[i]);
 #pragma unroll
             for (int t = 0; t < G; ++t) {
-                __builtin_amdgcn_sched_barrier(0); // (a group's conversions behind the products of the one in front of it: registers)
                 products(
                     t, [](uint32_t w, uint32_t e) __attribute__((always_inline)) {
                         e -= 0x01010101u * V_SHIFT;
@@ -895,7 +894,8 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 }
 
 template <int P, int WAVES, bool MQ, bool RING, bool ROWS, bool PRE>
-__global__ __launch_bounds__(WAVES * 64) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
+// (streaming chunks of heads up to 128 dims: registers for two workgroups on a compute unit, with one 256 rows over 2000 of q32/kv8/hd128 32.9 us, 29.2 with two)
+__global__ __launch_bounds__(WAVES * 64, MQ && !ROWS && P <= 128 ? 4 : 1) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
     fp4_attention_body<P, WAVES, MQ, RING, ROWS, PRE>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
