@@ -322,23 +322,23 @@ bool takes_f32_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
 }
 // The same for layers of 4 bits: the streaming kernel or the one that shares pages and V's conversion among 64 to 256 slots. The streaming
 // one has no prologue to speak of and converts V anew for every 16 slots; the other's start is the queries' conversion (3 us at
-// head_dim 128, 5 at 256). From 193 workgroups of 64 slots on that needs neither splits nor a merge and is the faster one everywhere. Over 3510
+// head_dim 128, 5 at 256). From 193 workgroups of 64 slots on that needs neither splits nor a merge and is the faster one nearly everywhere. Over 2340
 // chunks of 4 to 1024 rows in nine geometries, on layers in no cache, kernel and shape chosen are 0.6 % slower than the best on the
-// average. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
-// 16.7/23.8, 256 (70) 25.7/31.5, 64 over 8000 (65) 28.5/28.2, 512 over 512 (49, 256 workgroups) 24.8/23.2; q16/kv2/hd256, 64 over 8192 (33)
-// 28.7/35.8, 128 (66) 43.6/47.6, q16/kv8/hd256, 256 over 8000 (131) 70.4/68.3; q8/kv2/hd512 loses in the mean from 16 on.
+// average, 30 % at most. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
+// 18.4/24.7, 256 (70) 29.0/32.1, 64 over 8000 (65) 31.4/29.2, 512 over 512 (49, 256 workgroups) 27.4/24.3; q16/kv2/hd256, 64 over 8192 (33)
+// 32.3/37.1, 128 (66) 49.8/49.5, q16/kv8/hd256, 256 over 8000 (131) 81.6/78.4; q8/kv2/hd512 loses in the mean from 16 on.
 bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
     const size_t n_slots = n_queries * (size_t)g.gqa;
     if (tuning().prefill_tiles != 1 || n_slots < 64) return tuning().prefill_tiles > 1 && n_slots >= 64;
     const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, tiles = (n_slots + 15) / 16 * (size_t)g.kv_heads;
     const size_t walked = n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1;
-    return wgs > 192 || tiles * walked >= (g.P > 256 ? 17000u : g.P > 128 ? 48000u : 70000u);
+    return wgs > 192 || tiles * walked >= (g.P > 256 ? 16000u : g.P > 128 ? 42000u : g.P > 64 ? 52000u : 70000u);
 }
 // Slots of a workgroup of that kernel: 64 (two wavefronts to a tile), 128, or 256 (heads to 128 dims). Wider ones convert a page of V for
 // more slots, narrower ones fill the device sooner, and where the causal triangle is most of the work (`own`) they also share it out more
-// evenly. Lines in the same pairs. 64 / 128 / 256 slots, in us: q32/kv8/hd128, 512 rows over 0 (16) 17.0/26.5/32.8, over 4700 (313)
-// 74.8/71.4/73.2, 600 over 3763 111.3/93.3/76.4 (128 slots: 150 workgroups for 256 compute units); q16/kv2/hd256, 512 over 0
-// 29.5/33.2, 4096 72/68.6, 1761 over 0 (98) 61/81, 2442 over 998 (339) 171/142.
+// evenly. Lines in the same pairs. 64 / 128 / 256 slots, in us: q32/kv8/hd128, 512 rows over 0 (16) 18.1/27.1/34.7, over 4700 (313)
+// 75.5/75.4/80.1; q32/kv8/hd64, 699 over 4394 112.8/97.4/89.7 (128 slots: 176 workgroups for 256 compute units); q32/kv8/hd128, 2026 over
+// 2682 224/183/200; q16/kv2/hd256, 512 over 0 30.3/34.3, 4096 71.8/72.1, q16/kv8/hd256, 3929 over 1284 363/303.
 TileShape fp4_chunk_shape(const Geom &g, size_t n_queries, size_t n_pages) {
     if (g.P > 256) return TileShape::one_tile;
     const long knob = tuning().prefill_tiles2_min_pages;
@@ -347,14 +347,15 @@ TileShape fp4_chunk_shape(const Geom &g, size_t n_queries, size_t n_pages) {
     const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, tiles = (n_slots + 15) / 16 * (size_t)g.kv_heads;
     const size_t pairs = tiles * (n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1);
     if (g.P > 128) {
-        const size_t one = wgs <= 128 ? 120000 : wgs <= 192 ? 50000 : wgs <= 256 ? 150000 : wgs <= 512 ? 340000 : 180000;
+        const size_t one = wgs <= 128 ? 120000 : wgs <= 192 ? 45000 : wgs <= 256 ? 150000 : wgs <= 512 ? 340000 : 180000;
         return pairs < one ? TileShape::halves : TileShape::one_tile;
     }
-    if (wgs > 512) return pairs >= (wgs <= 1024 ? 900000u : 500000u) ? TileShape::two_tiles : TileShape::one_tile;
+    if (wgs > 1024) return pairs >= 500000 ? TileShape::two_tiles : TileShape::one_tile;
+    if (wgs > 512) return g.P <= 64 && pairs >= 900000 ? TileShape::two_tiles : TileShape::one_tile;
     if (wgs > 256) {
         const bool own = n_queries / 8 >= n_pages;
         if (wgs <= 340 && pairs >= 150000 && !own) return TileShape::two_tiles;
-        return pairs < (own ? 300000u : 120000u) ? TileShape::halves : pairs < 450000 ? TileShape::one_tile : TileShape::two_tiles;
+        return pairs < (own ? 300000u : 120000u) ? TileShape::halves : g.P > 64 || pairs < 450000 ? TileShape::one_tile : TileShape::two_tiles;
     }
     return pairs < (wgs <= 128 ? 120000u : wgs <= 192 ? 75000u : 180000u) ? TileShape::halves : TileShape::one_tile;
 }
