@@ -244,13 +244,17 @@ hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
 // context. The wavefronts of a workgroup hold the same slots and walk the page pairs in turn.
 //
 // S^T = K . Q^T takes the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4 with K as e2m1 (a lane's 16 bytes are a row's 32 dims of
-// a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as four terms in e2m3 with a power a group and term:
-// digits of base 32 of the values as whole numbers of 20 bits, off by at most 2^-19 of the group's largest value, about what two bf16 terms
-// leave of each value. Four such products of 128 dims take 64 cycles, two of bf16 (eight instructions of 32 dims) 128, and
-// the codes would have to be converted.
-// O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to bf16 (exact) in registers, per page and group of dims
-// four conversions, four scales and four byte selections for eight values a lane, and P is two bf16 terms; a pair of pages is the 32 keys of
-// v_mfma_f32_16x16x32_bf16.
+// a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as five terms in e2m3 with a power a group and term:
+// digits of base 32 of the values as whole numbers of 25 bits, off by at most 2^-24 of the group's largest value. Five such products of 128
+// dims take 80 cycles, two of bf16 (eight instructions of 32 dims, for queries of 16 bits) 128, and the codes would have to be converted.
+// O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to f16 (exact, but for powers that f16 does not have, see fp4_far) in
+// registers, per page and group of dims four conversions, four scales and four byte selections for eight values a lane, and P is two f16
+// terms; a pair of pages is the 32 keys of v_mfma_f32_16x16x32_f16. A pair with other powers is multiplied in bf16, P in two terms.
+// Contexts are 2e-7 from 64 bits (2-norm, relative), 3e-7 over 32768 rows; four terms and two bf16 ones left 2.6e-6, for 3 to 7 % less time.
+//
+// What bounds it: over long contexts memory, 34.8 MB of 32000 rows of q32/kv8/hd128 in 14.6 us with the merge (a bf16 layer 24.9), 69.6 of
+// q16/kv8/hd256 in 20.2 (45.1); over short ones the chain of table, pages, products, states and a second launch: 600 to 2000 rows 7.6 and
+// 8.9 us, 100 rows 5.3 and 6.4 (bf16, 2000 rows: 7.3 and 8.4). Six rows over 8192 of q16/kv2/hd256 15.9.
 // ------------------------------------------------------------------------------------
 template <int P>
 struct Fp4Tile {
@@ -278,8 +282,8 @@ struct Fp4Lds {
 // stores the chunk's rows itself, at most MQ_APPEND_ROWS of them, as a decode step's does its one. PRE: a step whose queries and new K row are
 // normed and rotated here, from LDS that belongs to the wavefronts' second pairs until the first barrier behind it (the
 // pairs lie by depth then, the states of the wavefronts over both behind one more barrier). A step of q32/kv8/hd128 over 2000 rows from its
-// projections: 9.5 us, 14.1 with norm, rotation and append as launches of their own; of q16/kv2/hd256, gated, 11.7 and 17.8. (The
-// step alone: 7.4 and 8.8. The chain load, ordered sum, rotation, digits is longer than the first pages' way.)
+// projections: 9.5 us, 14.2 with norm, rotation and append as launches of their own; of q16/kv2/hd256, gated, 12.2 and 18.1. (The
+// step alone: 7.6 and 9.3. The chain load, ordered sum, rotation, digits is longer than the first pages' way.)
 template <int P, int WAVES, bool MQ, bool RING, bool ROWS = false, bool PRE = false>
 __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const ChunkPages *c, const int split, const int kvh, const int tile_z) {
     using T = Fp4Tile<P>;
@@ -894,7 +898,8 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 }
 
 template <int P, int WAVES, bool MQ, bool RING, bool ROWS, bool PRE>
-// (streaming chunks of heads up to 128 dims: registers for two workgroups on a compute unit, with one 256 rows over 2000 of q32/kv8/hd128 32.9 us, 29.2 with two)
+// (streaming chunks of heads up to 128 dims: registers for two workgroups on a compute unit. 256 rows over 2000 of q32/kv8/hd128 29.2 us, 32.9 with
+// registers for one.)
 __global__ __launch_bounds__(WAVES * 64, MQ && !ROWS && P <= 128 ? 4 : 1) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
     fp4_attention_body<P, WAVES, MQ, RING, ROWS, PRE>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
 }

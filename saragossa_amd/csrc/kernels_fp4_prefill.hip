@@ -46,16 +46,22 @@ __device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
 //
 // One workgroup = WAVES wavefronts of TILES tiles of 16 query slots of one kv head and a range of the pages any of them attends (split). It walks its
 // pages once, in steps: K's codes go to LDS as they are (1 KiB a page of 128 dims) and into the scaled products as they are, against the
-// queries as four terms of e2m3 in registers (kernels_fp4.hip); V's codes are converted to bf16 once for the workgroup, a page (or part of one) a
-// wavefront, in the order of the operands of v_mfma_f32_16x16x32_bf16 over a pair of pages. Per pair of pages and tile the products take 128
-// + 256 cycles of the matrix pipe at 128 dims, where bf16 K takes 256 + 256.
-// Per pair: S^T of the next pair with the exponentials and the two terms of this pair's probabilities between its products, then O^T of this
-// pair. The softmax runs in base 2 against a base that is up to 4 above the largest score and moves only when a score passes it; the score
-// accumulators start at minus the base (see prefill_tile_kernel).
+// queries as five terms of e2m3 in registers (kernels_fp4.hip); V's codes are converted to f16 once for the workgroup, a page (or part of one) a
+// wavefront, in the order of the operands of v_mfma_f32_16x16x32_f16 over a pair of pages. Per pair of pages and tile the products take 160
+// + 256 cycles of the matrix pipe at 128 dims (two bf16 terms of the queries against K in bf16: 256 + 256).
+// Per pair: S^T of the next pair with the exponentials and the two f16 terms of this pair's probabilities between its products, then O^T of this
+// pair. The softmax runs in base 2 against a base that a slot's largest score is 4 below or up to 8 above, and that moves only when one
+// passes that; probabilities are 2^8 times themselves at most (V is 2^-8 times itself), the score accumulators start at minus the base (see
+// prefill_tile_kernel).
 // With HALVES = 2 (or 4) the wavefronts are parts that hold the same slots and take the page pairs in turn; their states join through LDS.
 //
-// Keys that no slot of the workgroup attends have their powers cleared when V is converted: 0 x NaN is NaN. A row that is NaN and that some
-// slots attend and others do not (a row behind theirs) is converted to zeros, and the slots that attend it get their NaN in a path of its own.
+// Keys that no slot of the workgroup attends have their powers set to 1 when V is converted: 0 x NaN is NaN. A row that is NaN and that some
+// slots attend and others do not (a row behind theirs) is converted as if its power were 1, and the slots that attend it get their NaN in a path
+// of its own. Pages with powers that f16 does not have are converted to zeros and added in bf16, from memory, behind the pair's products.
+//
+// What bounds it: over long contexts the matrix pipe, 512 rows over 32768 of q16/kv2/hd256 in 358 us (770 TFLOP/s of the products asked for, which take
+// 1.63 times their time at the bf16 rate: 1250, what a large bf16 product reaches; a bf16 layer 409); over short ones its start, at head_dim 128 3 us until the queries are
+// converted, 2 until the first V is, and 3 at the end: 512 rows over 0, 1024 of q32/kv8/hd128 18.1, 30.6 (16.5, 30.3).
 // ------------------------------------------------------------------------------------
 template <int P, int WAVES, int HALVES>
 struct Fp4Chunk {
@@ -381,7 +387,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
             }
         }
     };
-    // probabilities of the settled scores, as two bf16 terms, in steps that stand between products: step q takes the exponential of score q and
+    // probabilities of the settled scores, as two f16 terms, in steps that stand between products: step q takes the exponential of score q and
     // splits those of scores q - 2 and q - 1
     float pr[TILES][2], prev[TILES];
     uint32_t hi4[TILES][4], lo4[TILES][4];

@@ -581,12 +581,12 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.n_pages = (int)((L->len + 15) / 16 - first);
     a.waves = g.P > 256 ? 4 : 8;
     // A pair to each of half the wavefronts, where there are not more: with all eight busy a step takes longer, in us over 600, 2000 rows of
-    // q32/kv8/hd128 8.0/7.3, 8.2/7.3, of q16/kv8/hd256 9.8/8.4, 10.0/8.6; with two or three to a split as with four, but more partials.
+    // q32/kv8/hd128 8.0/7.3, 8.2/7.3, of q16/kv8/hd256 9.8/8.4, 10.0/8.6 (with four terms of the queries, 0.3 to 0.5 less than now); with two or three to a split as with four, but more partials.
     // Whole while one pair each does it: over 250 rows 5.6/7.2, 7.7/8.1 (a second one each, over 400, 8.0/7.2, 9.7/8.2).
     const int pairs = (a.n_pages + 1) / 2;
     a.splits = pairs <= a.waves && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
-        // (one workgroup to a compute unit)
+        // (at most one workgroup to a compute unit: of heads above 128 dims a second one would wait, and what splits save is less than a round)
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
         a.splits = (int)std::min<size_t>((size_t)a.splits, std::max<size_t>(256 / tiles, 1));
         if (tiles > (size_t)g.kv_heads) a.splits = xcd_splits(a.splits, g.kv_heads, pairs, a.waves, 10);
@@ -1659,7 +1659,7 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
 
 // The same on a 4-bit ring layer. Up to a ring's rows go into the ring at once, by a launch that copies the pages they go into to the scratch
 // as they were: a launch less, and every row is quantised once (512 rows of q16/kv8/hd256 on a ring of 1056 rows 36.8 us
-// against 39.2, 128 rows 20.1 against 22.3). More of them overwrite each other, so those lie in the scratch themselves until all are attended.
+// against 39.2, 128 rows 20.1 against 22.3, before the queries' fifth term). More of them overwrite each other, so those lie in the scratch themselves until all are attended.
 static int32_t ring_chunk_fp4(skv_layer *L, hipStream_t s, const float *q, const float *k, const float *v, size_t c, float *out) {
     const Geom &g = L->g;
     const size_t base = L->len, ring_pages = (size_t)g.ring_rows / 16;
