@@ -536,10 +536,10 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         // the values as whole numbers of 25 bits, at most 2^24 (a float's own bits), in digits of base 32 between -16 and 15 (the first: 16), here
         // each 16 too large
         const int power = max((int)(most >> 23), 23);
-        const float scale = a.qscale * __uint_as_float((uint32_t)(277 - power) << 23);
+        const float scale = __uint_as_float((uint32_t)(277 - power) << 23); // (times qscale it might not be finite)
         uint32_t digits[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) digits[e] = (uint32_t)((int)__builtin_rintf(y[e] * scale) + 16 * (1 + 32 + 1024 + 32768 + 1048576));
+        for (int e = 0; e < 4; ++e) digits[e] = (uint32_t)((int)__builtin_rintf(y[e] * a.qscale * scale) + 16 * (1 + 32 + 1024 + 32768 + 1048576));
 #pragma unroll
         for (int k = 0; k < 5; ++k) {
             uint32_t four = 0;

@@ -168,6 +168,45 @@ def test_values_whose_powers_half_precision_does_not_have(state, chunk_kernel, d
     p.check_rows()
 
 
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512), (5, 1, 33)], ids=str)
+def test_queries_of_any_size(state, chunk_kernel, dims):
+    """Rows of zeros, groups of zeros, 1e-36 and 1e4 times normal rows, and one large dim among small ones."""
+    p = Pair(state, dims, 500, seed=12)
+    fresh = p.new
+
+    def new(n):
+        k, v, q = fresh(n)
+        q = q.reshape(n, dims[0], dims[2])
+        q[0::6] = 0
+        q[1::6, :, :32] = 0
+        q[2::6] *= np.float32(1e-36)
+        q[3::6] *= np.float32(1e4)
+        q[4::6, :, 3] *= np.float32(1e5)
+        return k, v, q.reshape(n, -1)
+
+    p.new = new
+    p.append(260)
+    p.step()
+    p.chunk(12)
+    p.chunk(80)
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 512)], ids=str)
+@pytest.mark.parametrize("attn_scalar", [1e-8, 1e-3, 1e8])
+def test_steps_of_any_scale(state, dims, attn_scalar):
+    p = Pair(state, dims, 400, seed=13)
+    p.append(300)
+    for zeros in (False, True):
+        k, v, q = p.new(1)
+        if zeros:
+            q[:, :dims[2] // 2] = 0
+        kd, vd, qd, out = _dev(k), _dev(v), _dev(q), torch.zeros(p.q_dim, device="cuda")
+        p.kv.encode_decode_step_prekv(_stream(), None, 0, qd.data_ptr(), 0, kd.data_ptr(), 0, vd.data_ptr(), 0, None, None, 1e-6, attn_scalar, out.data_ptr())
+        p.holds(k, v)
+        want, tol = attention(q, p.k, p.v, dims, attn_scalar=attn_scalar)
+        assert (np.abs(out.cpu().numpy()[None] - want) <= tol).all()
+
+
 # ---- graphs ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dims,window,base,rows", [((16, 2, 256), 0, 2000, 6), ((8, 2, 64), 0, 900, 130), ((32, 8, 128), 0, 2000, 128),
