@@ -581,8 +581,9 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.n_pages = (int)((L->len + 15) / 16 - first);
     a.waves = g.P > 256 ? 4 : 8;
     // A pair to each of half the wavefronts, where there are not more: with all eight busy a step takes longer, in us over 600, 2000 rows of
-    // q32/kv8/hd128 8.0/7.3, 8.2/7.3, of q16/kv8/hd256 9.8/8.4, 10.0/8.6 (with four terms of the queries, 0.3 to 0.5 less than now); with two or three to a split as with four, but more partials.
-    // Whole while one pair each does it: over 250 rows 5.6/7.2, 7.7/8.1 (a second one each, over 400, 8.0/7.2, 9.7/8.2).
+    // q32/kv8/hd128 8.3/7.5, 8.3/7.6, of q16/kv8/hd256 10.3/8.7, 10.5/9.0; with one to three to a split as with four or up to 1.2 more, but more
+    // partials. Whole while one pair each does it: over 250 rows 6.1/7.4, 8.3/8.6 (a second one each, over 400, 8.0/7.2, 9.7/8.2 when the queries
+    // had a term less).
     const int pairs = (a.n_pages + 1) / 2;
     a.splits = pairs <= a.waves && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
