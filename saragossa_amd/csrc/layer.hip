@@ -565,11 +565,25 @@ void fill_decode_args(const skv_layer *L, const float *q_dev, float *out_dev, si
     a.g = g;
 }
 
+// Pairs of pages up to which a context of a 4-bit layer is walked whole, by one workgroup to a kv head and sequence, or tile of 16 query slots:
+// a launch less. One pair to each wavefront; steps of heads up to 128, 64, 32 dims two, two and a half, three, and of batches more the more
+// workgroups there are. Whole / split, us of a step: q32/kv8/hd128 over 270, 500, 750 rows 6.7/7.5, 7.2/7.5, 8.8/7.6, hd64 6.3/7.5, 6.6/7.5, 7.7/7.6,
+// q4/kv2/hd32 5.9/7.1, 6.0/7.1, 6.8/7.1; q16/kv2/hd256 over 250, 300, 400 8.6/9.1, 8.7/9.6, 10.5/9.2; q8/kv2/hd512 over 120, 250 10.6/10.6, 14.7/13.1.
+// Batches: q32/kv8/hd128, 4 sequences of 600 rows 8.4/8.7, of 800 10.0/9.1, 8 of 800 10.7/10.9, of 1000 12.0/11.0, 16 of 1000 13.5/14.1, of 1500
+// 16.4/16.3; q8/kv2/hd64, 16 of 800 10.3/10.8, of 1000 11.3/10.7; q16/kv8/hd256, 16 of 600 13.3/15.3, of 1000 17.9/17.4.
+int fp4_whole_pairs(const Geom &g, size_t n_queries, size_t seqs) {
+    if (g.P > 256) return 4;
+    if (n_queries > 1) return 8;
+    const size_t wgs = (size_t)g.kv_heads * seqs;
+    if (g.P > 128) return wgs >= 128 ? 20 : 10;
+    const int line = g.P > 64 ? 16 : g.P > 32 ? 20 : 24;
+    return wgs >= 128 ? line * 2 : wgs >= 64 ? line * 3 / 2 : wgs >= 32 ? line * 9 / 8 : line;
+}
 // The same for the 4-bit element, whose kernel walks the pages that the queries can see as a list in the order of positions: a.page_first is the
 // first one's number, a.ring_base its place in the table, a.ring_t where the table comes round. A wavefront takes a pair of pages at a
 // time; no split leaves one without.
 void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_t window_start, const float *k_new, const float *v_new,
-                   size_t n_queries, size_t target_wgs, DecodeArgs &a) {
+                   size_t n_queries, size_t target_wgs, DecodeArgs &a, size_t seqs = 1) {
     fill_decode_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, target_wgs, a);
     const Geom &g = L->g;
     // (a decode step's window_start is the caller's, who may want less than the layer's window or all that a ring holds)
@@ -582,10 +596,9 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     a.waves = g.P > 256 ? 4 : 8;
     // A pair to each of half the wavefronts, where there are not more: with all eight busy a step takes longer, in us over 600, 2000 rows of
     // q32/kv8/hd128 8.3/7.5, 8.3/7.6, of q16/kv8/hd256 10.3/8.7, 10.5/9.0; with one to three to a split as with four or up to 1.2 more, but more
-    // partials. Whole while one pair each does it: over 250 rows 6.1/7.4, 8.3/8.6 (a second one each, over 400, 8.0/7.2, 9.7/8.2 when the queries
-    // had a term less).
+    // partials.
     const int pairs = (a.n_pages + 1) / 2;
-    a.splits = pairs <= a.waves && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
+    a.splits = pairs <= fp4_whole_pairs(g, n_queries, seqs) && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     if (n_queries * (size_t)g.gqa > 16) {
         // (at most one workgroup to a compute unit: of heads above 128 dims a second one would wait, and what splits save is less than a round)
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
@@ -2291,7 +2304,7 @@ int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_s
             const size_t share = std::max<size_t>(decode_target_wgs() * ((rows + 15) / 16) / std::max<size_t>(pages_total, 1),
                                                   (size_t)L->g.kv_heads);
             const float *k = reinterpret_cast<const float *>(k_dev[first + i]), *v = reinterpret_cast<const float *>(v_dev[first + i]);
-            if (L->g.fp4) fill_fp4_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i]);
+            if (L->g.fp4) fill_fp4_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], n);
             else fill_decode_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], false, whole_ok, wgs);
         };
         bool split = false, unsplit = false;
