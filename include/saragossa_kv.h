@@ -95,7 +95,7 @@ size_t skv_sdpa_2pass_blocks(size_t len);         /* utils.rs:282-286 */
 /* Rows below which this library never splits the context of a decode launch: RETI_RUST_SDPA_2PASS_MIN_LEN
  * when it is set (the reference's parse, default 2048 when unparsable), and then it splits from there on; else 128.
  * While neither it nor SKV_DECODE_WGS, SKV_PREFILL_WGS, SKV_DECODE_MIN_PAGES or SKV_DECODE_WAVES is set, contexts that are
- * faster whole stay so for longer: steps of 4-bit layers up to 512 rows (heads up to 64, 32 dims 640, 768, of 129 to 256 320, above 128; in batches up to twice as many), steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
+ * faster whole stay so for longer: steps of 4-bit layers up to 512 rows (heads up to 64, 32 dims 640, 768, of 129 to 256 320, above 128; in batches up to twice as many, chunks of few rows as many and more), steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
  * batches further the more sequences and kv heads they have (16 sequences of 8 kv heads 784, 656, 416), chunks of up to some
  * hundred rows up to 400 to 1500. The reference's
  * own default (2048, utils.rs:270-278) is what skv_flag_sdpa_2pass_min_len reports; it was tuned

@@ -571,9 +571,17 @@ void fill_decode_args(const skv_layer *L, const float *q_dev, float *out_dev, si
 // q4/kv2/hd32 5.9/7.1, 6.0/7.1, 6.8/7.1; q16/kv2/hd256 over 250, 300, 400 8.6/9.1, 8.7/9.6, 10.5/9.2; q8/kv2/hd512 over 120, 250 10.6/10.6, 14.7/13.1.
 // Batches: q32/kv8/hd128, 4 sequences of 600 rows 8.4/8.7, of 800 10.0/9.1, 8 of 800 10.7/10.9, of 1000 12.0/11.0, 16 of 1000 13.5/14.1, of 1500
 // 16.4/16.3; q8/kv2/hd64, 16 of 800 10.3/10.8, of 1000 11.3/10.7; q16/kv8/hd256, 16 of 600 13.3/15.3, of 1000 17.9/17.4.
+// Chunks of few rows: 6 rows over 300, 500, 800 of q32/kv8/hd128 8.2/9.5, 9.0/9.3, 10.1/9.9, 16 (32 tiles) over 800 10.5/11.4, 40 (80) over 1200
+// 14.1/14.0; of q8/kv2/hd64 7.1/8.1, 7.6/8.1, 8.4/8.3, 40 (20) over 800 9.1/10.0; of q16/kv2/hd256 12.4/12.9, 14.2/13.1, 16.2/13.9, 16 (16) over 500
+// 15.2/15.1, 40 (40) over 500, 800 13.9/16.4, 16.1/17.6.
 int fp4_whole_pairs(const Geom &g, size_t n_queries, size_t seqs) {
     if (g.P > 256) return 4;
-    if (n_queries > 1) return 8;
+    if (n_queries * (size_t)g.gqa > 16) {
+        const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;
+        if (g.P > 128) return tiles >= 32 ? 28 : tiles >= 16 ? 16 : 10;
+        if (g.P > 64) return tiles >= 80 ? 36 : tiles >= 32 ? 26 : 16;
+        return tiles >= 16 ? 30 : 24;
+    }
     const size_t wgs = (size_t)g.kv_heads * seqs;
     if (g.P > 128) return wgs >= 128 ? 20 : 10;
     const int line = g.P > 64 ? 16 : g.P > 32 ? 20 : 24;
