@@ -119,7 +119,7 @@ def test_rows_of_an_earlier_ring_chunk_leave_no_trace(chunk_kernel, dims, window
     assert np.isfinite(outs[0]).all() and np.array_equal(*outs)
 
 
-@pytest.mark.parametrize("window,rollback", [(64, 0), (60, 0), (64, None), (33, 3)])
+@pytest.mark.parametrize("window,rollback", [(64, 0), (60, 0), (64, None), (33, 3), (1, 0), (5, 20), (16, 0)])
 @pytest.mark.parametrize("dims", [(16, 8, 256), (8, 2, 64), (12, 4, 96), (8, 2, 512)], ids=str)
 def test_chunks_about_as_long_as_their_ring(state, chunk_kernel, dims, window, rollback):
     """Up to a ring's rows are stored before the chunk attends, with what they overwrite kept aside, more of them after it."""
@@ -127,7 +127,7 @@ def test_chunks_about_as_long_as_their_ring(state, chunk_kernel, dims, window, r
     ring = p.kv.pages() * 16
     p.append(ring + 5)
     for n in (ring - 6, ring, 3, ring - 16, 13, ring + 1, 2, 2 * ring + 7, 16, 17, ring - 1):
-        p.chunk(n)
+        p.chunk(max(n, 1))
         p.step()
         p.check_rows(p.kv.len() - window)
 
