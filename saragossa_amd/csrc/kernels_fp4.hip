@@ -613,7 +613,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
     float4_t o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.0f;
+    float b_run = -INFINITY, l_run = 0.0f; // what weights are relative to, their sum
 
     // a pair whose place in LDS has been read
     auto next_pair = [&](int it) __attribute__((always_inline)) {
@@ -757,17 +757,20 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
         }
         float m_blk = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         m_blk = rows_max(m_blk);
-        const float m_new = fmaxf(m_run, m_blk), m_safe = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = fast_exp2(m_run - m_safe);
-        float pr[8], psum = 0.0f; // times 2^8
+        // (the base lies 8 below the maximum while that difference is exact; from 2^27 on a step of f32 is 16, the difference would be 0 or 16, and 2^16
+        // is more than f16 has)
+        const float b_blk = fabsf(m_blk) < 0x1p27f ? m_blk - V_SHIFT : m_blk;
+        const float b_new = fmaxf(b_run, b_blk), b_safe = b_new == -INFINITY ? 0.0f : b_new;
+        const float alpha = fast_exp2(b_run - b_safe);
+        float pr[8], psum = 0.0f; // at most 2^8
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            pr[i] = fast_exp2(s[i >> 2][i & 3] - (m_safe - V_SHIFT));
+            pr[i] = fast_exp2(s[i >> 2][i & 3] - b_safe);
             psum += pr[i];
         }
         l_run = l_run * alpha + psum;
-        const bool rescale = alpha != 1.0f && m_run != -INFINITY; // (a slot without a key so far holds zeros)
-        m_run = m_new;
+        const bool rescale = alpha != 1.0f && b_run != -INFINITY; // (a slot without a key so far holds zeros)
+        b_run = b_new;
         if (__builtin_amdgcn_ballot_w64(rescale)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= alpha;
@@ -841,7 +844,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 #pragma unroll
         for (int t = 0; t < NT; ++t) *reinterpret_cast<float4_t *>(dst + t * 16) = o[t];
         if (j == 0) {
-            xm[wave * STATE + n] = m_run;
+            xm[wave * STATE + n] = b_run;
             xl[wave * STATE + n] = l_run;
         }
     }

@@ -1,0 +1,133 @@
+"""The 4-bit element's softmax where its base and its weights' steps show: scores so large that a step of 32 bits is 8 and more."""
+import contextlib
+import os
+
+import numpy as np
+import pytest
+
+import saragossa_amd as skv
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).cuda()
+
+
+@contextlib.contextmanager
+def _env(**env):
+    saved = {k: os.environ.get(k) for k in env}
+    os.environ.update(env)
+    skv.flags.reload()
+    try:
+        yield
+    finally:
+        for k, was in saved.items():
+            os.environ.pop(k) if was is None else os.environ.__setitem__(k, was)
+        skv.flags.reload()
+
+
+def _step(kv, k, v, q):
+    kd, vd, qd, out = _dev(k), _dev(v), _dev(q), torch.zeros(q.size, device="cuda")
+    kv.encode_decode_step(_stream(), kd.data_ptr(), 0, vd.data_ptr(), 0, qd.data_ptr(), out.data_ptr())
+    return out.cpu().numpy().reshape(1, -1)
+
+
+def _projections(kv, k, v, q):
+    kd, vd, qd, out = _dev(k), _dev(v), _dev(q), torch.zeros(q.size, device="cuda")
+    kv.encode_decode_step_prekv(_stream(), None, 0, qd.data_ptr(), 0, kd.data_ptr(), 0, vd.data_ptr(), 0, None, None, 1e-6, float(kv.head_dim()), out.data_ptr())
+    return out.cpu().numpy().reshape(1, -1)
+
+
+def _chunk(kv, k, v, q):
+    return kv.prefill_rows(q, k, v).reshape(len(q), -1)
+
+
+# how the last rows are attended: their number, the call, the environment
+CALLS = {"step": (1, _step, {}), "whole step": (1, _step, {"RETI_RUST_SDPA_2PASS": "0"}), "from the projections": (1, _projections, {}), "few rows": (6, _chunk, {}),
+         "streaming chunk": (70, _chunk, {"SKV_PREFILL_TILES": "0"}), "chunk kernel": (70, _chunk, {"SKV_PREFILL_TILES": "2"})}
+
+
+def _layer_of(state, rng, dims, n, window):
+    kv = state.full_attention_fp4(n, *dims, window=window)
+    kv.set_block_table(rng.permutation(kv.pages()).astype(np.int32))
+    return kv
+
+
+def _ties(rng, dims, n, m, sign, octave):
+    """n rows whose keys have one dim that is not zero, 2^(octave - 7) or half of that, and m queries of one dim that is not zero, so that a score in
+    base 2 is exact in 32 bits and lies in [2^octave, 2^(octave + 1)), or is half of one that does: keys of the same size tie, the others are 2^(octave - 1)
+    away. The rows' keys and values, the queries, and a mask [n] of the larger keys."""
+    heads, kv_heads, hd = dims
+    large = rng.random(n) < 0.5
+    k = np.zeros((n, kv_heads, hd), np.float32)
+    k[:, :, 3] = np.where(large, 2.0, 1.0)[:, None] * 2.0 ** (octave - 8)
+    v = np.sign(rng.standard_normal((n, kv_heads, hd))) * rng.choice([1.0, 2.0, 4.0], (n, kv_heads, hd))
+    q = np.zeros((m, heads, hd), np.float32)
+    qscale = np.float32(np.float32(1.0) / np.sqrt(np.float32(hd))) * np.float32(1.4426950408889634)
+    q[:, :, 3] = sign * np.exp2(7.1 + 0.8 * rng.random((m, heads))) / qscale
+    if octave == 27:  # (steps of 16: about half of the largest scores are odd multiples)
+        s = np.abs(q[:, :, 3] * qscale).astype(np.float64) * 2.0 ** 20
+        assert (s / 16 % 2 == 1).any()
+    return k.reshape(n, -1), v.astype(np.float32).reshape(n, -1), q.reshape(m, -1), large
+
+
+def _mean_of_ties(dims, v, large, m, sign, window):
+    """The contexts of the last m rows: the mean over the keys of the largest score that a row sees, and how far sums of that many values in 32 bits
+    may be off in any order, a quotient and the joining of partials with them: half a step of the sum of magnitudes each."""
+    heads, kv_heads, hd = dims
+    n = len(v)
+    vv = np.repeat(v.astype(np.float64).reshape(n, kv_heads, hd), heads // kv_heads, 1)
+    want, tol = np.empty((m, heads, hd)), np.empty((m, heads, hd))
+    for i in range(m):
+        hi = n - m + i + 1
+        lo = max(0, hi - window) if window else 0
+        top = large[lo:hi] if sign > 0 else ~large[lo:hi]
+        keys = vv[lo:hi][top if top.any() else ~top]
+        want[i] = keys.mean(0)
+        tol[i] = (len(keys) + 40) * 2.0 ** -24 * np.abs(keys).mean(0)
+    return want.reshape(m, -1), tol.reshape(m, -1)
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512)], ids=str)
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("octave,window", [(26, 0), (27, 0), (27, 100), (40, 100)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size_have_finite_weights(state, dims, call, octave, sign, window):
+    m, run, env = CALLS[call]
+    rng = np.random.default_rng(octave + dims[2])
+    n = 333
+    k, v, q, large = _ties(rng, dims, n, m, sign, octave)
+    want, tol = _mean_of_ties(dims, v, large, m, sign, window)
+    kv = _layer_of(state, rng, dims, n, window)
+    kv.seed(k[:n - m], v[:n - m], n - m)
+    with _env(**env):
+        got = run(kv, k[n - m:], v[n - m:], q)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= tol).all(), np.abs((got - want) / tol).max()
+    kv.close()
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512)], ids=str)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size_in_batches(state, dims, sign):
+    rng = np.random.default_rng(dims[2])
+    seqs = []
+    for n in (1, 17, 200, 333, 900):
+        k, v, q, large = _ties(rng, dims, n, 1, sign, 27)
+        kv = _layer_of(state, rng, dims, n, 0)
+        if n > 1:
+            kv.seed(k[:-1], v[:-1], n - 1)
+        seqs.append((kv, _dev(k[-1]), _dev(v[-1]), _dev(q), torch.zeros(q.size, device="cuda"), _mean_of_ties(dims, v, large, 1, sign, 0)))
+    at = [[s[i].data_ptr() for s in seqs] for i in range(1, 5)]
+    skv.encode_decode_step_batch([s[0] for s in seqs], _stream(), *at)
+    for kv, _, _, _, out, (want, tol) in seqs:
+        got = out.cpu().numpy()[None]
+        assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
+        kv.close()
