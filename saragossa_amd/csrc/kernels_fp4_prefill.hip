@@ -50,8 +50,8 @@ __device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
 // wavefront, in the order of the operands of v_mfma_f32_16x16x32_f16 over a pair of pages. Per pair of pages and tile the products take 160
 // + 256 cycles of the matrix pipe at 128 dims (two bf16 terms of the queries against K in bf16: 256 + 256).
 // Per pair: S^T of the next pair with the exponentials and the two f16 terms of this pair's probabilities between its products, then O^T of this
-// pair. The softmax runs in base 2 against a base that a slot's largest score is 4 below or up to 8 above, and that moves only when one
-// passes that; probabilities are 2^8 times themselves at most (V is 2^-8 times itself), the score accumulators start at minus the base (see
+// pair. The softmax runs in base 2 against a base that a slot's largest score is 7 to 11 above, and that moves only when one passes that: weights are
+// held to 2^-32 of the largest at least (f16's steps end at 2^-24), V being 2^-8 times itself. The score accumulators start at minus the base (see
 // prefill_tile_kernel).
 // With HALVES = 2 (or 4) the wavefronts are parts that hold the same slots and take the page pairs in turn; their states join through LDS.
 //
@@ -313,8 +313,9 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     convert_v(0);
 
     float4_t o[TILES][NT], neg_m[TILES];
-    // a score whose bits reach thr moves the base: any more than 8 above it, or, of a slot without a key so far, whatever it is
-    constexpr int UNSEEN = INT32_MIN, SEEN = 0x41000001;
+    // a score whose bits reach thr moves the base, to 7 under it: any more than 11 above the base, or, of a slot without a key so far, whatever it
+    // is. (7 and not 8, which from 2^27 on, where a step of f32 is 16, would be 16 half of the time: 2^16 is more than f16 has.)
+    constexpr int UNSEEN = INT32_MIN, SEEN = 0x41300001;
     float m_base[TILES], l_run[TILES];
     int thr[TILES];
 #pragma unroll
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 const float mx = fmaxf(fmaxf(fmaxf(sa[t][0], sa[t][1]), fmaxf(sa[t][2], sa[t][3])), fmaxf(fmaxf(sb[t][0], sb[t][1]), fmaxf(sb[t][2], sb[t][3])));
                 const float top = rows_max(mx); // of the slot, relative to its base
                 const bool unseen = thr[t] < 0;
-                const float d = top > (unseen ? -INFINITY : 8.0f) ? top - 4.0f : 0.0f;
+                const float d = top > (unseen ? -INFINITY : 11.0f) ? top - 7.0f : 0.0f;
                 const float alpha = unseen ? 1.0f : fast_exp2(-d);
                 m_base[t] += d;
                 neg_m[t] = float4_t{-m_base[t], -m_base[t], -m_base[t], -m_base[t]};

@@ -1,4 +1,5 @@
-"""The 4-bit element's softmax where its base and its weights' steps show: scores so large that a step of 32 bits is 8 and more."""
+"""The 4-bit element's softmax where its base and its weights' steps show: scores so large that a step of 32 bits is 8 and more, and many
+keys far below one."""
 import contextlib
 import os
 
@@ -131,3 +132,43 @@ def test_scores_of_any_size_in_batches(state, dims, sign):
         got = out.cpu().numpy()[None]
         assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
         kv.close()
+
+
+# The kernels of chunks of many rows
+SHAPES = {"halves": {"SKV_PREFILL_TILES": "2"}, "one tile": {"SKV_PREFILL_TILES": "2", "SKV_PREFILL_TILES2_MIN_PAGES": "1000000"},
+          "two tiles": {"SKV_PREFILL_TILES": "2", "SKV_PREFILL_TILES2_MIN_PAGES": "0"}, "streaming": {"SKV_PREFILL_TILES": "0"}}
+
+
+@pytest.mark.parametrize("dims", [(8, 2, 64), (8, 1, 128), (4, 1, 256), (4, 1, 512)], ids=str)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_many_far_keys_behind_one_large_one_are_counted(state, dims, shape):
+    """Row 0 has a score of 29.5 (in base 2) and values of 0, 12 rows of each page a score of 0 and values of 1, the rest no weight to speak of: the
+    context is what the 12 rows' weights, 2^-29.5 each of the largest, are together, 3.2e-5.
+
+    Weights are in steps of 2^-24, the largest is 2^7 or more: each may be off by 2^-32 of the largest. Beside that by 2^-22 of itself, the
+    exponential by 2^-22, the score of 29.5 by its four roundings of 2^-24, which is 5e-6 of the weights' ratio, and sums of 2052 sums by half a step of 2^-24
+    each: 1.3e-4 of the context together."""
+    heads, kv_heads, hd = dims
+    n, m = 32768, 64
+    rng = np.random.default_rng(hd)
+    k = np.zeros((n + m, kv_heads, hd), np.float32)
+    row = np.arange(n + m) % 16
+    k[row < 4, :, 3] = -1.0
+    k[0, :, 3] = 1.0
+    v = np.ones((n + m, kv_heads * hd), np.float32)
+    v[0] = 0
+    q = np.zeros((m, heads, hd), np.float32)
+    q[:, :, 3] = 29.5 * np.sqrt(hd) / 1.4426950408889634
+    kv = _layer_of(state, rng, dims, n + m, 0)
+    k = k.reshape(n + m, -1)
+    for i in range(0, n, 8192):
+        kd, vd = _dev(k[i:i + 8192]), _dev(v[i:i + 8192])
+        kv.encode_append_batch(_stream(), kd.data_ptr(), vd.data_ptr(), 8192)
+        torch.cuda.synchronize()
+    with _env(SKV_PREFILL_MAX_SPLITS="1", **SHAPES[shape]):
+        got = _chunk(kv, k[n:], v[n:], q.reshape(m, -1))
+    for i in range(m):
+        far = (row[:n + i + 1] >= 4).sum() * 2.0 ** -29.5
+        want = far / (1 + far)
+        assert np.abs(got[i] - want).max() <= (row[:n + i + 1] >= 4).sum() * 2.0 ** -32 + 1.4e-4 * want, i
+    kv.close()
