@@ -958,11 +958,11 @@ hipError_t launch_decode(const DecodeArgs &a, hipStream_t s) {
 }
 
 // Whether the wavefront merge serves these partials: 16-byte column loads, 32-bit offsets
-// within a kv head, and a grid that fits.
+// within a kv head, a grid that fits, and at most the 16 x 16 splits that its widest variant reads.
 static bool merge_wave_fits(const DecodeArgs &a) {
     const uint64_t n_slots = (uint64_t)a.n_queries * a.g.gqa;
     return a.g.head_dim % 4 == 0 && (uint64_t)a.splits_total * n_slots * a.g.head_dim * 4 < (1ull << 32) &&
-           n_slots <= 65535 && a.g.kv_heads <= 65535 && a.splits_total <= 16 * MERGE_PER_LANE_MAX &&
+           n_slots <= 65535 && a.g.kv_heads <= 65535 && a.splits_total <= 16 * 16 &&
            ((uintptr_t)a.part_o & 15) == 0 && ((uintptr_t)a.out & 15) == 0;
 }
 
@@ -1000,6 +1000,7 @@ static hipError_t launch_merge_wave(const DecodeArgs &a, hipStream_t s) {
 
 hipError_t launch_merge(const DecodeArgs &a, hipStream_t s) {
     if (merge_wave_fits(a)) return launch_merge_wave(a, s);
+    if (a.splits_total > 16 * MERGE_PER_LANE_MAX) return launch_merge_rows(a, s); // (of a chunk, whose splits have no bound here)
     dim3 mgrid((unsigned)(a.g.kv_heads * a.n_queries * a.g.gqa), (unsigned)((a.g.head_dim + 15) / 16));
     const int per_lane = (a.splits_total + 15) / 16;
     if (per_lane <= 1) hipLaunchKernelGGL(decode_merge_kernel<1>, mgrid, dim3(256), 0, s, a);
