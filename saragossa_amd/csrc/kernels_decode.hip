@@ -123,7 +123,7 @@ __device__ __forceinline__ void decode_split_body(const DecodeArgs &a, const int
     // pages this workgroup's slots can see, divided among the splits
     const int page_lo = g.ring_rows > 0 ? 0 : ws_lo >> 4;
     const int page_hi = g.ring_rows > 0 ? a.n_pages : (lim_hi >> 4) + 1;
-    // (32-bit arithmetic: pages * splits stays far below 2^31)
+    // (32-bit arithmetic: see most_splits)
     const unsigned span = (unsigned)(page_hi - page_lo);
     const int pb0 = page_lo + (int)(((unsigned)split * span) / (unsigned)a.splits);
     const int pb1 = page_lo + (int)(((unsigned)(split + 1) * span) / (unsigned)a.splits);

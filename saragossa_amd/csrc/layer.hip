@@ -373,7 +373,7 @@ int chunk_splits(const Geom &g, size_t n_queries, size_t per_wg, size_t n_pages)
     const size_t tiles = (n_queries * (size_t)g.gqa + per_wg - 1) / per_wg * (size_t)g.kv_heads;
     size_t want = std::max<size_t>(tuning().prefill_wgs / tiles, 1);
     want = std::min<size_t>(want, std::max<size_t>(n_pages / 16, 1));
-    return (int)std::min<size_t>(want, tuning().prefill_max_splits);
+    return (int)std::min<size_t>(std::min(want, tuning().prefill_max_splits), most_splits(n_pages));
 }
 
 // Splits of a launch in which the workgroups of several query tiles walk the same pages. Workgroup ids, the split fastest,
@@ -404,7 +404,7 @@ int choose_splits(const skv_layer *L, int n_pages_scan, size_t rows, int waves, 
     // not down: with one page per wavefront no wavefront then walks a second page, which
     // would be a whole memory latency more for the launch).
     s = std::min<size_t>(s, ((size_t)n_pages_scan + min_pages - 1) / min_pages);
-    s = std::min<size_t>(s, (size_t)L->max_splits);
+    s = std::min<size_t>({s, (size_t)L->max_splits, most_splits((size_t)n_pages_scan)});
     return (int)std::max<size_t>(s, 1);
 }
 
@@ -607,6 +607,7 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     // partials.
     const int pairs = (a.n_pages + 1) / 2;
     a.splits = pairs <= fp4_whole_pairs(g, n_queries, seqs) && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
+    a.splits = (int)std::min<size_t>((size_t)a.splits, most_splits((size_t)a.n_pages)); // (of pages, not of pairs)
     if (n_queries * (size_t)g.gqa > 16) {
         // (at most one workgroup to a compute unit: of heads above 128 dims a second one would wait, and what splits save is less than a round)
         const size_t tiles = (n_queries * (size_t)g.gqa + 15) / 16 * (size_t)g.kv_heads;

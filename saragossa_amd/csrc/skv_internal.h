@@ -11,6 +11,7 @@
 #include <string>
 
 #include "../../include/saragossa_kv.h"
+#include "split_share.h"
 
 namespace skv {
 
