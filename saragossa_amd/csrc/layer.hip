@@ -326,7 +326,9 @@ bool takes_f32_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
 // chunks of 4 to 1024 rows in nine geometries, on layers in no cache, kernel and shape chosen are 0.6 % slower than the best on the
 // average, 30 % at most. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
 // 18.4/24.7, 256 (70) 29.0/32.1, 64 over 8000 (65) 31.4/29.2, 512 over 512 (49, 256 workgroups) 27.4/24.3; q16/kv2/hd256, 64 over 8192 (33)
-// 32.3/37.1, 128 (66) 49.8/49.5, q16/kv8/hd256, 256 over 8000 (131) 81.6/78.4; q8/kv2/hd512 loses in the mean from 16 on.
+// 32.3/37.1, 128 (66) 49.8/49.5, q16/kv8/hd256, 256 over 8000 (131) 81.6/78.4; q8/kv2/hd512 loses in the mean from 16 on. 16 rows, stored by the
+// streaming launch or by one of their own: q16/kv1/hd128 over 32000, 64000, 128000 (32, 64, 128) 21.0/22.4, 32.2/28.6, 52.9/42.3, q8/kv2/hd512 over 32000 (16)
+// 71.1/48.7.
 bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
     const size_t n_slots = n_queries * (size_t)g.gqa;
     if (tuning().prefill_tiles != 1 || n_slots < 64) return tuning().prefill_tiles > 1 && n_slots >= 64;
@@ -344,6 +346,7 @@ TileShape fp4_chunk_shape(const Geom &g, size_t n_queries, size_t n_pages) {
     const long knob = tuning().prefill_tiles2_min_pages;
     if (knob >= 0) return g.P <= 128 && (long)n_pages >= knob ? TileShape::two_tiles : TileShape::one_tile;
     const size_t n_slots = n_queries * (size_t)g.gqa;
+    if (n_slots <= 64) return TileShape::halves; // (a wider workgroup has wavefronts without slots: 16 rows over 64000 of q32/kv8/hd64 36.4 us, 48.2 with 128 slots)
     const size_t wgs = (n_slots + 63) / 64 * (size_t)g.kv_heads, tiles = (n_slots + 15) / 16 * (size_t)g.kv_heads;
     const size_t pairs = tiles * (n_pages > n_queries / 32 ? n_pages - n_queries / 32 : 1);
     if (g.P > 128) {
@@ -1830,10 +1833,10 @@ int32_t skv_prefill_chunk_device(skv_layer *L, skv_stream stream, const float *q
             out += c * q_dim;
             continue;
         }
-        // a few rows over a full bf16 layer (a speculative verify, the rest of a prompt): the multi-query launch
+        // a few rows over a full bf16 or 4-bit layer (a speculative verify, the rest of a prompt): the multi-query launch
         // appends them itself, as a decode step's does (its last query tile, which sees all of them, stores them)
-        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && tuning().fused_append &&
-            !context_over_rows(L, c, out, k, v) && (L->g.fp4 || !takes_tile_kernel(L->g, c, (L->len + c + 15) / 16))) {
+        if (c > 1 && c <= (size_t)MQ_APPEND_ROWS && ring == 0 && !L->g.f32 && tuning().fused_append && !context_over_rows(L, c, out, k, v) &&
+            !(L->g.fp4 ? takes_fp4_chunk_kernel : takes_tile_kernel)(L->g, c, (L->len + c + 15) / 16)) {
             RowsAhead ahead(L, c);
             rc = encode_attention(L, as_stream(stream), q, out, 0, k, v, c);
             if (rc) return rc;
