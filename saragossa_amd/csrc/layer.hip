@@ -594,7 +594,7 @@ int fp4_whole_pairs(const Geom &g, size_t n_queries, size_t seqs) {
 // first one's number, a.ring_base its place in the table, a.ring_t where the table comes round. A wavefront takes a pair of pages at a
 // time; no split leaves one without.
 void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_t window_start, const float *k_new, const float *v_new,
-                   size_t n_queries, size_t target_wgs, DecodeArgs &a, size_t seqs = 1) {
+                   size_t n_queries, size_t target_wgs, DecodeArgs &a, size_t seqs = 1, bool whole_ok = true) {
     fill_decode_args(L, q_dev, out_dev, window_start, k_new, v_new, n_queries, target_wgs, a);
     const Geom &g = L->g;
     // (a decode step's window_start is the caller's, who may want less than the layer's window or all that a ring holds)
@@ -609,7 +609,7 @@ void fill_fp4_args(const skv_layer *L, const float *q_dev, float *out_dev, size_
     // q32/kv8/hd128 8.3/7.5, 8.3/7.6, of q16/kv8/hd256 10.3/8.7, 10.5/9.0; with one to three to a split as with four or up to 1.2 more, but more
     // partials.
     const int pairs = (a.n_pages + 1) / 2;
-    a.splits = pairs <= fp4_whole_pairs(g, n_queries, seqs) && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
+    a.splits = whole_ok && pairs <= fp4_whole_pairs(g, n_queries, seqs) && may_stay_whole() ? 1 : choose_splits(L, pairs, L->len - window_start, 4, target_wgs);
     a.splits = (int)std::min<size_t>((size_t)a.splits, most_splits((size_t)a.n_pages)); // (of pages, not of pairs)
     if (n_queries * (size_t)g.gqa > 16) {
         // (at most one workgroup to a compute unit: of heads above 128 dims a second one would wait, and what splits save is less than a round)
@@ -2298,7 +2298,8 @@ int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_s
         }
         // All contexts stay whole or none does: the merge of one is a launch for all, and a whole one then only walks longer. Batches of two,
         // each by itself / none, us: q8/kv2/hd64 over 370, 400 rows 7.5/6.3, q16/kv2/hd256 over 150, 400 9.3/8.3, q4/kv1/hd128 over 250, 2000
-        // 7.7/6.9; four of q32/kv8/hd128 over 250, one of them over 600 8.5/8.0.
+        // 7.7/6.9; four of q32/kv8/hd128 over 250, one of them over 600 8.5/8.0. 4-bit layers: q32/kv8/hd128 over 500, 500, 500, 2000 17.1/12.6, over 250,
+        // 250, 250, 1000 9.8/8.8, q8/kv2/hd64, seven over 600 and one over 4000 12.1/9.3, q16/kv2/hd256 over 300, 300, 300, 4000 11.9/10.5.
         // (Arguments are filled again only where one had stayed whole. Host time of a call, 16 of q32/kv8/hd128 over 4000 rows, all filled
         // twice / once: 13.2/11.9.)
         const int wgs = (int)n * seqs[0]->g.kv_heads, line = whole_step_pages(seqs[0]->g, wgs);
@@ -2316,17 +2317,19 @@ int32_t skv_decode_step_batch_device(skv_layer *const *seqs, size_t n_seq, skv_s
             const size_t share = std::max<size_t>(decode_target_wgs() * ((rows + 15) / 16) / std::max<size_t>(pages_total, 1),
                                                   (size_t)L->g.kv_heads);
             const float *k = reinterpret_cast<const float *>(k_dev[first + i]), *v = reinterpret_cast<const float *>(v_dev[first + i]);
-            if (L->g.fp4) fill_fp4_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], n);
+            if (L->g.fp4) fill_fp4_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], n, whole_ok);
             else fill_decode_args(L, q_dev[first + i], out_dev[first + i], ws, k, v, 1, share, b.seq[i], false, whole_ok, wgs);
         };
+        uint32_t whole = is_short; // (4-bit sequences: by fp4_whole_pairs, known once their arguments are)
         bool split = false, unsplit = false;
         for (size_t i = 0; i < n; ++i) {
             fill(i, over == 0);
+            if (seqs[0]->g.fp4 && b.seq[i].splits == 1) whole |= 1u << i;
             split = split || b.seq[i].splits > 1;
             unsplit = unsplit || b.seq[i].splits == 1;
         }
         for (size_t i = 0; split && over == 0 && i < n; ++i)
-            if (is_short >> i & 1) fill(i, false);
+            if (whole >> i & 1) fill(i, false);
         // an unsplit context over what other workgroups read is written aside (see encode_attention)
         if (unsplit && !is_short) over = look();
         for (size_t i = 0; i < n; ++i)
