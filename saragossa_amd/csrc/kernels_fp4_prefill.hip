@@ -24,17 +24,18 @@ namespace {
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // two values rounded to bf16 (nearest even), the first in the low half: one instruction
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v_t{x, y}, bf16x2_t)); }
-// 32 values as e2m3 codes of x / scale, and the codes' values. These conversions take several passes and write their results as they go: a
-// result register that is also an operand is read back changed (seen: the scale in the first result register, the values after the first
-// few wrong), and the compiler does not know. Operands are kept alive behind the instruction, so that they have registers of their own.
-__device__ __forceinline__ u6 to_fp6(float16_t even, float16_t odd, float scale) { // (they take turns in the result)
-    u6 codes = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
-    asm volatile("" : "+v"(codes) : "v"(even), "v"(odd), "v"(scale));
+// 32 values as e2m3 codes of x / scale (those of `even` and `odd` take turns in the result), and the codes' values. These conversions take several
+// passes and write their results as they go: a result register that is also an operand is read back changed (seen: the scale in the first result
+// register, the values after the first few wrong). The compiler does not know of that, so results are early clobbers, which no operand
+// shares; nor then of the wait state that a reader of the result needs.
+__device__ __forceinline__ u6 to_fp6(float16_t even, float16_t odd, float scale) {
+    u6 codes;
+    asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(codes) : "v"(even), "v"(odd), "v"(scale));
     return codes;
 }
 __device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
-    float32_t x = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(codes, scale);
-    asm volatile("" : "+v"(x) : "v"(codes), "v"(scale));
+    float32_t x;
+    asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n\ts_nop 1" : "=&v"(x) : "v"(codes), "v"(scale));
     return x;
 }
 
