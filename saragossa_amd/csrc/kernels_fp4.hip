@@ -249,7 +249,7 @@ hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
 // dims take 80 cycles, two of bf16 (eight instructions of 32 dims, for queries of 16 bits) 128, and the codes would have to be converted.
 // O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to f16 (exact, but for powers that f16 does not have, see fp4_far) in
 // registers, per page and group of dims four conversions, four scales and four byte selections for eight values a lane, and P is two f16
-// terms; a pair of pages is the 32 keys of v_mfma_f32_16x16x32_f16. A pair with other powers is multiplied in bf16, P in two terms.
+// terms; a pair of pages is the 32 keys of v_mfma_f32_16x16x32_f16. A pair with other powers is multiplied in bf16, P in three terms (chunks of heads to 128 dims: two).
 // Contexts are 2e-7 from 64 bits (2-norm, relative), 3e-7 over 32768 rows; four terms and two bf16 ones left 2.6e-6, for 3 to 7 % less time.
 //
 // What bounds it: over long contexts memory, 34.8 MB of 32000 rows of q32/kv8/hd128 in 14.6 us with the merge (a bf16 layer 24.9), 69.6 of
@@ -776,11 +776,11 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
             for (int t = 0; t < NT; ++t) o[t] *= alpha;
         }
         // ---- O^T += V^T . P^T
-        uint32_t hi[4], lo[4], far = 0;
+        uint32_t far = 0;
 #pragma unroll
         for (int t = 0; t < G; ++t) far |= fp4_far(vp[0][t]) | fp4_far(vp[1][t]);
-        // dims 32 t + n and 32 t + 16 + n of the 32 keys, from the pairs that c0 .. c3 hold of each page
-        auto products = [&](int t, auto of_page, auto mfma) __attribute__((always_inline)) {
+        // dims 32 t + n and 32 t + 16 + n of the 32 keys, from the pairs that c0 .. c3 hold of each page, with weights in terms, the least first
+        auto products = [&](int t, auto of_page, auto mfma, const auto &terms) __attribute__((always_inline)) {
             u4 first, second;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -790,18 +790,29 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                 second[2 * h] = __builtin_amdgcn_perm(c[1], c[0], 0x07060302u);
                 second[2 * h + 1] = __builtin_amdgcn_perm(c[3], c[2], 0x07060302u);
             }
-            o[2 * t] = mfma(first, lo, o[2 * t]);
-            o[2 * t + 1] = mfma(second, lo, o[2 * t + 1]);
-            o[2 * t] = mfma(first, hi, o[2 * t]);
-            o[2 * t + 1] = mfma(second, hi, o[2 * t + 1]);
+#pragma unroll
+            for (const auto &x : terms) {
+                o[2 * t] = mfma(first, x, o[2 * t]);
+                o[2 * t + 1] = mfma(second, x, o[2 * t + 1]);
+            }
         };
-        if (__builtin_amdgcn_ballot_w64(far != 0)) { // uniform: powers that f16 does not have, or NaN
+        // Powers that f16 does not have, or NaN, in bf16 instead.
+        // Terms of 8 bits, the least first: three leave 2^-24 of a weight. Two, which leave 2^-17, where registers are those of two workgroups on a compute
+        // unit: the third's would be reloaded on every pair (128 rows over 512, 1024 on rings of q32/kv8/hd128 13.1/14.2, 16.5/18.3 us).
+        constexpr int TERMS = MQ && !ROWS && P <= 128 ? 2 : 3;
+        const bool any_far = __builtin_amdgcn_ballot_w64(far != 0) != 0; // uniform
+        if (TERMS == 3 ? __builtin_expect(any_far, false) : any_far) { // (apart from the code around it: steps of hd128 are 0.05 us faster; with two terms it spills)
+            uint32_t terms[TERMS][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 typedef __attribute__((ext_vector_type(2))) float f2;
-                const float x = pr[2 * i] * P_SCALE, y = pr[2 * i + 1] * P_SCALE;
-                hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf16x2_t));
-                lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u)}, bf16x2_t));
+                f2 left = {pr[2 * i] * P_SCALE, pr[2 * i + 1] * P_SCALE};
+#pragma unroll
+                for (int k = TERMS - 1; k >= 0; --k) {
+                    terms[k][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(left, bf16x2_t));
+                    left -= f2{__uint_as_float(terms[k][i] << 16), __uint_as_float(terms[k][i] & 0xffff0000u)};
+                }
+                pr[2 * i] = pr[2 * i + 1] = 0.0f; // (f16's products then add zeros: with a path of their own, o would be in two places)
             }
 #pragma unroll
             for (int t = 0; t < G; ++t) {
@@ -810,14 +821,16 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                     t, [](uint32_t w, uint32_t e) __attribute__((always_inline)) { return u4{code_pair<0>(w, e << 23), code_pair<1>(w, e << 15), code_pair<2>(w, e << 7), code_pair<3>(w, e >> 1)}; },
                     [](u4 v, const uint32_t(&x)[4], float4_t to) __attribute__((always_inline)) {
                         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, u4{x[0], x[1], x[2], x[3]}), to, 0, 0, 0);
-                    });
-                vc[0][t] = vc[1][t] = 0; // (f16's products then add zeros: with a path of their own, o would be in two places)
+                    },
+                    terms);
+                vc[0][t] = vc[1][t] = 0;
                 vp[0][t] = vp[1][t] = 0x7f7f7f7fu;
             }
         }
         {
+            uint32_t terms[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f16_terms(pr[2 * i], pr[2 * i + 1], hi[i], lo[i]);
+            for (int i = 0; i < 4; ++i) f16_terms(pr[2 * i], pr[2 * i + 1], terms[1][i], terms[0][i]);
 #pragma unroll
             for (int t = 0; t < G; ++t) {
                 products(
@@ -827,7 +840,8 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
                     },
                     [](u4 v, const uint32_t(&x)[4], float4_t to) __attribute__((always_inline)) {
                         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, v), __builtin_bit_cast(f16x8_t, u4{x[0], x[1], x[2], x[3]}), to, 0, 0, 0);
-                    });
+                    },
+                    terms);
             }
         }
         if constexpr (P > 128) next_pair(it + L::DEPTH);

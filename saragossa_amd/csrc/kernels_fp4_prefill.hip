@@ -492,23 +492,27 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int d = (pp * HALVES + half) * 2 + h, it = step * PAGES + d, e = entry(it);
-            uint32_t ph[TILES][2], pl[TILES][2];
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const f16x2_t a16 = __builtin_bit_cast(f16x2_t, hi4[t][2 * h + i]), b16 = __builtin_bit_cast(f16x2_t, lo4[t][2 * h + i]);
-                    const float x = ((float)a16[0] + (float)b16[0]) * P_SCALE, y = ((float)a16[1] + (float)b16[1]) * P_SCALE;
-                    ph[t][i] = bf16_pair(x, y);
-                    pl[t][i] = bf16_pair(x - __uint_as_float(ph[t][i] << 16), y - __uint_as_float(ph[t][i] & 0xffff0000u));
-                }
-            }
             const int pos = entry_pos<RING>(c, e) + j * 4, lo = max(wg_ws_lo, entry_lo<RING>(c, e)), hi = min(wg_lim_hi, entry_hi<RING>(c, e));
             uint32_t keep = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (it < n_it && pos + i >= lo && pos + i <= hi) keep |= 255u << (8 * i);
             const uint8_t *at = pool_of(it, true) + (uint64_t)(uint32_t)(RING ? fp4_ring_page(a, c, e) : (int)entry_place<false>(a, c, e)) * page_bytes;
+            uint32_t terms[TILES][3][2]; // of 8 bits each, which leave 2^-24 of a weight; the least first
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f16x2_t a16 = __builtin_bit_cast(f16x2_t, hi4[t][2 * h + i]), b16 = __builtin_bit_cast(f16x2_t, lo4[t][2 * h + i]);
+                    float x = ((float)a16[0] + (float)b16[0]) * P_SCALE, y = ((float)a16[1] + (float)b16[1]) * P_SCALE;
+#pragma unroll
+                    for (int k = 2; k >= 0; --k) {
+                        terms[t][k][i] = bf16_pair(x, y);
+                        x -= __uint_as_float(terms[t][k][i] << 16);
+                        y -= __uint_as_float(terms[t][k][i] & 0xffff0000u);
+                    }
+                }
+            }
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
                 if (__builtin_amdgcn_readfirstlane((int)far_of[((step & 1) * PAGES + d) * PARTS + part]) != step + 1) continue;
@@ -528,11 +532,12 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                         const u4 second = {__builtin_amdgcn_perm(c1, c0, 0x07060302u), __builtin_amdgcn_perm(c3, c2, 0x07060302u), 0, 0};
 #pragma unroll
                         for (int t = 0; t < TILES; ++t) {
-                            const bf16x8_t xh = __builtin_bit_cast(bf16x8_t, u4{ph[t][0], ph[t][1], 0, 0}), xl = __builtin_bit_cast(bf16x8_t, u4{pl[t][0], pl[t][1], 0, 0});
-                            o[t][2 * grp] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), xl, o[t][2 * grp], 0, 0, 0);
-                            o[t][2 * grp] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), xh, o[t][2 * grp], 0, 0, 0);
-                            o[t][2 * grp + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, second), xl, o[t][2 * grp + 1], 0, 0, 0);
-                            o[t][2 * grp + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, second), xh, o[t][2 * grp + 1], 0, 0, 0);
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {
+                                const bf16x8_t x = __builtin_bit_cast(bf16x8_t, u4{terms[t][k][0], terms[t][k][1], 0, 0});
+                                o[t][2 * grp] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), x, o[t][2 * grp], 0, 0, 0);
+                                o[t][2 * grp + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, second), x, o[t][2 * grp + 1], 0, 0, 0);
+                            }
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     }

@@ -172,3 +172,40 @@ def test_many_far_keys_behind_one_large_one_are_counted(state, dims, shape):
         want = far / (1 + far)
         assert np.abs(got[i] - want).max() <= (row[:n + i + 1] >= 4).sum() * 2.0 ** -32 + 1.4e-4 * want, i
     kv.close()
+
+
+@pytest.mark.parametrize("dims", [(32, 8, 128), (16, 2, 256), (8, 2, 64), (8, 2, 512)], ids=str)
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("power", [0, 60, -60])
+def test_weights_are_as_exact_for_values_that_half_precision_does_not_have(state, dims, call, power):
+    """Two rows have weights to speak of, and the one of less weight values: a context is that row's weight times its values, which are 2^power times
+    small ones. (The largest weight is a power of two, whose terms are exact.)
+
+    Relative to itself it may be off by the score's four roundings (2 * 4 * 2^-24 of 1 / log2(e) at most), an exponential either way, 2^-22
+    each, the weight as terms, 2^-22, and the sum, the quotient and the products' sums, 6 * 2^-24. Streaming chunks of heads up to 128 dims hold a
+    weight in two terms of bf16 against such values: a rest of 2^-8 at most whose step is 2^-16, 2^-17."""
+    m, run, env = CALLS[call]
+    heads, kv_heads, hd = dims
+    n = 200
+    rng = np.random.default_rng(hd)
+    k = np.zeros((n, kv_heads, hd), np.float32)
+    k[:, :, 5] = -64.0  # no weight
+    k[0, :, 5], k[1, :, 5] = 1.0, 0.0
+    v = np.zeros((n, kv_heads, hd), np.float32)
+    v[1] = rng.choice([-6.0, -2.0, 1.0, 3.0, 4.0, 6.0], (kv_heads, hd)) * 2.0 ** power
+    q = np.zeros((m, heads, hd), np.float32)
+    q[:, :, 5] = rng.uniform(0.8, 2.0, (m, heads)) * np.sqrt(hd) / 1.4426950408889634
+    k, v2, q = k.reshape(n, -1), v.reshape(n, -1), q.reshape(m, -1)
+    kv = _layer_of(state, rng, dims, n, 0)
+    kv.seed(k[:n - m], v2[:n - m], n - m)
+    with _env(**env):
+        got = run(kv, k[n - m:], v2[n - m:], q)
+    weight = 1.0 / (1.0 + np.exp(q.reshape(m, heads, hd)[:, :, 5].astype(np.float64) / np.sqrt(hd)))
+    want = (weight[:, :, None] * np.repeat(v[1].astype(np.float64), heads // kv_heads, 0)[None]).reshape(m, -1)
+    tol = 2 * 4 * 2.0 ** -24 * 0.7 + 3 * 2.0 ** -22 + 6 * 2.0 ** -24
+    if power and call == "streaming chunk" and hd <= 128:
+        tol += 2.0 ** -17
+    else:
+        assert tol < 1.5e-6
+    assert (np.abs(got / want - 1.0) <= tol).all(), np.abs(got / want - 1.0).max()
+    kv.close()
