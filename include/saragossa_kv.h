@@ -95,7 +95,7 @@ size_t skv_sdpa_2pass_blocks(size_t len);         /* utils.rs:282-286 */
 /* Rows below which this library never splits the context of a decode launch: RETI_RUST_SDPA_2PASS_MIN_LEN
  * when it is set (the reference's parse, default 2048 when unparsable), and then it splits from there on; else 128.
  * While neither it nor SKV_DECODE_WGS, SKV_PREFILL_WGS, SKV_DECODE_MIN_PAGES or SKV_DECODE_WAVES is set, contexts that are
- * faster whole stay so for longer: steps of 4-bit layers up to 512 rows (heads up to 64, 32 dims 640, 768, of 129 to 256 320, above 128; in batches up to twice as many, chunks of few rows as many and more), steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
+ * faster whole stay so for longer: steps of 4-bit layers up to 512 rows (heads up to 64, 32 dims 640, 768, of 129 to 256 320, above 128; in batches, of which all or none, up to twice as many, chunks of few rows as many and more), steps of bf16 layers up to 384 rows (heads of 97 to 128 dims 256, of 129 to 256 160), in
  * batches further the more sequences and kv heads they have (16 sequences of 8 kv heads 784, 656, 416), chunks of up to some
  * hundred rows up to 400 to 1500. The reference's
  * own default (2048, utils.rs:270-278) is what skv_flag_sdpa_2pass_min_len reports; it was tuned
@@ -181,10 +181,12 @@ int32_t skv_ctx_synchronize(skv_ctx *ctx);
  * room for pages of kv_heads * P * 32 bytes per tensor, P = head_dim rounded up to a power of two) or
  * SKV_DTYPE_F32 (rows verbatim; pages twice the bytes), or SKV_DTYPE_FP4: per row and 32 dims of a head (a group;
  * a head's last one may be shorter) a power 2^e and the dims as codes e2m1, 4 bits each, 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with
- * a sign, times it: 4.25 bits a value, 17 bytes where bf16 has 64. e is the smallest in [-125, 125] with max |x| <= 7 * 2^e, a
- * value the nearest code times 2^e, ties to the even code, off by at most 2^e, which is between 1/7 and 2/7 of the group's largest
- * value. A group that holds a NaN or an infinity reads back as NaN, and is NaN to every query that attends it. Values
- * read back are exact in bf16. head_dim up to 512 in all. Every
+ * a sign, times it: 4.25 bits a value, 17 bytes where bf16 has 64. e is the smallest in [-125, 125] with max |x| <= 7 * 2^e (125 above
+ * 7 * 2^125), a value the nearest code times 2^e, ties to the even code, off by at most 2^e, which is between 1/7 and 2/7 of the group's largest
+ * value; at the ends of f32 by more: values above 7 * 2^125 become 6 * 2^125, groups of at most 3.5 * 2^-125 have steps of 2^-126. A
+ * group that holds a NaN or an infinity reads back as NaN, and is NaN to every query that attends it. Values
+ * read back are exact in bf16. Attention takes queries to 2^-24 of the largest of their 32 dims and weights to 2^-22 of themselves
+ * or 2^-32 of the largest. head_dim up to 512 in all. Every
  * entry point below serves all three; where they differ it says so. */
 int32_t skv_layer_create(skv_ctx *ctx, size_t capacity, size_t q_heads, size_t kv_heads,
                          size_t head_dim, int32_t dtype, size_t window, skv_layer **out);

@@ -245,12 +245,13 @@ hipError_t launch_load_fp4(const GatherArgs &a, hipStream_t s) {
 //
 // S^T = K . Q^T takes the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4 with K as e2m1 (a lane's 16 bytes are a row's 32 dims of
 // a group, its power a byte of its own) and the queries, times log2(e) / sqrt(head_dim), as five terms in e2m3 with a power a group and term:
-// digits of base 32 of the values as whole numbers of 25 bits, off by at most 2^-24 of the group's largest value. Five such products of 128
+// digits of base 32 of the values as whole numbers of 25 bits, off by at most 2^-24 of the group's largest value (as exact as products in 32 bits, but
+// where the keys are small in a dim of the queries some thirty times the others: at 100 times 2.7e-6 off, at 1000 2.3e-5). Five such products of 128
 // dims take 80 cycles, two of bf16 (eight instructions of 32 dims, for queries of 16 bits) 128, and the codes would have to be converted.
 // O^T += V^T . P^T sums over keys, whose powers differ, so V is converted to f16 (exact, but for powers that f16 does not have, see fp4_far) in
 // registers, per page and group of dims four conversions, four scales and four byte selections for eight values a lane, and P is two f16
 // terms; a pair of pages is the 32 keys of v_mfma_f32_16x16x32_f16. A pair with other powers is multiplied in bf16, P in three terms (chunks of heads to 128 dims: two).
-// Contexts are 2e-7 from 64 bits (2-norm, relative), 3e-7 over 32768 rows; four terms and two bf16 ones left 2.6e-6, for 3 to 7 % less time.
+// Contexts are 2e-7 from 64 bits (2-norm, relative), 3e-7 over 32768 rows; four terms and two bf16 ones left 2.6e-6, for 4 to 10 % less time.
 //
 // What bounds it: over long contexts memory, 34.8 MB of 32000 rows of q32/kv8/hd128 in 14.6 us with the merge (a bf16 layer 24.9), 69.6 of
 // q16/kv8/hd256 in 20.2 (45.1); over short ones the chain of table, pages, products, states and a second launch: 600 to 2000 rows 7.6 and
@@ -916,7 +917,7 @@ __device__ __forceinline__ void fp4_attention_body(const DecodeArgs &a, const Ch
 
 template <int P, int WAVES, bool MQ, bool RING, bool ROWS, bool PRE>
 // (streaming chunks of heads up to 128 dims: registers for two workgroups on a compute unit. 256 rows over 2000 of q32/kv8/hd128 29.2 us, 32.9 with
-// registers for one.)
+// registers for one, although at 128 dims 7 or 8 are then spilled, and a wait for one reloaded among the pages is a wait for their copies too.)
 __global__ __launch_bounds__(WAVES * 64, MQ && !ROWS && P <= 128 ? 4 : 1) void fp4_attention_kernel(DecodeArgs a, ChunkPages c) {
     fp4_attention_body<P, WAVES, MQ, RING, ROWS, PRE>(a, &c, blockIdx.x, blockIdx.y, blockIdx.z);
 }

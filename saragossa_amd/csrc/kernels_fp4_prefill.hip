@@ -60,8 +60,9 @@ __device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
 // slots attend and others do not (a row behind theirs) is converted as if its power were 1, and the slots that attend it get their NaN in a path
 // of its own. Pages with powers that f16 does not have are converted to zeros and added in bf16, from memory, behind the pair's products.
 //
-// What bounds it: over long contexts the matrix pipe, 512 rows over 32768 of q16/kv2/hd256 in 358 us (770 TFLOP/s of the products asked for, which take
-// 1.63 times their time at the bf16 rate: 1250, what a large bf16 product reaches; a bf16 layer 409); over short ones its start, at head_dim 128 3 us until the queries are
+// What bounds it: over long contexts the products, 512 rows over 32768 of q16/kv2/hd256 in 358 us (770 TFLOP/s of those asked for, which take
+// 1.63 times their time at the bf16 rate: 1250, what a large bf16 product reaches; a bf16 layer 409). The matrix pipe is busy 55 % of the cycles: V of the
+// next step is converted between a step's last products and its barrier, where both wavefronts of a SIMD stand. Over short contexts its start, at head_dim 128 3 us until the queries are
 // converted, 2 until the first V is, and 3 at the end: 512 rows over 0, 1024 of q32/kv8/hd128 18.1, 30.6 (16.5, 30.3).
 // ------------------------------------------------------------------------------------
 template <int P, int WAVES, int HALVES>

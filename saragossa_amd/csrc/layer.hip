@@ -324,7 +324,7 @@ bool takes_f32_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
 // one has no prologue to speak of and converts V anew for every 16 slots; the other's start is the queries' conversion (3 us at
 // head_dim 128, 5 at 256). From 193 workgroups of 64 slots on that needs neither splits nor a merge and is the faster one nearly everywhere. Over 2340
 // chunks of 4 to 1024 rows in nine geometries, on layers in no cache, kernel and shape chosen are 0.6 % slower than the best on the
-// average, 30 % at most. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
+// average, 32 % at most. Streaming / the chunk kernel, in us, with the (16 slots, page) pairs walked in thousands: q32/kv8/hd128, 128 rows over 2000 (34)
 // 18.4/24.7, 256 (70) 29.0/32.1, 64 over 8000 (65) 31.4/29.2, 512 over 512 (49, 256 workgroups) 27.4/24.3; q16/kv2/hd256, 64 over 8192 (33)
 // 32.3/37.1, 128 (66) 49.8/49.5, q16/kv8/hd256, 256 over 8000 (131) 81.6/78.4; q8/kv2/hd512 loses in the mean from 16 on. 16 rows, stored by the
 // streaming launch or by one of their own: q16/kv1/hd128 over 32000, 64000, 128000 (32, 64, 128) 21.0/22.4, 32.2/28.6, 52.9/42.3, q8/kv2/hd512 over 32000 (16)
@@ -340,7 +340,9 @@ bool takes_fp4_chunk_kernel(const Geom &g, size_t n_queries, size_t n_pages) {
 // more slots, narrower ones fill the device sooner, and where the causal triangle is most of the work (`own`) they also share it out more
 // evenly. Lines in the same pairs. 64 / 128 / 256 slots, in us: q32/kv8/hd128, 512 rows over 0 (16) 18.1/27.1/34.7, over 4700 (313)
 // 75.5/75.4/80.1; q32/kv8/hd64, 699 over 4394 112.8/97.4/89.7 (128 slots: 176 workgroups for 256 compute units); q32/kv8/hd128, 2026 over
-// 2682 224/183/200; q16/kv2/hd256, 512 over 0 30.3/34.3, 4096 71.8/72.1, q16/kv8/hd256, 3929 over 1284 363/303.
+// 2682 224/183/200; q16/kv2/hd256, 512 over 0 30.3/34.3, 4096 71.8/72.1, q16/kv8/hd256, 3929 over 1284 363/303. The lines are fitted to the same sweep:
+// they go up and down with the rounds of 256 compute units that a shape's workgroups are (one round of 64 slots, 193 to 256 workgroups, holds out longest
+// against 128, which then leave half of the device idle), and single shapes between the geometries lose up to 32 %.
 TileShape fp4_chunk_shape(const Geom &g, size_t n_queries, size_t n_pages) {
     if (g.P > 256) return TileShape::one_tile;
     const long knob = tuning().prefill_tiles2_min_pages;
@@ -1684,8 +1686,8 @@ static int32_t ring_chunk(skv_layer *L, hipStream_t s, const float *q, const flo
 }
 
 // The same on a 4-bit ring layer. Up to a ring's rows go into the ring at once, by a launch that copies the pages they go into to the scratch
-// as they were: a launch less, and every row is quantised once (512 rows of q16/kv8/hd256 on a ring of 1056 rows 36.8 us
-// against 39.2, 128 rows 20.1 against 22.3, before the queries' fifth term). More of them overwrite each other, so those lie in the scratch themselves until all are attended.
+// as they were: a launch less (2.2 to 2.4 us of 128 and 512 rows of q16/kv8/hd256 on a ring of 1056), and every row is quantised once. More of them
+// overwrite each other, so those lie in the scratch themselves until all are attended.
 static int32_t ring_chunk_fp4(skv_layer *L, hipStream_t s, const float *q, const float *k, const float *v, size_t c, float *out) {
     const Geom &g = L->g;
     const size_t base = L->len, ring_pages = (size_t)g.ring_rows / 16;
