@@ -186,7 +186,7 @@ int32_t skv_ctx_synchronize(skv_ctx *ctx);
  * value; at the ends of f32 by more: values above 7 * 2^125 become 6 * 2^125, groups of at most 3.5 * 2^-125 have steps of 2^-126. A
  * group that holds a NaN or an infinity reads back as NaN, and is NaN to every query that attends it. Values
  * read back are exact in bf16. Attention takes queries to 2^-24 of the largest of their 32 dims and weights to 2^-22 of themselves
- * or 2^-32 of the largest. head_dim up to 512 in all. Every
+ * or 2^-33 of the largest. head_dim up to 512 in all. Every
  * entry point below serves all three; where they differ it says so. */
 int32_t skv_layer_create(skv_ctx *ctx, size_t capacity, size_t q_heads, size_t kv_heads,
                          size_t head_dim, int32_t dtype, size_t window, skv_layer **out);

@@ -112,8 +112,8 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t power) {
 }
 
 // V as f16, at 2^-8 of its value, against probabilities at 2^8 of theirs: exact for powers of 2^-15 to 2^16 (codes are multiples of 1/2 up to 6, f16's
-// steps 2^-24, its largest 65504), and two f16 terms hold a probability to 2^-22 of itself, or 2^-33 of the largest (of chunks of many rows 2^-32, see
-// fp4_chunk_kernel), where two bf16 terms hold 2^-17, three 2^-24.
+// steps 2^-24, its largest 65504), and two f16 terms hold a probability to 2^-22 of itself, or 2^-33 of the largest,
+// where two bf16 terms hold 2^-17, three 2^-24.
 // Four rows' powers, those above and below it at 255 or below 112: bits in `far`.
 constexpr int V_SHIFT = 8;
 constexpr float P_SCALE = 1.0f / 256.0f; // of the sums of probabilities

@@ -51,9 +51,9 @@ __device__ __forceinline__ float32_t from_fp6(u6 codes, float scale) {
 // wavefront, in the order of the operands of v_mfma_f32_16x16x32_f16 over a pair of pages. Per pair of pages and tile the products take 160
 // + 256 cycles of the matrix pipe at 128 dims (two bf16 terms of the queries against K in bf16: 256 + 256).
 // Per pair: S^T of the next pair with the exponentials and the two f16 terms of this pair's probabilities between its products, then O^T of this
-// pair. The softmax runs in base 2 against a base that a slot's largest score is 7 to 11 above, and that moves only when one passes that: weights are
-// held to 2^-32 of the largest at least (f16's steps end at 2^-24), V being 2^-8 times itself. The score accumulators start at minus the base (see
-// prefill_tile_kernel).
+// pair. The softmax runs in base 2 against a base that a slot's largest score is 4 to 8 above, and that moves only when one passes that. As terms, weights are 2^4
+// times that and so held to 2^-33 of the largest (f16's steps end at 2^-24); with a base further down instead, scores round in larger steps (contexts 1.5 times
+// as far from 64 bits). V is 2^-8 times itself. The score accumulators start at minus the base (see prefill_tile_kernel).
 // With HALVES = 2 (or 4) the wavefronts are parts that hold the same slots and take the page pairs in turn; their states join through LDS.
 //
 // Keys that no slot of the workgroup attends have their powers set to 1 when V is converted: 0 x NaN is NaN. A row that is NaN and that some
@@ -315,9 +315,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     convert_v(0);
 
     float4_t o[TILES][NT], neg_m[TILES];
-    // a score whose bits reach thr moves the base, to 7 under it: any more than 11 above the base, or, of a slot without a key so far, whatever it
-    // is. (7 and not 8, which from 2^27 on, where a step of f32 is 16, would be 16 half of the time: 2^16 is more than f16 has.)
-    constexpr int UNSEEN = INT32_MIN, SEEN = 0x41300001;
+    // a score whose bits reach thr moves the base, to 4 under it: any more than 8 above the base, or, of a slot without a key so far, whatever it is
+    constexpr int UNSEEN = INT32_MIN, SEEN = 0x41000001;
     float m_base[TILES], l_run[TILES];
     int thr[TILES];
 #pragma unroll
@@ -372,7 +371,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 const float mx = fmaxf(fmaxf(fmaxf(sa[t][0], sa[t][1]), fmaxf(sa[t][2], sa[t][3])), fmaxf(fmaxf(sb[t][0], sb[t][1]), fmaxf(sb[t][2], sb[t][3])));
                 const float top = rows_max(mx); // of the slot, relative to its base
                 const bool unseen = thr[t] < 0;
-                const float d = top > (unseen ? -INFINITY : 11.0f) ? top - 7.0f : 0.0f;
+                const float d = top > (unseen ? -INFINITY : 8.0f) ? top - 4.0f : 0.0f;
                 const float alpha = unseen ? 1.0f : fast_exp2(-d);
                 m_base[t] += d;
                 neg_m[t] = float4_t{-m_base[t], -m_base[t], -m_base[t], -m_base[t]};
@@ -394,6 +393,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     // splits those of scores q - 2 and q - 1
     float pr[TILES][2], prev[TILES];
     uint32_t hi4[TILES][4], lo4[TILES][4];
+    constexpr float RAISED = 16.0f; // of weights as terms: the largest is then 2^8 to 2^12, a rounding to f16's last step 2^-33 of it at most
     auto prob_step = [&](int q) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
                 l_run[t] += prev[t];
                 pr[t][e & 1] = prev[t];
                 if (e & 1) {
-                    f16_terms(pr[t][0], pr[t][1], hi4[t][e >> 1], lo4[t][e >> 1]);
+                    f16_terms(pr[t][0] * RAISED, pr[t][1] * RAISED, hi4[t][e >> 1], lo4[t][e >> 1]);
                 }
             }
             if (q < 8) prev[t] = fast_exp2(q < 4 ? sa[t][q & 3] : sb[t][q & 3]);
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_chunk_kernel(DecodeArgs a, Chu
     const bool vec_ok = (g.head_dim & 3) == 0 && (a.splits_total > 1 || (reinterpret_cast<uintptr_t>(a.out) & 15) == 0);
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-        const float l = rows_sum(l_run[t]) * P_SCALE;
+        const float l = rows_sum(l_run[t]) * (RAISED * P_SCALE);
         const int slot = wg_slot0 + (tw * TILES + t) * 16 + n;
         if (!t_on[t] || slot >= n_slots) continue;
         float *dst;
