@@ -257,28 +257,30 @@ def _run_evict(s):
 
 
 def _linear_pointers(s):
-    case, rows, stride = s["case"], s["qkv"].shape[1], s["qkv"].shape[2] * 4
-    keys, decays = case["k_heads"] * case["k_dim"] * 4, case["v_heads"] if case["per_token"] else 0
-    at, g, old, new, out = (s[x].data_ptr() for x in ("qkv", "g", "state", "new", "out"))
-    steps = [rows * stride] + [s[x][0].numel() * 4 for x in ("g", "state", "new", "out")]
+    case, stride = s["case"], s["qkv"].shape[2] * 4
+    base, keys = s["qkv"].data_ptr(), case["k_heads"] * case["k_dim"] * 4
+    decays = case["v_heads"] if case["per_token"] else 0
     for li in range(case["layers"]):
-        yield (at, stride // 4, at + keys, stride // 4, at + 2 * keys, stride // 4, g, decays), old, new, out
-        at, g, old, new, out = (x + step for x, step in zip((at, g, old, new, out), steps))
+        at = base + li * s["qkv"].shape[1] * stride
+        yield li, at, at + keys, at + 2 * keys, stride // 4, s["g"][li].data_ptr(), decays
 
 
 def _run_linear_rows(s):
-    stream, op, n = _stream(), s["op"], s["out"].shape[1]
-    for rows, old, new, out in _linear_pointers(s):
-        op.encode_rows(stream, *rows, n, old, new, out)
-    return [s["out"], s["new"]]
+    stream, op, out = _stream(), s["op"], s["out"]
+    for li, q, k, v, stride, g, decays in _linear_pointers(s):
+        op.encode_rows(stream, q, stride, k, stride, v, stride, g, decays, out.shape[1], s["state"][li].data_ptr(),
+                       s["new"][li].data_ptr(), out[li].data_ptr())
+    return [out, s["new"]]
 
 
 def _run_linear_step(s):
-    stream, op, seqs = _stream(), s["op"], s["case"]["seqs"]
+    stream, op, out, seqs = _stream(), s["op"], s["out"], s["case"]["seqs"]
     size = s["state"][0, 0].numel() * 4
-    for rows, old, new, out in _linear_pointers(s):
-        op.encode_step(stream, *rows, [old + i * size for i in range(seqs)], [new + i * size for i in range(seqs)], out)
-    return [s["out"], s["new"]]
+    for li, q, k, v, stride, g, decays in _linear_pointers(s):
+        old, new = s["state"][li].data_ptr(), s["new"][li].data_ptr()
+        op.encode_step(stream, q, stride, k, stride, v, stride, g, decays, [old + i * size for i in range(seqs)],
+                       [new + i * size for i in range(seqs)], out[li].data_ptr())
+    return [out, s["new"]]
 
 
 # ---- plain forms -------------------------------------------------------------------------
