@@ -523,8 +523,8 @@ size_t skv_linear_state_bytes(const skv_linear *linear);
  * rows, null = zeros (nothing has come before); new_state_dev receives the one behind them and may be
  * state_dev. With another buffer the old state stays, to go back to from a draft that is not accepted. The outputs and the new state may lie
  * over no other argument (SKV_ERR_DIMENSION). More than 128 rows: with scratch as a prefill chunk's. A v that is infinite or NaN makes its
- * dim of the outputs and the state infinite or NaN from its token on, and nothing else. More than 8 rows are taken in chunks of 32, whose factors are held to 22 bits (f32's sums: outputs 1e-7 off), or to
- * 2^-37 of the largest v of their dim, or weighted k, in the chunk. */
+ * dim of the outputs and the state infinite or NaN from its token on, and nothing else. More than 8 rows are taken in chunks of 32 on the matrix cores, every factor with its 24 bits (what of it
+ * lies below 2^-126 may count as 0; |x| up to 3.38e38), sums in f32. */
 int32_t skv_linear_rows_device(skv_linear *linear, skv_stream stream, const float *q_dev, size_t q_stride,
                                const float *k_dev, size_t k_stride, const float *v_dev, size_t v_stride,
                                const float *log_decay_dev, size_t decay_stride, size_t n_rows, const float *state_dev,

@@ -219,33 +219,24 @@ hipError_t launch_linear_recurrent(const LinearRows &rows, const float *before, 
 // 16 columns of it are the operand of S^T q as they lie, which fixes the order in which every operand counts its contraction: a lane's eight
 // are 4g .. 4g + 3 and 16 + 4g .. of 32, g = lane / 16.
 //
-// Factors are two f16 terms each, 22 bits of what they stand for, three products (the fourth is below 2^-23). f16 has no range to speak of, so
-// every factor is divided by a power of two: a token's q, a token's k (for the scores), a query's 16 weights by one that makes the largest of them one
-// of 2^14 .. 2^15; the weighted k of the chunk by one, 2^xk, and a column of v by another, 2^xv, that leave at most 2^13 and 2^12 of them; and the
-// state's column is held in units of 2^(xk + xv), u for short, those of the products that are added to it, so that a chunk
-// costs it one operation: xv is chosen so that the column, faded, is below 2^30 in its new units, as the sum of the 32 products is, and
-// 2^-16 of the state is the next chunk's operand. What is 2^-25 of its group's largest (a token's 2^-28) still has its 11 bits, and below that an
-// error of 2^-37 of that largest one is left. u falls by at most 2^100 a chunk.
+// Every factor is three bf16 terms, which are it exactly (each leaves at most 2^-8 of what it stands for), and a product six: the three smallest of the
+// nine are below 2^-23 together. bf16 has f32's range, so no factor has units that another one could spoil: a large v, k or row of the
+// state leaves what lies beside it as exact as it was, and small factors have all their bits (a term below 2^-126 may count as 0). Two f16 terms in units of
+// their group's largest, three products, took about as long and held neither.
 //
 // OUT = false: the state alone, from part to part. Parts are independent but for the state in front of them: a first launch makes what each
 // adds (the first one from the caller's state), linear_scan_kernel turns that into the states, the last launch the outputs.
-//
-// 16384 tokens of 16 / 32 heads of 128 dims, 0.8 GB in and out: 122 us for the states (k and v once more, 3.3 TB/s), 10 for the scan, 240 for the
-// outputs; 2000 tokens 26, 11 and 43. Bound by the vector unit, busy for two thirds of the outputs' launch with the terms and the scales (the matrix
-// cores for a fifth), and by the chain of a chunk's three barriers: one workgroup alone takes 10000 cycles a chunk, two on a CU 12000 for both. So two workgroups
-// of eight wavefronts a CU, which 72 KB of LDS and 128 registers allow (four wavefronts of 32 columns: 298 us for the outputs).
 // ------------------------------------------------------------------------------------
 constexpr int CH = 32; // tokens of a chunk
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
-typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
-typedef __attribute__((ext_vector_type(4))) int int4_t;
-constexpr int K_LEVEL = 12, V_LEVEL = 11, STATE_LEVEL = 28, STATE_SHIFT = 16; // powers of two that the largest weighted k, v, faded state begin with; of the state as an operand
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) short short4_t;
 
 // Rows of `dims` floats, `stride` apart, of which `n` are left (a chunk's at most: within 2^31 bytes): what lies behind them reads as 0 and is not written.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_left(const float *p, int n, long stride, int dims) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, (int)((unsigned)(n - 1) * (unsigned)stride + (unsigned)dims) * 4, 0x00027000);
 }
 constexpr unsigned OUTSIDE = 0x80000000u; // an offset behind all rows, and still with a row's added
+constexpr int NO_COLUMN = 1 << 20;        // behind all of a row's
 // Columns col .. col + N - 1 of rows of n, from `at` bytes on
 template <int N, bool VEC>
 __device__ __forceinline__ auto load_cols(__amdgpu_buffer_rsrc_t rows, unsigned at, int col, int n) {
@@ -275,89 +266,78 @@ __device__ __forceinline__ void store_cols(__amdgpu_buffer_rsrc_t rows, unsigned
 }
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// Groups' largest magnitudes as bits, whose order is theirs (NaN above all)
-__device__ __forceinline__ float top_of(float top, float4_t x) {
+// Operands: eight values (half of one: four) as three terms, in the products' order
+constexpr int TERMS = 3;
+struct Half {
+    uint2 x[TERMS];
+};
+struct Operand {
+    uint4 x[TERMS];
+    __device__ __forceinline__ Half half(int i) const {
+        Half h;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, __builtin_fabsf(x[e]));
-    return top;
-}
-// The exponent x with top / 2^x one of 2^LEVEL .. 2^(LEVEL + 1); of what is below 2^-63 that of 2^-63
-template <int LEVEL>
-__device__ __forceinline__ int exponent_of(uint32_t top) { return max((int)(top >> 23), 64) - (127 + LEVEL); }
-__device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-// Largest of N neighbouring lanes, N a power of two up to 32, every one receiving it
-template <int N>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    const auto with = [&](auto ctrl) { v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xf, 0xf, true)); };
-    if constexpr (N >= 2) with(std::integral_constant<int, 0xb1>{});  // pairs exchanged
-    if constexpr (N >= 4) with(std::integral_constant<int, 0x4e>{});  // of fours
-    if constexpr (N >= 8) with(std::integral_constant<int, 0x141>{}); // eights turned round
-    if constexpr (N >= 16) with(std::integral_constant<int, 0x140>{}); // sixteens
-    if constexpr (N >= 32) {
-        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = max((uint32_t)a[0], (uint32_t)a[1]);
+        for (int p = 0; p < TERMS; ++p) h.x[p] = i == 0 ? make_uint2(x[p].x, x[p].y) : make_uint2(x[p].z, x[p].w);
+        return h;
     }
-    return v;
-}
-// of lanes l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ uint32_t sixteens_max(uint32_t v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((uint32_t)a[0], (uint32_t)a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max((uint32_t)b[0], (uint32_t)b[1]);
-}
-
-// Eight values, as they are or times `by`, as two terms in the products' order. (The mixed operations with f16 results would scale and round
-// in one, but take twice an f32 operation's time: 16384 tokens 4 % slower.)
-__device__ __forceinline__ void terms_of(float4_t a, float4_t b, uint4 &hi, uint4 &lo) {
+};
+__device__ __forceinline__ Half terms_of(float4_t v) {
     typedef __attribute__((ext_vector_type(2))) float f2;
-    typedef __attribute__((ext_vector_type(2))) _Float16 h2;
-    uint32_t h[4], l[4];
-    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    Half h;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const h2 t = __builtin_convertvector(f2{x[2 * i], x[2 * i + 1]}, h2);
-        const f2 left = {__builtin_fmaf((float)t[0], -1.0f, x[2 * i]), __builtin_fmaf((float)t[1], -1.0f, x[2 * i + 1])};
-        h[i] = __builtin_bit_cast(uint32_t, t);
-        l[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(left, h2));
+    for (int p = 0; p < TERMS; ++p) {
+        uint32_t t[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            t[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{v[2 * i], v[2 * i + 1]}, b2));
+            v[2 * i] -= __uint_as_float(t[i] << 16);
+            v[2 * i + 1] -= __uint_as_float(t[i] & 0xffff0000u);
+        }
+        h.x[p] = make_uint2(t[0], t[1]);
     }
-    hi = make_uint4(h[0], h[1], h[2], h[3]);
-    lo = make_uint4(l[0], l[1], l[2], l[3]);
+    return h;
 }
-__device__ __forceinline__ void terms_of(float4_t a, float4_t b, float by, uint4 &hi, uint4 &lo) { terms_of(a * by, b * by, hi, lo); }
-__device__ __forceinline__ float4_t products(uint4 ah, uint4 al, uint4 bh, uint4 bl, float4_t acc) {
-    const f16x8_t a = __builtin_bit_cast(f16x8_t, ah), b = __builtin_bit_cast(f16x8_t, bh);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, al), b, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8_t, bl), acc, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
+__device__ __forceinline__ Operand terms_of(float4_t a, float4_t b) {
+    const Half l = terms_of(a), h = terms_of(b);
+    Operand o;
+#pragma unroll
+    for (int p = 0; p < TERMS; ++p) o.x[p] = make_uint4(l.x[p].x, l.x[p].y, h.x[p].x, h.x[p].y);
+    return o;
+}
+// f(term of a, term of b), the smallest first
+template <class F>
+__device__ __forceinline__ void pairs(F f) {
+    f(2, 0), f(0, 2), f(1, 1), f(1, 0), f(0, 1), f(0, 0);
+}
+__device__ __forceinline__ float4_t products(const Operand &a, const Operand &b, float4_t acc) {
+    pairs([&](int p, int q) __attribute__((always_inline)) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a.x[p]), __builtin_bit_cast(bf16x8_t, b.x[q]), acc, 0, 0, 0);
+    });
+    return acc;
 }
 // of half an operand: 16 of the 32
-__device__ __forceinline__ float4_t products(uint2 ah, uint2 al, uint2 bh, uint2 bl) {
-    const f16x4_t a = __builtin_bit_cast(f16x4_t, ah), b = __builtin_bit_cast(f16x4_t, bh);
-    float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    acc = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, al), b, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x16f16(a, __builtin_bit_cast(f16x4_t, bl), acc, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, acc, 0, 0, 0);
+__device__ __forceinline__ float4_t products(const Half &a, const Half &b, float4_t acc) {
+    pairs([&](int p, int q) __attribute__((always_inline)) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a.x[p]), __builtin_bit_cast(short4_t, b.x[q]), acc, 0, 0, 0);
+    });
+    return acc;
 }
 
 // W wavefronts, 16 v dims each.
 template <int DK, int W, bool OUT>
 struct LinearLds {
     static constexpr int KK = DK / 32, VB = 16 * W;
-    uint4 kt_hi[DK / 16][64], kt_lo[DK / 16][64]; // e^{b_31 - b_j} k_j, rows are k dims
-    uint4 vt_hi[W][64], vt_lo[W][64];             // v_j, rows are v dims
-    uint4 q_hi[OUT ? 2 : 0][KK][64], q_lo[OUT ? 2 : 0][KK][64], k_hi[OUT ? 2 : 0][KK][64], k_lo[OUT ? 2 : 0][KK][64];
-    uint2 p_hi[OUT ? 3 : 0][64], p_lo[OUT ? 3 : 0][64]; // weights, (keys 0, queries 0), (0, 1), (1, 1)
-    int xq[OUT ? CH : 0], xk[OUT ? CH : 0], xp[OUT ? 3 : 0][16]; // exponents: of tokens, of the weights' queries
-    alignas(16) int u[2][VB], xv[VB]; // of the state's columns, in front of the chunk and behind it (by its parity), of v's columns
-    alignas(16) int faded[VB];        // u for which the state, not faded yet, is one of 2^STATE_LEVEL .. 2^(STATE_LEVEL + 1)
-    uint32_t k_top;       // the largest weighted key that is finite
+    uint4 kt[TERMS][DK / 16][64];                // e^{b_31 - b_j} k_j, rows are k dims
+    uint4 vt[TERMS][W][64];                      // v_j, rows are v dims
+    uint4 q[OUT ? TERMS : 0][2][KK][64];         // q_i, rows are tokens
+    uint2 p[OUT ? TERMS : 0][3][64];             // weights, (keys 0, queries 0), (0, 1), (1, 1)
     alignas(16) double b[2][CH];
     float from[2][CH], to[2][CH]; // e^{b_i}, e^{b_31 - b_j}
     float whole[2];               // e^{b_31}
     int bad[2][VB];               // the first token whose v is not finite there (CH = none)
     int any_bad[2];
 };
+static_assert(2 * sizeof(LinearLds<128, 8, true>) <= 160 * 1024, "two workgroups on a CU");
 
 struct LinearChunkArgs {
     LinearRows r;
@@ -407,19 +387,10 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
 #pragma unroll
         for (int i = 0; i < DT; ++i) p[i * 64] = S[i];
     };
-    // the column's units, and what the next chunk may choose them by
-    const auto note = [&](int u) __attribute__((always_inline)) {
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) top = top_of(top, S[i]);
-        const int x = (int)(sixteens_max(__float_as_uint(top)) >> 23) - 127 - STATE_LEVEL + u;
-        if (g4 == 0) m.faded[wave * 16 + n16] = x;
-        return x;
-    };
-    // a chunk's decays, by the last wavefront (one without a tile of scores), asked for two chunks ahead: sums in 64 bits, what is below e^-1000
+    // a chunk's decays, by the last wavefront (one without scores), asked for two chunks ahead: sums in 64 bits, what is below e^-1000
     // counted as that (0 in 32 bits, and nothing is lost beside it). In powers of two from here on.
     double total = 0.0; // of the part
-    // Where a lane's operand of q or k lies: the sixteen of a line are turned against each other, by the unit's number, so that the threads of
+    // Where a lane's operand of q lies: the sixteen of a line are turned against each other, by the unit's number, so that the threads of
     // one row, who write the same place of sixteen lines, meet no bank twice (k dims by columns and v, four lines: by the tile's number)
     const auto unit_of = [&](int kk) { return lane ^ ((kk * 4 + g4) & 15); };
     const auto decay = [&](int c0) { return r.g[(long)min(c0 + (lane & (CH - 1)), t1 - 1) * r.g_stride + h]; };
@@ -454,8 +425,9 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
         if (lane == 0) m.whole[buf] = exp2_of(all);
     };
 
-    // Registers of the chunk on its way; what lies past the part's last token or a head's last dim is 0.
-    // Eight tokens of CW columns, k's (whole wavefronts), then v's; with eight wavefronts and tokens to load, the first four's.
+    // Registers of the chunk on its way; what lies past the part's last token or a head's last dim is 0. Columns: eight tokens of CW dims of k (whole
+    // wavefronts), then of v; with outputs and eight wavefronts the first four's. The next two, the scorers: 16 keys each, as an operand lies. The last two: eight dims
+    // of tokens of q. Four wavefronts have columns and q all, the first two of them keys too.
     constexpr bool APART = OUT && W == 8;
     constexpr int CW = !OUT && W == 8 ? 2 : 4;
     typedef __attribute__((ext_vector_type(CW))) float cols_t;
@@ -463,11 +435,11 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
     constexpr int KN = DK * 4 / CW, KI = KN < 64 ? 64 : KN;
     constexpr int ITEMS = KI + VB * 4 / CW;
     constexpr int NI = (ITEMS + CT - 1) / CT;
-    // Eight dims of a token, of q and of k; the last four of eight wavefronts' (or everyone's)
-    constexpr int UNITS = CH * DK / 8;
-    constexpr int NU = OUT ? (UNITS + 255) / 256 : 0;
-    constexpr int QAT = APART ? 0 : NI * 2 * CW; // a wavefront with columns has no tokens
-    constexpr int HELD = APART ? (NI > (NU + 1) / 2 ? NI : (NU + 1) / 2) * 8 : QAT + NU * 4;
+    constexpr int UNITS = CH * DK / 8, QT = APART ? 128 : 256; // of q, and the threads that have them
+    constexpr int NU = OUT ? (UNITS + QT - 1) / QT : 0;
+    constexpr int C_LOADS = NI * 8, K_LOADS = OUT ? KK * 2 : 0;
+    static_assert(!APART || (K_LOADS <= C_LOADS && NU * 2 <= C_LOADS));
+    constexpr int K_AT = APART ? 0 : C_LOADS * CW / 4, Q_AT = APART ? 0 : K_AT + K_LOADS, HELD = APART ? C_LOADS : Q_AT + NU * 2;
     float4_t held[HELD];
     const auto column = [&](int u, int e) __attribute__((always_inline)) {
         if constexpr (CW == 4) return held[u * 8 + e];
@@ -477,189 +449,140 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
 #pragma unroll
         for (int c = 0; c < CW; ++c) held[(u * 8 + e) * CW / 4][(e * CW + c) & 3] = x[c];
     };
-    const bool has_columns = !APART || wave < 4, has_tokens = OUT && (!APART || wave >= 4);
+    const bool has_columns = !APART || wave < 4, has_q = OUT && (!APART || wave >= 6);
+    const int jt = wave - (APART ? 4 : 0); // a scorer's keys
+    const bool scorer = OUT && jt >= 0 && jt < 2;
+    const auto unit = [&](int u) { return tid - (APART ? 384 : 0) + u * QT; }; // of q
     const auto item = [&](int u, bool &is_k, int &grp, int &col) __attribute__((always_inline)) {
         const int idx = tid + u * CT;
         is_k = wave * 64 + u * CT < KI; // uniform
         const int i = is_k ? idx : min(idx, ITEMS - 1) - KI; // (wavefronts without one of their own load the last one's, too)
-        // sixteen lanes a row, so that its bytes are asked for together; the four groups of tokens of a column look for its largest among themselves
+        // sixteen lanes a row, so that its bytes are asked for together
         grp = i >> 4 & 3, col = ((i >> 6) * 16 + (i & 15)) * CW;
         const bool mine = KN >= 64 || !is_k || col < DK;
         if (!mine) col = DK - CW;
         return mine;
     };
     // One path for all: were the loads themselves under a condition, what they bring would be moved where the conditions meet, and waited for.
-    // Eight loads at a time: an item of columns, or two units of tokens (q twice, k twice each); what a wavefront has no use for is its last one again.
-    constexpr int NG_T = (NU + 1) / 2, NG = APART ? (NI > NG_T ? NI : NG_T) : NI + NG_T;
+    // So a wavefront's part says what it reads from where in the slots that all share, in numbers: columns rows, a scorer dims, the last one (q) both.
+    // What it has no use for lies behind the rows' dims and costs no access.
     const auto fetch = [&](int c0) __attribute__((always_inline)) {
         const int left = min(t1 - c0, CH);
-        const auto qs = rows_left(qp + (long)c0 * r.q_stride, left, r.q_stride, d.k_dim), ks = rows_left(kp + (long)c0 * r.k_stride, left, r.k_stride, d.k_dim),
-                   vs = rows_left(vp + (long)c0 * r.v_stride, left, r.v_stride, d.v_dim);
+        const auto rows_of = [&](bool v, bool q) __attribute__((always_inline)) {
+            // (by masks: a choice between variables is made by their addresses, and puts them into memory)
+            const long as_v = -(long)v, as_q = ~as_v & -(long)q, as_k = ~as_v & ~as_q;
+            const long stride = (r.v_stride & as_v) | (r.q_stride & as_q) | (r.k_stride & as_k);
+            const long from = ((long)vp & as_v) | ((long)qp & as_q) | ((long)kp & as_k);
+            return rows_left(reinterpret_cast<const float *>(from) + (long)c0 * stride, left, stride, v ? d.v_dim : d.k_dim);
+        };
         const unsigned q_step = (unsigned)r.q_stride * 4u, k_step = (unsigned)r.k_stride * 4u, v_step = (unsigned)r.v_stride * 4u;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const bool columns = APART ? has_columns : g < NI;
-            bool is_k = true;
-            unsigned at_a = 0, at_b = 0; // of q or columns, of k by tokens
-            int col[2] = {0, 0}, dims = d.k_dim;
-            if (columns) {
-                int grp;
-                item(min(g, NI - 1), is_k, grp, col[0]);
-                dims = is_k ? d.k_dim : d.v_dim;
-                col[0] += is_k ? 0 : col0;
-                col[1] = col[0];
-                at_a = at_b = (unsigned)(grp * 4) * (is_k ? k_step : v_step);
-            } else if (OUT) {
-                const int idx = min((tid & 255) + (APART ? min(g, NG_T - 1) : g - NI) * 512, UNITS - 1), un = idx % (DK / 8), row = idx / (DK / 8);
-                col[0] = (un >> 2) * 32 + (un & 3) * 4;
-                col[1] = col[0] + 16;
-                at_a = (unsigned)row * q_step;
-                at_b = (unsigned)row * k_step;
-            }
-            const auto first = columns ? (is_k ? ks : vs) : qs, second = columns ? (is_k ? ks : vs) : ks;
-            const unsigned step_a = columns ? (is_k ? k_step : v_step) : q_step, step_b = columns ? (is_k ? k_step : v_step) : k_step;
-            const int TU = 256 / (DK / 8); // tokens from a thread's unit to its next one
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (!APART && g >= NI && ((g - NI) * 2 + j / 4) >= NU) continue;
-                const bool second_half = j & 2;
-                const unsigned rows = columns ? (j >> 2) * 16 + (j & 3) : NU > 1 ? (j >> 2) * TU : 0;
-                const unsigned at = (second_half ? at_b : at_a) + rows * (second_half ? step_b : step_a);
-                const auto x = second_half ? second : first;
-                const int c = col[j & 1];
-                if (CW == 4 || !(APART || g < NI)) held[APART || g < NI ? g * 8 + j : QAT + (g - NI) * 8 + j] = load_cols<4, VEC>(x, at, c, dims);
-                else set_column(g, j, load_cols<CW, VEC>(x, at, c, dims));
-            }
-        }
-    };
-    // k's columns times their decays to the chunk's end, and the largest of them
-    const auto weigh = [&](int buf) __attribute__((always_inline)) {
+        const unsigned keys_at = (unsigned)(jt * 16 + n16) * k_step;
+        const int keys_col = scorer ? g4 * 4 : NO_COLUMN;
+        const unsigned q_at = (unsigned)(unit(0) / (DK / 8)) * q_step, q_next = (unsigned)(QT * 8 / DK) * q_step; // (a thread's units are of the same dims)
+        const int q_col = has_q && unit(0) < UNITS ? (unit(0) % (DK / 8) >> 2) * 32 + (unit(0) & 3) * 4 : NO_COLUMN;
+        const unsigned per_pair = APART && has_q ? q_next : 0u;
+        const int col_pair = scorer ? 32 : 0, col_half = 16;
 #pragma unroll
         for (int u = 0; u < NI; ++u) {
             bool is_k;
             int grp, col;
             item(u, is_k, grp, col);
-            if (!is_k) continue; // uniform
-            const float4_t w0 = *reinterpret_cast<const float4_t *>(&m.to[buf][grp * 4]);
-            const float4_t w1 = *reinterpret_cast<const float4_t *>(&m.to[buf][16 + grp * 4]);
-            float top = 0.0f;
+            is_k |= !has_columns;
+            unsigned at = (unsigned)(grp * 4) * (is_k ? k_step : v_step);
+            col += is_k ? 0 : col0;
+            if constexpr (APART) {
+                at = has_columns ? at : has_q ? q_at : keys_at;
+                col = has_columns ? col : has_q ? q_col : keys_col;
+            }
+            const auto x = rows_of(!is_k, APART && has_q);
+            const int dims = is_k ? d.k_dim : d.v_dim;
+            const unsigned per_row = has_columns ? is_k ? k_step : v_step : 0u;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const cols_t x = column(u, e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
-                set_column(u, e, x);
-#pragma unroll
-                for (int c = 0; c < CW; ++c) top = __builtin_elementwise_maximum(top, __builtin_fabsf(x[c]));
+                const int s = u * 8 + e;
+                const unsigned add = (unsigned)((e >> 2) * 16 + (e & 3)) * per_row + (APART ? (unsigned)(s / 2) * per_pair : 0u);
+                const int more = APART && !has_columns ? s / 2 * col_pair + (s & 1) * col_half : 0;
+                const auto y = load_cols<CW, VEC>(x, at + add, col + more, dims);
+                if constexpr (CW == 4) held[s] = y;
+                else set_column(u, e, y);
             }
-            if (!(top < INFINITY)) { // the largest of those that are finite: a k dim that is not spoils its own row alone
-                top = 0.0f;
+        }
+        if constexpr (!APART && OUT) {
+            const auto ks = rows_of(false, false), qs = rows_of(false, true);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+            for (int s = 0; s < K_LOADS; ++s) held[K_AT + s] = load_cols<4, VEC>(ks, keys_at, keys_col + s / 2 * 32 + (s & 1) * 16, d.k_dim);
 #pragma unroll
-                    for (int c = 0; c < CW; ++c) {
-                        const float y = __builtin_fabsf(column(u, e)[c]);
-                        top = fmaxf(top, y < INFINITY ? y : 0.0f);
-                    }
-            }
-            const uint32_t all = sixteens_max(lanes_max<16>(__float_as_uint(top)));
-            if (lane == 0) atomicMax(&m.k_top, (uint32_t)__builtin_amdgcn_readfirstlane((int)all));
+            for (int s = 0; s < NU * 2; ++s) held[Q_AT + s] = load_cols<4, VEC>(qs, q_at + (unsigned)(s / 2) * q_next, q_col + (s & 1) * 16, d.k_dim);
         }
     };
     const auto stage_columns = [&](int buf) __attribute__((always_inline)) {
-        const int xk = exponent_of<K_LEVEL>(m.k_top);
 #pragma unroll
         for (int u = 0; u < NI; ++u) {
             bool is_k;
             int grp, col;
-            const bool mine = item(u, is_k, grp, col); // (lanes without a column of their own take part: they are asked across)
-            if (wave * 64 + u * CT < ITEMS) {
-                float tops[CW];
+            const bool mine = item(u, is_k, grp, col);
+            if (wave * 64 + u * CT >= ITEMS) continue; // (uniform)
+            if (is_k) { // times their decays to the chunk's end
+                const float4_t w0 = *reinterpret_cast<const float4_t *>(&m.to[buf][grp * 4]);
+                const float4_t w1 = *reinterpret_cast<const float4_t *>(&m.to[buf][16 + grp * 4]);
 #pragma unroll
-                for (int c = 0; c < CW; ++c) {
-                    tops[c] = 0.0f;
-                    if (is_k) continue; // (uniform)
+                for (int e = 0; e < 8; ++e) set_column(u, e, column(u, e) * (e < 4 ? w0[e & 3] : w1[e & 3]));
+            } else {
+                // a v that is not finite would reach the tokens in front of it through weights of 0: its dim is kept out of the
+                // products and is NaN from that token on
+                float top = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) tops[c] = __builtin_elementwise_maximum(tops[c], __builtin_fabsf(column(u, e)[c]));
-                }
-                if (!is_k) {
-                    // a v that is not finite would reach the tokens in front of it through weights of 0: its dim is kept out of the
-                    // products and is NaN from that token on
-                    float top = tops[0];
+                for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int c = 1; c < CW; ++c) top = __builtin_elementwise_maximum(top, tops[c]);
-                    if (!(top < INFINITY)) {
-                        int first[CW];
+                    for (int c = 0; c < CW; ++c) top = __builtin_elementwise_maximum(top, __builtin_fabsf(column(u, e)[c]));
+                if (!(top < INFINITY)) {
+                    int first[CW];
 #pragma unroll
-                        for (int c = 0; c < CW; ++c) first[c] = CH, tops[c] = 0.0f;
+                    for (int c = 0; c < CW; ++c) first[c] = CH;
 #pragma unroll
-                        for (int e = 7; e >= 0; --e) {
-                            cols_t x = column(u, e);
+                    for (int e = 7; e >= 0; --e) {
+                        cols_t x = column(u, e);
 #pragma unroll
-                            for (int c = 0; c < CW; ++c) {
-                                const bool bad = !(__builtin_fabsf(x[c]) < INFINITY);
-                                first[c] = bad ? (e >> 2) * 16 + grp * 4 + (e & 3) : first[c];
-                                x[c] = bad ? 0.0f : x[c];
-                                tops[c] = fmaxf(tops[c], __builtin_fabsf(x[c]));
-                            }
-                            set_column(u, e, x);
+                        for (int c = 0; c < CW; ++c) {
+                            const bool bad = !(__builtin_fabsf(x[c]) < INFINITY);
+                            first[c] = bad ? (e >> 2) * 16 + grp * 4 + (e & 3) : first[c];
+                            x[c] = bad ? 0.0f : x[c];
                         }
-#pragma unroll
-                        for (int c = 0; c < CW; ++c) atomicMin(&m.bad[buf][col + c], first[c]);
-                        m.any_bad[buf] = 1;
+                        set_column(u, e, x);
                     }
+#pragma unroll
+                    for (int c = 0; c < CW; ++c) atomicMin(&m.bad[buf][col + c], first[c]);
+                    m.any_bad[buf] = 1;
                 }
-                int x[CW];
-                if (is_k) {
+            }
 #pragma unroll
-                    for (int c = 0; c < CW; ++c) x[c] = xk;
-                } else {
-                    typedef __attribute__((ext_vector_type(CW))) int ints_t;
-                    const int fading = (int)(__float_as_uint(m.whole[buf]) >> 23 & 255) - 127 + 1;
-                    const ints_t faded = *reinterpret_cast<const ints_t *>(&m.faded[col]), before = *reinterpret_cast<const ints_t *>(&m.u[buf ^ 1][col]);
-                    ints_t units, own;
+            for (int c = 0; c < CW; ++c) {
+                const Operand x = terms_of(float4_t{column(u, 0)[c], column(u, 1)[c], column(u, 2)[c], column(u, 3)[c]},
+                                           float4_t{column(u, 4)[c], column(u, 5)[c], column(u, 6)[c], column(u, 7)[c]});
+                const int at = grp * 16 + (((col + c) ^ (col >> 4 & 3)) & 15);
+                if (KN >= 64 || mine) {
 #pragma unroll
-                    for (int c = 0; c < CW; ++c) {
-                        units[c] = xk + exponent_of<V_LEVEL>(sixteens_max(__float_as_uint(tops[c])));
-                        units[c] = min(max(max(units[c], faded[c] + fading), before[c] - 100), 300);
-                        own[c] = x[c] = units[c] - xk;
-                    }
-                    if (grp == 0) {
-                        *reinterpret_cast<ints_t *>(&m.u[buf][col]) = units;
-                        *reinterpret_cast<ints_t *>(&m.xv[col]) = own;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < CW; ++c) {
-                    uint4 hi, lo;
-                    terms_of(float4_t{column(u, 0)[c], column(u, 1)[c], column(u, 2)[c], column(u, 3)[c]},
-                             float4_t{column(u, 4)[c], column(u, 5)[c], column(u, 6)[c], column(u, 7)[c]}, power_of(-x[c]), hi, lo);
-                    const int at = grp * 16 + (((col + c) ^ (col >> 4 & 3)) & 15);
-                    if (KN >= 64 || mine) {
-                        (is_k ? m.kt_hi : m.vt_hi)[(col + c) >> 4][at] = hi;
-                        (is_k ? m.kt_lo : m.vt_lo)[(col + c) >> 4][at] = lo;
-                    }
+                    for (int p = 0; p < TERMS; ++p) (is_k ? m.kt[p] : m.vt[p])[(col + c) >> 4][at] = x.x[p];
                 }
             }
         }
     };
-    const auto stage_tokens = [&]() __attribute__((always_inline)) {
+    const auto stage_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int idx = (tid & 255) + u * 256, row = idx / (DK / 8), un = idx % (DK / 8);
-            if (UNITS % 256 == 0 || idx < UNITS) {
-                const float4_t qx[2] = {held[QAT + u * 4], held[QAT + u * 4 + 1]}, kx[2] = {held[QAT + u * 4 + 2], held[QAT + u * 4 + 3]};
-                uint4 hi, lo;
-                const int at = (un & 3) * 16 + ((row ^ un) & 15);
-                const int xq = exponent_of<14>(lanes_max<DK / 8>(__float_as_uint(top_of(top_of(0.0f, qx[0]), qx[1]))));
-                const int xk = exponent_of<14>(lanes_max<DK / 8>(__float_as_uint(top_of(top_of(0.0f, kx[0]), kx[1]))));
-                if (un == 0) m.xq[row] = xq, m.xk[row] = xk;
-                terms_of(qx[0], qx[1], power_of(-xq), hi, lo);
-                m.q_hi[row >> 4][un >> 2][at] = hi;
-                m.q_lo[row >> 4][un >> 2][at] = lo;
-                terms_of(kx[0], kx[1], power_of(-xk), hi, lo);
-                m.k_hi[row >> 4][un >> 2][at] = hi;
-                m.k_lo[row >> 4][un >> 2][at] = lo;
+            const int row = unit(u) / (DK / 8), un = unit(u) % (DK / 8);
+            if (UNITS % QT == 0 || unit(u) < UNITS) {
+                const Operand x = terms_of(held[Q_AT + u * 2], held[Q_AT + u * 2 + 1]);
+#pragma unroll
+                for (int p = 0; p < TERMS; ++p) m.q[p][row >> 4][un >> 2][(un & 3) * 16 + ((row ^ un) & 15)] = x.x[p];
             }
         }
+    };
+    const auto q_operand = [&](int it, int kk) __attribute__((always_inline)) {
+        Operand x;
+#pragma unroll
+        for (int p = 0; p < TERMS; ++p) x.x[p] = m.q[p][it][kk][unit_of(kk)];
+        return x;
     };
 
     // (everything asked for before anything is waited for: decays, the first chunk, the state)
@@ -685,21 +608,12 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
     if (wave == W - 1) decays(t0, 0, g0);
     if (tid < VB) m.bad[0][tid] = CH;
     if (tid < 2) m.any_bad[tid] = 0;
-    if (tid == 0) m.k_top = 0;
-    {
-        const int u = min(max(note(0), -100), 100);
-        const float by = power_of(-u);
-#pragma unroll
-        for (int i = 0; i < DT; ++i) S[i] *= by;
-        if (g4 == 0) m.u[1][wave * 16 + n16] = u;
-    }
     if constexpr (OUT) { // (to nowhere: as many stores behind the first chunk's loads as a chunk has behind the next one's, so that the loads can be waited for without the stores)
         const auto outs = rows_left(r.out, 1, 0, d.v_dim);
+        const float x = __int_as_float(tid);
 #pragma unroll
-        for (int it = 0; it < 2; ++it) store_cols<VEC>(outs, OUTSIDE, 0, d.v_dim, float4_t{0.f, 0.f, 0.f, 0.f});
+        for (int it = 0; it < 2; ++it) store_cols<VEC>(outs, OUTSIDE, 0, d.v_dim, float4_t{x, x, x, x});
     }
-    __syncthreads();
-    if (has_columns) weigh(0);
     __syncthreads();
     int buf = 0;
     for (int c0 = t0; c0 < t1; c0 += CH, buf ^= 1) {
@@ -707,78 +621,79 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
         // for all loads on their way
         asm("" : "+v"(tid));
         lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
+        if (has_q) stage_q();
         if (has_columns) stage_columns(buf);
-        if constexpr (OUT) {
-            if (has_tokens) stage_tokens();
-        }
         __syncthreads();
+        // (the other workgroup's wavefronts, that bring a chunk in, fill what these leave)
+        if constexpr (OUT) __builtin_amdgcn_s_setprio(2);
+        if (tid < VB) m.bad[buf ^ 1][tid] = CH; // (read last in the chunk before this one, a barrier ago)
+        if (tid == 0) m.any_bad[buf ^ 1] = 0;
+        const bool any_bad = m.any_bad[buf] != 0;
+        float4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if constexpr (OUT) {
+            if (scorer) { // both tiles of its keys, as weights into LDS
+                float4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const Operand k = terms_of(held[K_AT + 2 * kk], held[K_AT + 2 * kk + 1]);
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) s[it] = products(k, q_operand(it, kk), s[it]);
+                }
+                const double *const bj = &m.b[buf][jt * 16 + g4 * 4];
+                const double b[4] = {bj[0], bj[1], bj[2], bj[3]};
+#pragma unroll
+                for (int it = 0; it < 2; ++it) {
+                    const int i = it * 16 + n16;
+                    const double bi = m.b[buf][i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float f = exp2_of(bi - b[e]) * d.scale * s[it][e];
+                        asm("" : "+v"(f)); // (not under the condition: four waits one after the other)
+                        s[it][e] = jt * 16 + g4 * 4 + e <= i ? f : 0.0f;
+                    }
+                    const Half x = terms_of(s[it]);
+                    if (it >= jt) {
+#pragma unroll
+                        for (int p = 0; p < TERMS; ++p) m.p[p][it + jt][lane] = x.x[p];
+                    }
+                }
+            }
+        }
+        if constexpr (OUT) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const Operand x = terms_of(S[2 * kk], S[2 * kk + 1]);
+#pragma unroll
+                for (int it = 0; it < 2; ++it) o[it] = products(x, q_operand(it, kk), o[it]);
+            }
+#pragma unroll
+            for (int it = 0; it < 2; ++it) o[it] *= m.from[buf][it * 16 + n16] * d.scale;
+        }
         {
             const float x = gx;
             gx = decay(c0 + 2 * CH);
             fetch(min(c0 + CH, last_chunk));
             if (wave == W - 1 && c0 + CH < t1) decays(c0 + CH, buf ^ 1, x);
         }
-        // (the other workgroup's wavefronts, that bring a chunk in, fill what these leave: 259 -> 240 us of 16384 tokens)
-        if constexpr (OUT) __builtin_amdgcn_s_setprio(2);
-        if (tid < VB) m.bad[buf ^ 1][tid] = CH; // (read last in the chunk before this one, a barrier ago)
-        if (tid == 0) m.any_bad[buf ^ 1] = 0, m.k_top = 0;
-        const bool any_bad = m.any_bad[buf] != 0;
-        float4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        if constexpr (OUT) {
-            // scores, keys by queries: wavefronts 0, 1, 2 a tile each, (keys 0, queries 0), (0, 1), (1, 1); as weights into LDS
-            if (wave < 3) {
-                const int jt = wave == 2, it = wave != 0, i = it * 16 + n16;
-                float4_t s = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (OUT) __syncthreads(); // the weights
+        Operand v;
 #pragma unroll
-                for (int t = 0; t < KK; ++t)
-                    s = products(m.k_hi[jt][t][unit_of(t)], m.k_lo[jt][t][unit_of(t)], m.q_hi[it][t][unit_of(t)], m.q_lo[it][t][unit_of(t)], s);
-                const int4_t xk = *reinterpret_cast<const int4_t *>(&m.xk[jt * 16 + g4 * 4]);
-                const double *const bj = &m.b[buf][jt * 16 + g4 * 4];
-                const double b[4] = {bj[0], bj[1], bj[2], bj[3]}, bi = m.b[buf][i];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float f = exp2_of(bi - b[e]) * d.scale;
-                    asm("" : "+v"(f)); // (not under the condition: four waits one after the other)
-                    f = __builtin_ldexpf(s[e] * f, xk[e]);
-                    s[e] = jt * 16 + g4 * 4 + e <= i ? f : 0.0f;
-                }
-                const int x = exponent_of<14>(sixteens_max(__float_as_uint(top_of(0.0f, s))));
-                uint4 hi, lo;
-                terms_of(s, s, power_of(-x), hi, lo);
-                m.p_hi[wave][lane] = make_uint2(hi.x, hi.y);
-                m.p_lo[wave][lane] = make_uint2(lo.x, lo.y);
-                if (g4 == 0) m.xp[wave][n16] = x + m.xq[i];
-            }
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                uint4 sh, sl;
-                terms_of(S[2 * kk], S[2 * kk + 1], 1.0f / (1 << STATE_SHIFT), sh, sl);
-#pragma unroll
-                for (int it = 0; it < 2; ++it) o[it] = products(sh, sl, m.q_hi[it][kk][unit_of(kk)], m.q_lo[it][kk][unit_of(kk)], o[it]);
-            }
-#pragma unroll
-            for (int it = 0; it < 2; ++it) o[it] *= m.from[buf][it * 16 + n16] * d.scale;
-            __syncthreads(); // the weights
-        }
-        const uint4 vh = m.vt_hi[wave][lane ^ (wave & 3)], vl = m.vt_lo[wave][lane ^ (wave & 3)];
+        for (int p = 0; p < TERMS; ++p) v.x[p] = m.vt[p][wave][lane ^ (wave & 3)];
         if constexpr (OUT) {
             const int col = wave * 16 + g4 * 4;
             const auto outs = rows_left(r.out + (long)c0 * (d.v_heads * d.v_dim) + (long)h * d.v_dim, min(t1 - c0, CH), (long)d.v_heads * d.v_dim, d.v_dim);
-            const int4_t xs = *reinterpret_cast<const int4_t *>(&m.u[buf ^ 1][col]), xv = *reinterpret_cast<const int4_t *>(&m.xv[col]);
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
-                const int i = it * 16 + n16, xq = m.xq[i];
+                const int i = it * 16 + n16;
+                float4_t add = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[it][e] = __builtin_ldexpf(o[it][e], xq + STATE_SHIFT + xs[e]);
+                for (int j = 0; j <= it; ++j) {
+                    Half w;
 #pragma unroll
-                for (int jt = 0; jt <= it; ++jt) {
-                    const uint2 ph = m.p_hi[it + jt][lane], pl = m.p_lo[it + jt][lane];
-                    const float4_t add = jt == 0 ? products(make_uint2(vh.x, vh.y), make_uint2(vl.x, vl.y), ph, pl)
-                                                 : products(make_uint2(vh.z, vh.w), make_uint2(vl.z, vl.w), ph, pl);
-                    const int xp = m.xp[it + jt][n16];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[it][e] += __builtin_ldexpf(add[e], xp + xv[e]);
+                    for (int p = 0; p < TERMS; ++p) w.x[p] = m.p[p][it + j][lane];
+                    add = products(v.half(j), w, add);
                 }
+                o[it] += add;
                 if (any_bad) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -787,25 +702,20 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
                 store_cols<VEC>(outs, (unsigned)(i * (d.v_heads * d.v_dim)) * 4u, col0 + col, d.v_dim, o[it]);
             }
         }
-        const int col = wave * 16 + n16, u = m.u[buf][col];
-        const float f = any_bad && m.bad[buf][col] < CH ? __builtin_nanf("") : m.whole[buf] * power_of(m.u[buf ^ 1][col] - u);
+        const float f = any_bad && m.bad[buf][wave * 16 + n16] < CH ? __builtin_nanf("") : m.whole[buf];
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
-            const float4_t add = products(m.kt_hi[i][lane ^ (i & 3)], m.kt_lo[i][lane ^ (i & 3)], vh, vl, float4_t{0.f, 0.f, 0.f, 0.f});
+            Operand k;
+#pragma unroll
+            for (int p = 0; p < TERMS; ++p) k.x[p] = m.kt[p][i][lane ^ (i & 3)];
+            const float4_t add = products(k, v, float4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int e = 0; e < 4; ++e) S[i][e] = __builtin_fmaf(S[i][e], f, add[e]); // (one rounding a chunk: summed by the matrix instruction it was off by twice as much)
         }
-        if constexpr (!OUT) __syncthreads(); // the next chunk's decays
         if constexpr (OUT) __builtin_amdgcn_s_setprio(0);
-        note(u);
-        if (has_columns) weigh(buf ^ 1);
         __syncthreads();
     }
     if (OUT && part < a.parts - 1) return;
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[i][e] = __builtin_ldexpf(S[i][e], m.u[buf ^ 1][wave * 16 + n16]);
     if (OUT) {
         const auto rows = rows_left(a.after + state_at, d.k_dim, d.v_dim, d.v_dim);
 #pragma unroll
