@@ -230,6 +230,7 @@ hipError_t launch_linear_recurrent(const LinearRows &rows, const float *before, 
 constexpr int CH = 32; // tokens of a chunk
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) short short4_t;
+typedef __attribute__((ext_vector_type(4))) int int4_t;
 
 // Rows of `dims` floats, `stride` apart, of which `n` are left (a chunk's at most: within 2^31 bytes): what lies behind them reads as 0 and is not written.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_left(const float *p, int n, long stride, int dims) {
@@ -264,7 +265,15 @@ __device__ __forceinline__ void store_cols(__amdgpu_buffer_rsrc_t rows, unsigned
             __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)x[e]), rows, (int)(col + e < n ? (unsigned)(col + e) * 4u + at : OUTSIDE + at), 0, 0);
     }
 }
-__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
+// 2^x as m 2^n, m near 1: exact to two steps whatever x is, and no product with it leaves f32 but one that has to
+struct Power {
+    float m;
+    int n;
+};
+__device__ __forceinline__ Power power_of(double x) {
+    const double n = __builtin_fmax(__builtin_fmin(__builtin_rint(x), 4096.0), -4096.0); // (a NaN's is in m)
+    return {__builtin_amdgcn_exp2f((float)(x - n)), (int)n};
+}
 
 // Operands: eight values (half of one: four) as three terms, in the products' order
 constexpr int TERMS = 3;
@@ -332,8 +341,9 @@ struct LinearLds {
     uint4 q[OUT ? TERMS : 0][2][KK][64];         // q_i, rows are tokens
     uint2 p[OUT ? TERMS : 0][3][64];             // weights, (keys 0, queries 0), (0, 1), (1, 1)
     alignas(16) double b[2][CH];
-    float from[2][CH], to[2][CH]; // e^{b_i}, e^{b_31 - b_j}
-    float whole[2];               // e^{b_31}
+    float from_m[2][CH], to_m[2][CH]; // e^{b_i}, e^{b_31 - b_j}
+    int from_n[2][CH], to_n[2][CH];
+    Power whole[2];               // e^{b_31}
     int bad[2][VB];               // the first token whose v is not finite there (CH = none)
     int any_bad[2];
 };
@@ -345,7 +355,7 @@ struct LinearChunkArgs {
     float *after;
     float *slots;  // [parts - 1][v_heads][v blocks]: states behind each part but the last, in the order of the accumulators; then the caller's
                    // old one, where its new one goes to the same place (one part's workgroups may be done before another's begin)
-    float *decays; // [parts - 1][v_heads]: what a part multiplies the state by
+    Power *decays; // [parts - 1][v_heads]: what a part multiplies the state by
     int parts, part_rows, blocks;
 };
 
@@ -419,10 +429,11 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
         total += all;
         if (lane < CH) {
             m.b[buf][lane] = s;
-            m.from[buf][lane] = exp2_of(s);
-            m.to[buf][lane] = exp2_of(all - s);
+            const Power from = power_of(s), to = power_of(all - s);
+            m.from_m[buf][lane] = from.m, m.from_n[buf][lane] = from.n;
+            m.to_m[buf][lane] = to.m, m.to_n[buf][lane] = to.n;
         }
-        if (lane == 0) m.whole[buf] = exp2_of(all);
+        if (lane == 0) m.whole[buf] = power_of(all);
     };
 
     // Registers of the chunk on its way; what lies past the part's last token or a head's last dim is 0. Columns: eight tokens of CW dims of k (whole
@@ -523,10 +534,18 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
             const bool mine = item(u, is_k, grp, col);
             if (wave * 64 + u * CT >= ITEMS) continue; // (uniform)
             if (is_k) { // times their decays to the chunk's end
-                const float4_t w0 = *reinterpret_cast<const float4_t *>(&m.to[buf][grp * 4]);
-                const float4_t w1 = *reinterpret_cast<const float4_t *>(&m.to[buf][16 + grp * 4]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) set_column(u, e, column(u, e) * (e < 4 ? w0[e & 3] : w1[e & 3]));
+                for (int i = 0; i < 2; ++i) {
+                    const float4_t w = *reinterpret_cast<const float4_t *>(&m.to_m[buf][i * 16 + grp * 4]);
+                    const int4_t n = *reinterpret_cast<const int4_t *>(&m.to_n[buf][i * 16 + grp * 4]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        cols_t x = column(u, i * 4 + e) * w[e];
+#pragma unroll
+                        for (int c = 0; c < CW; ++c) x[c] = __builtin_ldexpf(x[c], n[e]);
+                        set_column(u, i * 4 + e, x);
+                    }
+                }
             } else {
                 // a v that is not finite would reach the tokens in front of it through weights of 0: its dim is kept out of the
                 // products and is NaN from that token on
@@ -647,7 +666,8 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
                     const double bi = m.b[buf][i];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float f = exp2_of(bi - b[e]) * d.scale * s[it][e];
+                        const Power w = power_of(bi - b[e]);
+                        float f = __builtin_ldexpf(s[it][e] * (w.m * d.scale), w.n);
                         asm("" : "+v"(f)); // (not under the condition: four waits one after the other)
                         s[it][e] = jt * 16 + g4 * 4 + e <= i ? f : 0.0f;
                     }
@@ -667,7 +687,12 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
                 for (int it = 0; it < 2; ++it) o[it] = products(x, q_operand(it, kk), o[it]);
             }
 #pragma unroll
-            for (int it = 0; it < 2; ++it) o[it] *= m.from[buf][it * 16 + n16] * d.scale;
+            for (int it = 0; it < 2; ++it) {
+                o[it] *= m.from_m[buf][it * 16 + n16] * d.scale;
+                const int n = m.from_n[buf][it * 16 + n16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[it][e] = __builtin_ldexpf(o[it][e], n);
+            }
         }
         {
             const float x = gx;
@@ -702,7 +727,15 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
                 store_cols<VEC>(outs, (unsigned)(i * (d.v_heads * d.v_dim)) * 4u, col0 + col, d.v_dim, o[it]);
             }
         }
-        const float f = any_bad && m.bad[buf][wave * 16 + n16] < CH ? __builtin_nanf("") : m.whole[buf];
+        int n = __builtin_amdgcn_readfirstlane(m.whole[buf].n);
+        if (n < -120 || n > 120) { // (a factor of its own would leave f32)
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[i][e] = __builtin_ldexpf(S[i][e], n);
+            n = 0;
+        }
+        const float f = any_bad && m.bad[buf][wave * 16 + n16] < CH ? __builtin_nanf("") : __builtin_ldexpf(m.whole[buf].m, n);
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
             Operand k;
@@ -724,21 +757,21 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
             for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)S[i][e]), rows, (int)state_byte(i, e), 0, 0);
     } else {
         to_slot(part);
-        if (tid == (W - 1) * 64 && vb == 0) a.decays[(long)part * d.v_heads + h] = exp2_of(total);
+        if (tid == (W - 1) * 64 && vb == 0) a.decays[(long)part * d.v_heads + h] = power_of(total);
     }
 }
 
 // What the parts add, into the states behind them: state_p = decay_p * state_(p - 1) + added_p.
-__global__ __launch_bounds__(256) void linear_scan_kernel(float4_t *slots, const float *decays, int parts, int heads, long per_head, long per_part) {
+__global__ __launch_bounds__(256) void linear_scan_kernel(float4_t *slots, const Power *decays, int parts, int heads, long per_head, long per_part) {
     const long at = (long)blockIdx.x * 256 + threadIdx.x;
     if (at >= per_part) return;
     const int h = (int)(at / per_head);
     float4_t s = slots[at];
     for (int p = 1; p < parts; ++p) {
         const float4_t x = slots[p * per_part + at];
-        const float w = decays[(long)p * heads + h];
+        const Power w = decays[(long)p * heads + h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = w * s[e] + x[e];
+        for (int e = 0; e < 4; ++e) s[e] = __builtin_ldexpf(w.m * s[e], w.n) + x[e];
         slots[p * per_part + at] = s;
     }
 }
@@ -797,7 +830,7 @@ hipError_t launch_linear_chunks(const LinearRows &rows, const LinearParts &p, co
     const int VB = v_block_of(d.v_dim), DK = k_tiles_of(d.k_dim);
     a.blocks = (d.v_dim + VB - 1) / VB;
     a.slots = static_cast<float *>(scratch);
-    a.decays = a.slots + (size_t)p.parts * d.v_heads * a.blocks * DK * VB;
+    a.decays = reinterpret_cast<Power *>(a.slots + (size_t)p.parts * d.v_heads * a.blocks * DK * VB);
     if (VB == 64) {
         switch (DK) {
         case 32: return launch_chunks<32, 4>(a, s);

@@ -8,6 +8,8 @@ torch = pytest.importorskip("torch")
 
 pytestmark = pytest.mark.gpu
 
+GEOMETRIES = [(1, 2, 32, 64), (2, 2, 64, 80), (1, 2, 128, 128), (1, 1, 100, 200), (1, 1, 256, 128), (1, 1, 256, 40)]
+
 
 def _inputs(geo, n, seed):
     kh, vh, dk, dv = geo
@@ -36,6 +38,17 @@ def _check(ctx, geo, q, k, v, g, s, scale=0.25, **how):
     out, new = _run(ctx, geo, q, k, v, g, s, scale)
     close(out, want, tol, "outputs")
     close(new, last, last_tol, "state")
+
+
+@pytest.mark.parametrize("n", [9, 40, 300, 1500])
+@pytest.mark.parametrize("geo", GEOMETRIES)
+def test_single_products(state, geo, n):
+    """One dim of q and one of k a token, so that a sum has few terms: factors of fewer bits than f32's show."""
+    q, k, v, g, s, gen = _inputs(geo, n, n)
+    dk = geo[2]
+    for x, dims in ((k, torch.arange(n) * 5 % dk), (q, torch.randint(dk, (n,), generator=gen))):
+        x *= torch.nn.functional.one_hot(dims, dk)[:, None, :]
+    _check(state, geo, q, k, v, g, s, single=True)
 
 
 @pytest.mark.parametrize("n", [33, 64, 700])
@@ -81,3 +94,20 @@ def test_a_large_row_of_the_state_leaves_the_others_alone(state, geo, n, size):
     g = g * 0.0
     s[:, 9], q[:, :, 9], k[:, :, 9] = s[:, 9] * 2.0 ** size, 0.0, 0.0
     _check(state, geo, q, k, v, g, s)
+
+
+@pytest.mark.parametrize("n,there,back", [(70, (3, 9), (40, 44)), (70, (3, 9), (15, 20)), (700, (130, 140), (300, 310)), (700, (20, 130), (200, 400))])
+@pytest.mark.parametrize("size,growth", [(-100, 55.0), (100, -55.0), (0, -60.0)])
+def test_decays_beyond_what_f32_holds(state, n, there, back, size, growth):
+    """Two tokens together take the state up or down by 2^158 and two others bring it back, within one chunk, from chunk to chunk and
+    from part to part: the states are ordinary numbers all the way, so a factor between two of them may not be infinite or 0."""
+    geo = (1, 2, 64, 80)
+    q, k, v, g, s, _ = _inputs(geo, n, n)
+    for t in there:
+        g[t] = growth
+    for t in back:
+        g[t] = -growth
+    small = 2.0 ** (min(size, 0) / 2 - 10)
+    if growth < 0:  # nothing new: what comes back is what was there
+        k[there[0]:back[1]] = 0.0
+    _check(state, geo, q, k * small, v * small, g, s * 2.0 ** size)
