@@ -444,11 +444,14 @@ int32_t skv_attention_weights_device(skv_layer *layer, skv_stream stream, const 
  * counts positions itself from then on (skv_decode_step_prekv_device takes one), and skv_len is the number of rows.
  * What the rows behind the new length held stays as it was. Until the layer is emptied (skv_truncate to 0, skv_seed, or a
  * prompt restored by skv_hot_match_restore or skv_prompt_cache_get) it can be truncated to no fewer rows than this left it, and skv_hot_remember,
- * skv_hot_remember_range and skv_prompt_cache_put refuse it (SKV_ERR_CONFIG): its rows are no longer a prompt's. Block snapshots copy it
- * as it is. Nothing is waited for; scratch as above (not where few rows can move). keep_rows == len moves nothing. Ring layers: SKV_ERR_CONFIG. */
+ * skv_hot_remember_range and skv_prompt_cache_put refuse it (SKV_ERR_CONFIG): its rows are no longer a prompt's. The mark goes with the
+ * rows: block snapshots copy them as they are and bring it along to where they are restored, and rows that a truncate to more rows than have been written
+ * since the layer was empty brings back have theirs. A captured call does this to the layer when it is captured; a replay changes nothing on the host's
+ * side, and after each the host calls skv_truncate(layer, keep_rows), also where that is its length already, which on such a layer sets the length and the
+ * mark as the call itself does. Nothing is waited for; scratch as above (not where few rows can move). keep_rows == len moves nothing. Ring layers: SKV_ERR_CONFIG. */
 int32_t skv_evict_device(skv_layer *layer, skv_stream stream, float *weights_dev, size_t keep_rows, size_t first_rows,
                          size_t last_rows, int32_t *kept_dev);
-/* keep_rows of the last eviction since the layer was empty, 0 = none. */
+/* keep_rows of the last eviction since the layer was empty (of rows that were restored or came back: those up to the last of them), 0 = none. */
 size_t skv_evicted_rows(const skv_layer *layer);
 
 /* ---- measurement aids (no counterpart in the reference; used by bench.py) ---- */

@@ -1,4 +1,5 @@
 // Host side of eviction by attention weight: argument checks, the scratch, and what an eviction leaves of a layer.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -87,10 +88,18 @@ int32_t skv_evict_device(skv_layer *L, skv_stream stream, float *weights_dev, si
         if (rc) return rc;
     }
     place_evict(a, scratch);
+    const bool leaves = keep_rows < L->len;
+    if (leaves) { // (what may fail for want of memory before anything is queued)
+        mark_moved(L, 0);
+        if (stream_captured(s) && std::find(L->captured_evictions.begin(), L->captured_evictions.end(), keep_rows) == L->captured_evictions.end())
+            L->captured_evictions.push_back(keep_rows);
+    }
     SKV_HIP(launch_evict(a, s));
-    if (keep_rows < L->len) {
+    if (leaves) {
+        L->written = std::max(L->written, L->len);
         L->len = keep_rows;
         L->evicted = keep_rows;
+        mark_moved(L, keep_rows);
     }
     return SKV_OK;
 } catch (...) {

@@ -76,6 +76,9 @@ struct skv_layer {
     size_t window = 0;    // 0 = full cache
     size_t floor_pos = 0; // ring layers: oldest position still held
     size_t evicted = 0;   // rows the last eviction left, no longer in the order of positions (0 = none since the layer was empty)
+    size_t written = 0;   // rows in front that have held the layer's own since it was empty (at least those up to len)
+    std::vector<uint8_t> moved; // logical pages that hold an eviction's rows, whatever the length says (empty = none)
+    std::vector<size_t> captured_evictions; // the lengths that captured evictions leave
     int n_pages = 0;
     uint16_t *k_pool = nullptr;
     uint16_t *v_pool = nullptr;
@@ -94,6 +97,14 @@ struct skv_layer {
     size_t scores_cap = 0;
     std::vector<std::pair<void *, size_t>> leased; // buffers from the context's arena, with their sizes
 };
+
+namespace skv {
+// The mark of an eviction goes with the rows (layer.hip): a layer that is emptied keeps it for the pages that are not written again.
+void mark_moved(skv_layer *L, size_t rows);      // rows [0, rows) are an eviction's
+void layer_emptied(skv_layer *L);                // len and the eviction are forgotten
+void page_filled(skv_layer *L, size_t page, bool moved); // a page's rows have been replaced
+bool stream_captured(hipStream_t s);
+} // namespace skv
 
 // flags.cpp: generation counter of the cached runtime flags
 uint64_t skv_internal_flags_epoch();

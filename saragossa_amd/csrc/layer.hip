@@ -1099,6 +1099,23 @@ int32_t skv::stream_scratch(skv_ctx *ctx, hipStream_t s, size_t need, StreamScra
     return status == 0 ? SKV_OK : scratch_error(status, need, what);
 }
 
+bool skv::stream_captured(hipStream_t s) { return capturing(s); }
+
+void skv::mark_moved(skv_layer *L, size_t rows) {
+    if (L->moved.empty()) L->moved.assign((size_t)L->n_pages, 0);
+    std::fill(L->moved.begin(), L->moved.begin() + (long)std::min((rows + 15) / 16, L->moved.size()), (uint8_t)1);
+}
+void skv::layer_emptied(skv_layer *L) {
+    const size_t own = std::max(L->written, L->len) / 16; // pages written since the layer was empty
+    for (size_t p = 0; p < std::min(own, L->moved.size()); ++p) L->moved[p] = p * 16 < L->evicted;
+    L->len = L->floor_pos = L->evicted = L->written = 0;
+}
+void skv::page_filled(skv_layer *L, size_t page, bool moved) {
+    if (moved && L->moved.empty()) L->moved.assign((size_t)L->n_pages, 0);
+    if (page < L->moved.size()) L->moved[page] = moved;
+    if (moved && page * 16 < L->len) L->evicted = std::max(L->evicted, std::min(L->len, page * 16 + 16));
+}
+
 extern "C" {
 
 const char *skv_last_error(void) { return g_last_error.c_str(); }
@@ -1399,8 +1416,19 @@ int32_t skv_truncate(skv_layer *L, size_t len) try {
     if (len != 0 && len < L->evicted)
         return fail(SKV_ERR_DIMENSION, "truncate KV " + std::to_string(len) + ": une éviction a laissé " + std::to_string(L->evicted) +
                                            " lignes sans ordre");
+    if (len == 0) {
+        layer_emptied(L);
+        return SKV_OK;
+    }
+    L->written = std::max(L->written, L->len);
+    if (len > L->written) // rows that were there before come back, an eviction's with their mark
+        for (size_t p = L->written / 16; p < L->moved.size() && p * 16 < len; ++p)
+            if (L->moved[p]) L->evicted = std::max(L->evicted, std::min(len, p * 16 + 16));
+    if (std::find(L->captured_evictions.begin(), L->captured_evictions.end(), len) != L->captured_evictions.end()) { // a replay's, for all that is known
+        mark_moved(L, len);
+        L->evicted = len;
+    }
     L->len = len;
-    if (len == 0) L->floor_pos = L->evicted = 0;
     return SKV_OK;
 } catch (...) {
     return skv::fail_exception();
@@ -1420,9 +1448,7 @@ int32_t skv_seed(skv_layer *L, const float *keys, const float *values, size_t n_
                                            "), reçu " + std::to_string(n_elems));
     if (n_rows > 0 && (!keys || !values)) return fail(SKV_ERR_DEVICE, "seed: pointeur nul");
     SKV_HIP(hipSetDevice(L->ctx->device));
-    L->len = 0;
-    L->floor_pos = 0;
-    L->evicted = 0;
+    layer_emptied(L);
     if (n_rows == 0) return SKV_OK;
     hipStream_t s = L->ctx->stream;
     // RETI_RUST_KV_BF16_SIM_KONLY / _VONLY (src/decode_resident/attention.rs:573-585): on an

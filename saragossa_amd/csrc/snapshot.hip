@@ -272,6 +272,7 @@ struct skv_snapshot {
     // block snapshots
     SlotLayout layout;
     size_t n_pages = 0;
+    std::vector<uint8_t> moved; // [layers][blocks]: rows that an eviction had put there (empty = none)
     // state snapshots
     std::vector<size_t> sizes;   // bytes of each buffer
     std::vector<size_t> offsets; // 256-byte aligned offsets inside `base`
@@ -342,9 +343,17 @@ int32_t skv_snapshot_blocks(skv_ctx *ctx, skv_stream stream, skv_layer *const *l
         pages[i] = (int32_t)block_ids[i];
         slots[i] = (int32_t)i;
     }
+    std::vector<uint8_t> moved;
+    for (size_t l = 0; l < n_layers; ++l)
+        for (size_t i = 0; i < n_blocks; ++i)
+            if (block_ids[i] * 16 < layers[l]->evicted) {
+                if (moved.empty()) moved.assign(n_layers * n_blocks, 0);
+                moved[l * n_blocks + i] = 1;
+            }
     SKV_HIP(hipSetDevice(ctx->device));
     skv_snapshot *snap = new skv_snapshot();
     snap->ctx = ctx;
+    snap->moved = std::move(moved);
     snap->layout.build(layers, n_layers, n_blocks, true);
     snap->n_pages = n_blocks;
     snap->bytes = n_blocks * snap->layout.slot_bytes;
@@ -395,6 +404,9 @@ int32_t skv_restore_blocks(skv_ctx *ctx, skv_stream stream, const skv_snapshot *
     }
     if (n_blocks == 0) return SKV_OK;
     SKV_HIP(hipSetDevice(ctx->device));
+    for (size_t l = 0; l < n_layers; ++l)
+        if (layers[l]->g.ring_rows == 0)
+            for (size_t i = 0; i < n_blocks; ++i) page_filled(layers[l], dst_block_ids[i], !snap->moved.empty() && snap->moved[l * n_blocks + i]);
     return copy_pages(snap->layout, snap->base, layers, n_layers, pages.data(), slots.data(), n_blocks,
                       nullptr, false, as_stream(stream));
 } catch (...) {
@@ -805,11 +817,7 @@ int32_t skv_hot_match_restore(skv_hot *h, skv_stream stream, const uint8_t root[
     // over rows that are no longer its own.
     auto fail_emptied = [&](int32_t code) {
         if (done_blocks > 0)
-            for (size_t l = 0; l < n_layers; ++l) {
-                layers[l]->len = 0;
-                layers[l]->floor_pos = 0;
-                layers[l]->evicted = 0;
-            }
+            for (size_t l = 0; l < n_layers; ++l) layer_emptied(layers[l]);
         return code;
     };
     for (;;) {
@@ -869,9 +877,9 @@ int32_t skv_hot_match_restore(skv_hot *h, skv_stream stream, const uint8_t root[
     }
     for (size_t l = 0; l < n_layers; ++l) {
         skv_layer *L = layers[l];
+        layer_emptied(L);
         L->len = reused;
         L->floor_pos = (size_t)first_page[l] * 16;
-        L->evicted = 0;
     }
     *reused_tokens = reused;
     if (hash_out) std::memcpy(hash_out, hit.hash, 32);
@@ -1098,9 +1106,9 @@ int32_t skv_prompt_cache_get(skv_prompt_cache *c, skv_stream stream, const uint6
     rc = skv_state_restore(c->ctx, stream, hit.state, state_ptrs, state_bytes, n_states);
     if (rc) return rc;
     for (size_t l = 0; l < n_layers; ++l) {
+        layer_emptied(layers[l]);
         layers[l]->len = cached;
         layers[l]->floor_pos = (size_t)first_page[l] * 16;
-        layers[l]->evicted = 0;
     }
     // the hit becomes the most recent entry (generation.rs:3007-3012)
     if (index > 0) std::rotate(c->entries.begin(), c->entries.begin() + index, c->entries.begin() + index + 1);
