@@ -433,7 +433,8 @@ int32_t skv_gather_device(skv_layer *layer, skv_stream stream, size_t first, siz
  * behind len, are left as they were; a weight is the same whenever the same call is made. Scores are those of f32 queries for
  * up to 64 query heads times rows a kv head, above that (bf16 and 4-bit layers) of queries as two bf16 terms, 2^-16 of
  * themselves. A query with a NaN or an infinity in it, or that meets one among its rows, may give NaN to all rows it sees, and to no other. Async on `stream`, with
- * scratch as a prefill chunk's (above): a capture wants the same call made once before it. At most 2^21 query heads times
+ * scratch as a prefill chunk's (above; some 256 MiB at most, or a single query's scores, 4 bytes a query head and row: more queries are taken in
+ * parts): a capture wants the same call made once before it. At most 2^21 query heads times
  * rows a kv head; weights may not lie over the queries (SKV_ERR_DIMENSION). Ring layers: SKV_ERR_CONFIG. */
 int32_t skv_attention_weights_device(skv_layer *layer, skv_stream stream, const float *q_dev, size_t n_rows, float attn_scalar,
                                      float *weights_dev);

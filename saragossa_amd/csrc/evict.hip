@@ -27,24 +27,28 @@ int32_t skv_attention_weights_device(skv_layer *L, skv_stream stream, const floa
     if (n_rows * (size_t)g.gqa > (size_t)1 << 21) // (the grid of the widest heads' kernel then has 32768 workgroups along its last dimension)
         return fail(SKV_ERR_DIMENSION, "attention weights: trop de requêtes");
     WeightsArgs a{};
-    a.q = q_dev;
     a.k_pool = L->k_pool;
     a.table = L->table_dev;
     a.weights = weights_dev;
     a.stride = (long)L->capacity;
-    a.len = (int)L->len;
-    a.n_queries = (int)n_rows;
-    a.n_slots = (int)(n_rows * (size_t)g.gqa);
     a.qscale = (1.0f / std::sqrt(attn_scalar > 0.0f ? attn_scalar : (float)g.head_dim)) * 1.4426950408889634f;
-    a.rows16 = (int)((L->len + 15) / 16 * 16);
     a.g = g;
-    StreamScratch::Lease lease;
-    void *scratch = nullptr;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const int32_t rc = stream_scratch(L->ctx, s, plan_weights(a), lease, &scratch, "attention weights");
-    if (rc) return rc;
-    place_weights(a, scratch);
-    SKV_HIP(launch_weights(a, s));
+    for (size_t first = 0; first < n_rows;) { // queries whose scratch stays within bounds at a time: those of the last rows but the ones behind them
+        const size_t len = L->len - (n_rows - first), n = weights_at_once(g, len, n_rows - first);
+        a.q = q_dev + first * (size_t)g.q_heads * g.head_dim;
+        a.len = (int)(len + n);
+        a.n_queries = (int)n;
+        a.n_slots = (int)(n * (size_t)g.gqa);
+        a.rows16 = (a.len + 15) / 16 * 16;
+        StreamScratch::Lease lease;
+        void *scratch = nullptr;
+        const int32_t rc = stream_scratch(L->ctx, s, plan_weights(a), lease, &scratch, "attention weights");
+        if (rc) return rc;
+        place_weights(a, scratch);
+        SKV_HIP(launch_weights(a, s));
+        first += n;
+    }
     return SKV_OK;
 } catch (...) {
     return skv::fail_exception();

@@ -668,9 +668,7 @@ __global__ __launch_bounds__(256) void weights_collect_kernel(WeightsArgs a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------
-static bool few_slots(const WeightsArgs &a) {
-    return a.n_slots <= FEW_SLOTS && (size_t)a.g.kv_heads * a.n_slots * a.rows16 <= (size_t)64 << 20; // (256 MiB of scores)
-}
+static bool few_slots(const WeightsArgs &a) { return a.n_slots <= FEW_SLOTS; }
 
 template <int EL, int P>
 static size_t plan_as(WeightsArgs &a) {
@@ -730,6 +728,14 @@ static hipError_t launch_as(const WeightsArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int EL, int P>
+static size_t at_once_as(const Geom &g, size_t before, size_t left) {
+    const size_t kvh = (size_t)g.kv_heads, gqa = (size_t)g.gqa, rows16 = (before + left + 15) / 16 * 16;
+    const size_t per_slot = left * gqa <= FEW_SLOTS ? kvh * rows16 * sizeof(float) : kvh * Many<EL, P>::OPS * 64;
+    const size_t most = (size_t)(left * gqa <= FEW_SLOTS ? 256 : 128) << 20;
+    return std::min(left, std::max<size_t>(most / (per_slot * gqa), 1));
+}
+
 // f<EL, P>(..) of the layer's element and padded head
 #define SKV_WEIGHTS_OF(f, g, ...)                                                                    \
     do {                                                                                             \
@@ -747,6 +753,7 @@ static hipError_t launch_as(const WeightsArgs &a, hipStream_t s) {
     default: return f<EL, 512>(__VA_ARGS__);       \
     }
 
+size_t weights_at_once(const Geom &g, size_t before, size_t left) { SKV_WEIGHTS_OF(at_once_as, g, g, before, left); }
 size_t plan_weights(WeightsArgs &a) { SKV_WEIGHTS_OF(plan_as, a.g, a); }
 void place_weights(WeightsArgs &a, void *scratch) { SKV_WEIGHTS_OF(place_as, a.g, a, static_cast<char *>(scratch)); }
 hipError_t launch_weights(const WeightsArgs &args, hipStream_t s) {

@@ -32,6 +32,9 @@ struct WeightsArgs {
     int sum_splits;
     Geom g;
 };
+// Of the queries of `left` rows behind `before` others as many as one plan_weights takes within 256 MiB of scores (few slots; at least a query's) or
+// 128 MiB of operands
+size_t weights_at_once(const Geom &g, size_t before, size_t left);
 // Fills in how the launches divide their work and returns the scratch bytes they want; place_weights points them at it.
 size_t plan_weights(WeightsArgs &a);
 void place_weights(WeightsArgs &a, void *scratch);
