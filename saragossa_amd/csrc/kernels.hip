@@ -130,7 +130,8 @@ hipError_t launch_probe_empty(hipStream_t s) {
 // tile: rows go out in wide stores, and what the loads leave of a line the same workgroup's other rows take. V's words are four rows of a dim: a thread
 // reads a stretch of them, 128 bytes of bf16 (eight dims and the eight 16 further on), 64 of f32 (four dims), and writes
 // it as four rows. 16384 rows of two heads of 256 dims, 33.5 MB read and as much written: 18.8 us (one dim a store, V's gathered by twos: 54);
-// 2048 of eight heads of 128: 7.3 us (14.1).
+// 2048 of eight heads of 128: 7.3 us (14.1). Heads that are no multiple of 16 bytes write as widely but for their last dims: 8000 rows of three bf16 heads of
+// 100 dims 6.5 us (dim by dim 14), of two of 509 25 (46).
 // ------------------------------------------------------------------------------------
 template <class E, int P>
 struct GatherTile {
@@ -140,21 +141,26 @@ struct GatherTile {
     static constexpr int V_UNITS = P * 16 * (int)sizeof(E) / (16 * STRETCH);
 };
 
-template <class E, bool VEC>
+// 16 bytes of a row in one store, wherever the row begins; what a head has of its last ones (TAIL) one by one
+template <class E>
+struct __attribute__((packed, aligned(sizeof(E)))) Piece {
+    uint32_t x[4];
+};
+template <class E, bool TAIL>
 __device__ __forceinline__ void put_dims(E *row, int d, int head_dim, uint4 x) {
     constexpr int N = 16 / sizeof(E);
-    if (VEC) {
-        if (d < head_dim) *reinterpret_cast<uint4 *>(row + d) = x;
-        return;
-    }
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    if (d + N <= head_dim) {
+        *reinterpret_cast<Piece<E> *>(row + d) = Piece<E>{{x.x, x.y, x.z, x.w}};
+    } else if (TAIL) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (d + e < head_dim) row[d + e] = sizeof(E) == 4 ? (E)w[e & 3] : (E)(w[e >> 1 & 3] >> ((e & 1) * 16));
+        for (int e = 0; e < N - 1; ++e)
+            if (d + e < head_dim) row[d + e] = sizeof(E) == 4 ? (E)w[e & 3] : (E)(w[e >> 1 & 3] >> ((e & 1) * 16));
+    }
 }
 
 // E: the bits of an element
-template <class E, int P, bool VEC>
+template <class E, int P, bool TAIL>
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a, unsigned k_blocks) {
     using T = GatherTile<E, P>;
     const Geom &g = a.g;
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a, unsigned k_bl
     if (!is_v) {
         const int grp = unit % (P / T::PIECE), r = unit / (P / T::PIECE);
         const uint4 x = reinterpret_cast<const uint4 *>(from)[grp * 16 + r];
-        if (out(r)) put_dims<E, VEC>(to + r * kv_dim, grp * T::PIECE, g.head_dim, x);
+        if (out(r)) put_dims<E, TAIL>(to + r * kv_dim, grp * T::PIECE, g.head_dim, x);
         return;
     }
     uint4 x[T::STRETCH];
@@ -194,8 +200,8 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a, unsigned k_bl
                 hi[e] = __builtin_amdgcn_perm(r < 2 ? x[2 * e + 1].z : x[2 * e + 1].w, r < 2 ? x[2 * e].z : x[2 * e].w, sel);
             }
             E *const row = to + (quad * 4 + r) * kv_dim;
-            put_dims<E, VEC>(row, d, g.head_dim, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-            put_dims<E, VEC>(row, d + 16, g.head_dim, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            put_dims<E, TAIL>(row, d, g.head_dim, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            put_dims<E, TAIL>(row, d + 16, g.head_dim, make_uint4(hi[0], hi[1], hi[2], hi[3]));
         }
     } else {
         const int four = unit & 3, blk = unit / 4 % (P / 16), quad = unit / 4 / (P / 16);
@@ -205,7 +211,7 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a, unsigned k_bl
         for (int r = 0; r < 4; ++r) {
             if (!out(quad * 4 + r)) continue;
             const auto word = [&](int i) { return r == 0 ? x[i].x : r == 1 ? x[i].y : r == 2 ? x[i].z : x[i].w; };
-            put_dims<E, VEC>(to + (quad * 4 + r) * kv_dim, blk * 16 + four * 4, g.head_dim, make_uint4(word(0), word(1), word(2), word(3)));
+            put_dims<E, TAIL>(to + (quad * 4 + r) * kv_dim, blk * 16 + four * 4, g.head_dim, make_uint4(word(0), word(1), word(2), word(3)));
         }
     }
 }
@@ -219,10 +225,9 @@ hipError_t gather_as(const GatherArgs &a, hipStream_t s) {
     const long k_blocks = a.k_dst ? (tiles * T::K_UNITS + 255) / 256 : 0, v_blocks = a.v_dst ? (tiles * T::V_UNITS + 255) / 256 : 0;
     if (k_blocks + v_blocks == 0) return hipSuccess;
     if (k_blocks + v_blocks > 0x7fffffffl) return hipErrorInvalidValue;
-    const bool vec = a.g.head_dim % T::PIECE == 0 && (((uintptr_t)a.k_dst | (uintptr_t)a.v_dst) & 15) == 0;
     const dim3 grid((unsigned)(k_blocks + v_blocks));
-    if (vec) hipLaunchKernelGGL((gather_kernel<E, P, true>), grid, dim3(256), 0, s, a, (unsigned)k_blocks);
-    else hipLaunchKernelGGL((gather_kernel<E, P, false>), grid, dim3(256), 0, s, a, (unsigned)k_blocks);
+    if (a.g.head_dim % T::PIECE == 0) hipLaunchKernelGGL((gather_kernel<E, P, false>), grid, dim3(256), 0, s, a, (unsigned)k_blocks);
+    else hipLaunchKernelGGL((gather_kernel<E, P, true>), grid, dim3(256), 0, s, a, (unsigned)k_blocks);
     return hipGetLastError();
 }
 template <class E>
