@@ -282,10 +282,10 @@ struct Half {
 };
 struct Operand {
     uint4 x[TERMS];
-    __device__ __forceinline__ Half half(int i) const {
+    __device__ __forceinline__ Half first() const {
         Half h;
 #pragma unroll
-        for (int p = 0; p < TERMS; ++p) h.x[p] = i == 0 ? make_uint2(x[p].x, x[p].y) : make_uint2(x[p].z, x[p].w);
+        for (int p = 0; p < TERMS; ++p) h.x[p] = make_uint2(x[p].x, x[p].y);
         return h;
     }
 };
@@ -649,6 +649,8 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
         if (tid == 0) m.any_bad[buf ^ 1] = 0;
         const bool any_bad = m.any_bad[buf] != 0;
         float4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if (wave == W - 1 && c0 + CH < t1) decays(c0 + CH, buf ^ 1, gx);
+        gx = decay(c0 + 2 * CH);
         if constexpr (OUT) {
             if (scorer) { // both tiles of its keys, as weights into LDS
                 float4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -694,12 +696,7 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
                 for (int e = 0; e < 4; ++e) o[it][e] = __builtin_ldexpf(o[it][e], n);
             }
         }
-        {
-            const float x = gx;
-            gx = decay(c0 + 2 * CH);
-            fetch(min(c0 + CH, last_chunk));
-            if (wave == W - 1 && c0 + CH < t1) decays(c0 + CH, buf ^ 1, x);
-        }
+        fetch(min(c0 + CH, last_chunk));
         if constexpr (OUT) __syncthreads(); // the weights
         Operand v;
 #pragma unroll
@@ -710,15 +707,20 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
                 const int i = it * 16 + n16;
-                float4_t add = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j <= it; ++j) {
+                if (it == 0) { // (sees the first 16 alone)
                     Half w;
 #pragma unroll
-                    for (int p = 0; p < TERMS; ++p) w.x[p] = m.p[p][it + j][lane];
-                    add = products(v.half(j), w, add);
+                    for (int p = 0; p < TERMS; ++p) w.x[p] = m.p[p][0][lane];
+                    o[it] += products(v.first(), w, float4_t{0.f, 0.f, 0.f, 0.f});
+                } else {
+                    Operand w;
+#pragma unroll
+                    for (int p = 0; p < TERMS; ++p) {
+                        const uint2 x = m.p[p][1][lane], y = m.p[p][2][lane];
+                        w.x[p] = make_uint4(x.x, x.y, y.x, y.y);
+                    }
+                    o[it] += products(v, w, float4_t{0.f, 0.f, 0.f, 0.f});
                 }
-                o[it] += add;
                 if (any_bad) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
