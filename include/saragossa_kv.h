@@ -504,14 +504,14 @@ int32_t skv_state_snapshot(skv_ctx *ctx, skv_stream stream, const void *const *d
 int32_t skv_state_restore(skv_ctx *ctx, skv_stream stream, const skv_snapshot *snapshot,
                           void *const *dev_ptrs, const size_t *bytes, size_t n);
 
-/* ---- linear attention with a decay: the other layers of a hybrid model ------------------------- */
+/* ---- linear attention with a decay: layers that keep a state in place of rows ------------------ */
 
 /* What such a layer keeps of its context is a state S [k_dim][v_dim] per v head, f32, in place of rows: v head h reads q and
  * k of head h / (v_heads / k_heads), and token t makes of them
  *
  *   S_t = exp(g_t) S_(t-1) + k_t v_t^T,      o_t = scale * S_t^T q_t
  *
- * (the recurrence without the delta rule of src/linear_attention.rs, whose layers' states these shapes are). The states are the
+ * (for models with a plain decay; the gated delta rule of src/linear_attention.rs, whose states have these shapes, is not computed). The states are the
  * caller's device buffers of skv_linear_state_bytes, [v_heads][k_dim][v_dim], 4-byte aligned (16-byte aligned ones are read and
  * written faster), what skv_state_snapshot, skv_hot_* and skv_prompt_cache_* copy as state_ptrs (16-byte aligned there). A handle is
  * the geometry alone and holds no device memory; heads of 1 to 256 dims, v_heads a multiple of k_heads (SKV_ERR_CONFIG). */

@@ -21,7 +21,8 @@ namespace skv {
 // r >= keep that stays is mover S(r) - S(keep).
 //
 // Bound by the chain of passes and by what a CU alone brings in, not by bytes: 2000 rows of two heads 6.6 us, 8000 10.3, 16000 18;
-// 32768 18.5 and 4.7 for the counts, where one workgroup a head took 64.
+// 32768 18.5 and 4.7 for the counts, where one workgroup a head took 64. Beyond, every workgroup reads all weights anew in each pass: half of 32768 rows of two
+// heads of 256 dims leave in 39 us with their moves, of 32769 in 56, of 65536 in 96, of 131072 in 210.
 // ------------------------------------------------------------------------------------
 static_assert(sizeof(Mover) == 3 * sizeof(int32_t), "as scratch is counted");
 constexpr int SEL_THREADS = 1024, SEL_WAVES = SEL_THREADS / 64, BINS = 2048, STRETCHES = 8, STRETCH = 4096, CHOSEN = 16 * SEL_THREADS;
