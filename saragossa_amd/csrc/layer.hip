@@ -1387,6 +1387,12 @@ int32_t skv_layer_set_block_table(skv_layer *L, const int32_t *table, size_t n) 
         seen[table[i]] = 1;
     }
     SKV_HIP(hipSetDevice(L->ctx->device));
+    if (!L->moved.empty()) { // the marks go with the pages
+        std::vector<uint8_t> of_page(n), moved(n);
+        for (size_t i = 0; i < n; ++i) of_page[(size_t)L->table[i]] = L->moved[i];
+        for (size_t i = 0; i < n; ++i) moved[i] = of_page[(size_t)table[i]];
+        L->moved.swap(moved);
+    }
     L->table.assign(table, table + n);
     SKV_HIP(hipMemcpyAsync(L->table_dev, L->table.data(), n * sizeof(int32_t), hipMemcpyHostToDevice,
                            L->ctx->stream));

@@ -345,7 +345,7 @@ int32_t skv_snapshot_blocks(skv_ctx *ctx, skv_stream stream, skv_layer *const *l
     }
     std::vector<uint8_t> moved;
     for (size_t l = 0; l < n_layers; ++l)
-        for (size_t i = 0; i < n_blocks; ++i)
+        for (size_t i = 0; layers[l]->evicted > 0 && i < n_blocks; ++i)
             if (block_ids[i] * 16 < layers[l]->evicted) {
                 if (moved.empty()) moved.assign(n_layers * n_blocks, 0);
                 moved[l * n_blocks + i] = 1;
@@ -405,7 +405,7 @@ int32_t skv_restore_blocks(skv_ctx *ctx, skv_stream stream, const skv_snapshot *
     if (n_blocks == 0) return SKV_OK;
     SKV_HIP(hipSetDevice(ctx->device));
     for (size_t l = 0; l < n_layers; ++l)
-        if (layers[l]->g.ring_rows == 0)
+        if (layers[l]->g.ring_rows == 0 && !(snap->moved.empty() && layers[l]->moved.empty()))
             for (size_t i = 0; i < n_blocks; ++i) page_filled(layers[l], dst_block_ids[i], !snap->moved.empty() && snap->moved[l * n_blocks + i]);
     return copy_pages(snap->layout, snap->base, layers, n_layers, pages.data(), slots.data(), n_blocks,
                       nullptr, false, as_stream(stream));

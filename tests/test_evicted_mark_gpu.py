@@ -170,3 +170,15 @@ def test_a_replayed_eviction(state, steady):
             _refused(state, kv)
             with pytest.raises(skv.DimensionError):
                 kv.truncate(39)
+
+
+def test_a_new_block_table_takes_the_mark_along(state):
+    kv, w = _layer(state)
+    _evict(kv, w, 20)  # pages 0 and 1 of eight
+    kv.truncate(0)
+    kv.set_block_table(np.array([2, 3, 4, 5, 6, 1, 7, 0], np.int32))
+    kv.truncate(80)
+    assert kv.evicted_rows() == 0
+    kv.truncate(96)
+    assert kv.evicted_rows() == 96
+    _refused(state, kv)
