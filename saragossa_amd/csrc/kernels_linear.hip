@@ -637,7 +637,7 @@ __global__ __launch_bounds__(W * 64, linear_occupancy(DK, W, OUT)) void linear_c
         const auto outs = rows_left(r.out, 1, 0, d.v_dim);
         const float x = __int_as_float(tid);
 #pragma unroll
-        for (int it = 0; it < 2; ++it) store_cols<VEC>(outs, OUTSIDE, 0, d.v_dim, float4_t{x, x, x, x});
+        for (int it = 0; it < 2; ++it) store_cols<VEC>(outs, 0, NO_COLUMN, d.v_dim, float4_t{x, x, x, x});
     }
     __syncthreads();
     int buf = 0;
